@@ -545,6 +545,150 @@ int ks_b200_import_ggml_q4_0_async(const void *blocks, size_t block_row_stride,
                                    void *weight_scales, int scale_type,
                                    size_t scale_stride, void *stream);
 
+/*
+ * The paged 4-bit key/value cache and the attention that reads it (no
+ * counterpart in the reference).  Keys and values of each token and key/value
+ * head are held as signed int4 codes with f16 group scales:
+ *   scale = max(max(v, 0) / 7, -min(v, 0) / 8) rounded to f16, kept within the
+ *           positive finite f16 values, 1 if the group is all zeros
+ *   code  = clamp(round_half_even(v / scale), -8, 7),  value = code * scale
+ * (the rule of ks_b200_import_ggml_q4_0_async with f16 scales).
+ *
+ * A pool is n_pages pages of page_size tokens, ks_b200_kv4_page_bytes bytes
+ * each, [kv_heads][page_size / 16][block].  A block is 16 tokens of one head:
+ * key codes [16][head_dim / 2], key scales f16 [16][head_dim / group_size],
+ * then value codes and value scales likewise.  A byte holds elements d
+ * (even, low nibble) and d + 1; in its row it is byte
+ *   keys    ((d % 32) / 8) * (head_dim / 8) + (d / 32) * 4 + (d % 8) / 2
+ *   values  ((d % 16) / 2) * (head_dim / 16) + d / 16.
+ * weights, if not NULL, holds one f32 per token and head,
+ * [n_pages][kv_heads][page_size]: the attention weight the token has
+ * received, which ks_b200_kv4_evict_async goes by.
+ *
+ * Sequences.  All calls describe their sequences alike: token p of sequence s
+ * is slot p % page_size of page page_table[s * page_table_stride + p /
+ * page_size]; seq_lens[s] counts the sequence's cached tokens, its newest ones
+ * included; the newest are rows token_offsets[s] .. token_offsets[s + 1] - 1
+ * of the packed [n_tokens] tensors of keys, values, queries and outputs, in
+ * order (token_offsets NULL: one row each, row s).  page_table, seq_lens and
+ * token_offsets are int32 device memory, read when the call runs, so a
+ * captured graph follows them.  Table entries past a sequence's tokens are not
+ * read.  Rows below token_offsets[0] or from token_offsets[n_seqs] on are left
+ * as they are.  Tensors are [n_tokens][heads][head_dim] with strides in
+ * elements, the last dimension contiguous, of type KS_B200_DTYPE_*.
+ *
+ * Device pointers, queued on `stream`, no allocation, capturable.  status
+ * word 0 becomes 1 if the device finds a length beyond the table (or
+ * max_len), a page outside the pool, offsets outside n_tokens, more new
+ * tokens than the sequence has or a key or value that is not finite (stored
+ * as 0 if NaN, else as the largest code): no call reads or writes outside
+ * its buffers then, the sequences concerned are unspecified.
+ * head_dim must be 64 or 128, group_size 32, 64 or 128 and at most head_dim,
+ * page_size 16, 32, 64, 128 or 256, else KS_ERR_UNSUPPORTED.
+ */
+#define KS_B200_DTYPE_F32 0
+#define KS_B200_DTYPE_F16 1
+#define KS_B200_DTYPE_BF16 2
+
+typedef struct ks_b200_kv4_cache {
+  void *pool;        /* device, 16-byte aligned */
+  float *weights;    /* device, or NULL */
+  size_t n_pages, page_size, kv_heads, head_dim, group_size;
+} ks_b200_kv4_cache;
+
+/* Bytes of one page (0 for an unsupported shape). */
+size_t ks_b200_kv4_page_bytes(size_t page_size, size_t kv_heads,
+                              size_t head_dim, size_t group_size);
+
+/*
+ * Quantise the newest tokens of each sequence into the cache: rows i of k and
+ * v become tokens seq_lens[s] - (token_offsets[s + 1] - token_offsets[s]) ..
+ * seq_lens[s] - 1.  Their accumulated weights, if kept, become 0.  A slot may
+ * be written by one row of the call.
+ */
+int ks_b200_kv4_append_async(const ks_b200_kv4_cache *cache,
+                             const int32_t *page_table, size_t page_table_stride,
+                             const int32_t *seq_lens, const int32_t *token_offsets,
+                             size_t n_seqs, size_t n_tokens, const void *k,
+                             size_t k_token_stride, size_t k_head_stride,
+                             const void *v, size_t v_token_stride,
+                             size_t v_head_stride, int dtype,
+                             uint32_t *status, void *stream);
+
+/*
+ * The reverse: the newest tokens of each sequence (all of them, where
+ * token_offsets counts as many as seq_lens) as code * scale, rounded once to
+ * the type.
+ */
+int ks_b200_kv4_read_async(const ks_b200_kv4_cache *cache,
+                           const int32_t *page_table, size_t page_table_stride,
+                           const int32_t *seq_lens, const int32_t *token_offsets,
+                           size_t n_seqs, size_t n_tokens, void *k,
+                           size_t k_token_stride, size_t k_head_stride, void *v,
+                           size_t v_token_stride, size_t v_head_stride,
+                           int dtype, uint32_t *status, void *stream);
+
+/*
+ * Attention of the newest tokens over the cache, causal among them: with n
+ * new tokens, the j-th sees positions 0 .. seq_lens[s] - n + j, and query head
+ * h reads key/value head h / (q_heads / kv_heads):
+ *   out = sum_t exp(scale * q . k_t - lse) v_t,  lse = log sum_t exp(scale * q . k_t).
+ * A row that sees nothing gets zeros and lse -inf.  Sums are f32; for f32
+ * tensors the products keep 22 bits of queries and probabilities, so results
+ * agree with f32 arithmetic; queries are finite and below 2^110.  lse: f32
+ * [n_tokens][q_heads], or NULL.  accumulate != 0 adds to cache->weights of
+ * every cached token the attention weight it received, summed over the
+ * sequence's new tokens and the query heads of its key/value head, in a fixed
+ * order; then lse may not be NULL, and no page may belong to two sequences of
+ * the call (without it, sequences may share pages).
+ * max_new and max_len bound the new and the cached tokens of any sequence
+ * (max_new <= max_len <= page_table_stride * page_size): they size the launch.
+ * out may not overlap q.  workspace: device memory, 16-byte aligned,
+ * ks_b200_kv4_attention_workspace(...) bytes for these sizes, not shared by
+ * calls that may run at the same time (two graphs that replay at the same time
+ * need one each); its contents do not matter.
+ */
+size_t ks_b200_kv4_attention_workspace(const ks_b200_kv4_cache *cache,
+                                       size_t q_heads, size_t n_seqs,
+                                       size_t n_tokens, size_t max_new,
+                                       size_t max_len);
+int ks_b200_kv4_attention_async(const ks_b200_kv4_cache *cache,
+                                const int32_t *page_table, size_t page_table_stride,
+                                const int32_t *seq_lens, const int32_t *token_offsets,
+                                size_t n_seqs, size_t n_tokens, size_t max_new,
+                                size_t max_len, const void *q,
+                                size_t q_token_stride, size_t q_head_stride,
+                                size_t q_heads, float scale, void *out,
+                                size_t out_token_stride, size_t out_head_stride,
+                                int dtype, float *lse, int accumulate,
+                                void *workspace, size_t workspace_bytes,
+                                uint32_t *status, void *stream);
+
+/*
+ * Evict by accumulated attention weight (cache->weights, not NULL).  A
+ * sequence of at most `budget` tokens keeps all; of a longer one every head
+ * keeps its newest `recent` tokens (recent <= budget) and, of the older ones,
+ * the budget - recent with the largest weight, the lower position first among
+ * equal ones (a NaN weight is below all).  Heads may keep different tokens.
+ * What is kept moves, in order and with its weights, to positions 0, 1, ... of
+ * the pages that to_table names, and to_lens[s] becomes min(seq_lens[s],
+ * budget); to_lens may be seq_lens.  The pages of to_table must be other
+ * pages than those that hold the sequences, which keep their contents and are
+ * free for other use afterwards.  kept: int32 [n_seqs][kv_heads][budget], or
+ * NULL: the old position of each kept token; entries past a sequence's kept
+ * tokens are left as they are.  max_len bounds the sequences' lengths.
+ * workspace as for the attention.
+ */
+size_t ks_b200_kv4_evict_workspace(const ks_b200_kv4_cache *cache, size_t n_seqs,
+                                   size_t max_len, size_t budget);
+int ks_b200_kv4_evict_async(const ks_b200_kv4_cache *cache,
+                            const int32_t *page_table, size_t page_table_stride,
+                            const int32_t *seq_lens, size_t n_seqs, size_t max_len,
+                            const int32_t *to_table, size_t to_table_stride,
+                            int32_t *to_lens, size_t budget, size_t recent,
+                            int32_t *kept, void *workspace, size_t workspace_bytes,
+                            uint32_t *status, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

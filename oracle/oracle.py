@@ -325,3 +325,69 @@ def q4_0_encode(values: np.ndarray, rng_: np.random.Generator | None = None) -> 
     out[:, :, 0:2] = d.view(np.uint8).reshape(rows, nb, 2)
     out[:, :, 2:] = qs
     return out.reshape(rows, nb * Q4_0_BLOCK_BYTES)
+
+
+# ---- the paged 4-bit key/value cache, in 64 bits --------------------------
+def kv4_quantize(x: np.ndarray, group: int):
+    """x [..., head_dim] -> (codes int8 [..., head_dim], scales f16 [..., head_dim / group]) by the cache's rule, every
+    rounding decided by the exact quotient (f64; f16 and small integers divide far from its own rounding)."""
+    v = np.asarray(x, np.float64)
+    v = np.where(np.isnan(v), 0.0, v).reshape(*v.shape[:-1], -1, group)
+    hi, lo = np.maximum(v.max(-1), 0), np.minimum(v.min(-1), 0)
+    s = np.maximum(hi / 7, -lo / 8)
+    scale = np.where(s == 0, 1.0, np.clip(s, 2.0**-24, 65504.0)).astype(np.float16)
+    with np.errstate(over="ignore"):
+        q = np.clip(np.rint(v / scale.astype(np.float64)[..., None]), -8, 7)
+    return q.astype(np.int8).reshape(x.shape), scale
+
+
+def kv4_value(codes: np.ndarray, scale: np.ndarray) -> np.ndarray:
+    group = codes.shape[-1] // scale.shape[-1]
+    return codes.astype(np.float64) * np.repeat(scale.astype(np.float64), group, axis=-1)
+
+
+def kv4_byte(head_dim: int, values: bool) -> np.ndarray:
+    """The byte of each element's pair in a token's row of codes."""
+    d = np.arange(head_dim)
+    if values:
+        return (d % 16) // 2 * (head_dim // 16) + d // 16
+    return (d % 32) // 8 * (head_dim // 8) + d // 32 * 4 + d % 8 // 2
+
+
+def kv4_pool(k, v, group: int) -> np.ndarray:
+    """Pool bytes [pages, heads, page_size / 16, block] of keys and values [pages, heads, page_size, head_dim]."""
+    parts = []
+    for x, values in ((k, False), (v, True)):
+        pages, heads, page, d = x.shape
+        codes, scale = kv4_quantize(x, group)
+        rows = np.zeros((pages, heads, page // 16, 16, d // 2), np.uint8)
+        q = (codes.reshape(pages, heads, page // 16, 16, d) & 15).astype(np.uint8)
+        at = kv4_byte(d, values)
+        rows[..., at[::2]] = q[..., ::2] | (q[..., 1::2] << 4)
+        parts.append(rows.reshape(pages, heads, page // 16, -1))
+        parts.append(np.ascontiguousarray(scale.reshape(pages, heads, page // 16, -1)).view(np.uint8))
+    return np.concatenate(parts, axis=-1)
+
+
+def kv4_attention(q, k, v, scale: float, n_new: int):
+    """One sequence: q [n_new, q_heads, d], cached k, v [len, kv_heads, d], all f64.  Returns out, lse, the weight of
+    every cached token [kv_heads, len], and for each row sum_t p |v| and max_t sum_d |q k| (for error bounds)."""
+    length, heads, d = k.shape
+    group = q.shape[1] // heads
+    out, lse = np.zeros(q.shape), np.full(q.shape[:2], -np.inf)
+    size, dots = np.zeros(q.shape), np.zeros(q.shape[:2])
+    weight = np.zeros((heads, length))
+    for j in range(n_new):
+        seen = min(max(length - n_new + j + 1, 0), length)
+        if seen == 0:
+            continue
+        for h in range(q.shape[1]):
+            kk, vv = k[:seen, h // group], v[:seen, h // group]
+            x = kk @ q[j, h] * scale
+            lse[j, h] = x.max() + np.log(np.exp(x - x.max()).sum())
+            p = np.exp(x - lse[j, h])
+            out[j, h] = p @ vv
+            size[j, h] = p @ np.abs(vv)
+            dots[j, h] = abs(scale) * (np.abs(kk) @ np.abs(q[j, h])).max()
+            weight[h // group, :seen] += p
+    return out, lse, weight, size, dots

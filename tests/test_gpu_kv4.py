@@ -1,0 +1,653 @@
+"""The paged 4-bit key/value cache on the GPU against its definition in 64 bits (oracle.kv4_*): append and read bit
+for bit, attention within bounds that follow from its roundings, eviction exactly."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+import oracle as O
+
+pytestmark = pytest.mark.gpu
+
+TYPES = ["f32", "f16", "bf16"]
+
+
+def _type(name):
+    import torch
+
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[name]
+
+
+class Seqs:
+    """A cache on the GPU with random contents, its sequences, and the same keys and values in f64."""
+
+    def __init__(self, ks, cuda, lens, news, heads, d, group, page, seed=0, weights=False, spare=2, garbage=True,
+                 table_slack=1):
+        import torch
+
+        rng = np.random.default_rng(seed)
+        self.ks, self.cuda, self.rng = ks, cuda, rng
+        self.lens, self.news, self.heads, self.d, self.group, self.page = list(lens), list(news), heads, d, group, page
+        each = [-(-x // page) for x in lens]
+        self.n_pages = sum(each) + spare
+        channel = 1 + 3 * (rng.random((heads, 1, d)) < 0.06)
+        k = rng.standard_normal((self.n_pages, heads, page, d)) * channel
+        v = rng.standard_normal((self.n_pages, heads, page, d)) * np.exp(rng.standard_normal((self.n_pages, heads,
+                                                                                              page, 1)))
+        self.k = O.kv4_value(*O.kv4_quantize(k, group))
+        self.v = O.kv4_value(*O.kv4_quantize(v, group))
+        self.scale_max = O.kv4_quantize(k, group)[1].astype(np.float64).max()
+        pool = O.kv4_pool(k, v, group)
+        ids = rng.permutation(self.n_pages)
+        self.pages, at = [], 0
+        self.table_np = np.full((len(lens), max(each + [1]) + table_slack), -1, np.int32)
+        for s, n in enumerate(each):
+            self.pages.append(ids[at:at + n])
+            self.table_np[s, :n] = ids[at:at + n]
+            at += n
+        if garbage:  # slots that no token stands in hold anything, NaN scales among it
+            used = np.zeros((self.n_pages, page), bool)
+            for s, n in enumerate(lens):
+                for i, p in enumerate(self.pages[s]):
+                    used[p, : min(page, n - i * page)] = True
+            half, codes, per = pool.shape[-1] // 2, 8 * d, 2 * (d // group)
+            p, slot = np.nonzero(~used)
+            for h in (0, half):
+                for b in range(per):
+                    pool[p, :, slot // 16, h + codes + (slot % 16) * per + b] = 0xFF
+        self.pool = torch.from_numpy(pool).to(cuda)
+        self.table = torch.from_numpy(self.table_np).to(cuda)
+        self.seq_lens = torch.tensor(lens, dtype=torch.int32, device=cuda)
+        self.first = np.concatenate([[0], np.cumsum(news)]).astype(int)
+        self.tokens = int(self.first[-1])
+        self.offsets = torch.tensor(self.first, dtype=torch.int32, device=cuda)
+        self.w = None
+        if weights:
+            self.w = torch.from_numpy(rng.random((self.n_pages, heads, page)).astype(np.float32)).to(cuda)
+        self.cache = ks.Kv4Cache(self.pool, self.n_pages, page, heads, d, group, weights=self.w)
+        self.status = torch.zeros(2, dtype=torch.int32, device=cuda)
+
+    def cached(self, s, which):
+        """Keys or values of sequence s, [len, heads, d]."""
+        x = (self.k if which == "k" else self.v)[self.pages[s]]
+        return x.transpose(0, 2, 1, 3).reshape(-1, self.heads, self.d)[: self.lens[s]]
+
+    def weights_of(self, s, w):
+        return w[self.pages[s]].transpose(1, 0, 2).reshape(self.heads, -1)[:, : self.lens[s]]
+
+    def ok(self):
+        import torch
+
+        torch.cuda.synchronize()
+        assert self.status.cpu().tolist() == [0, 0]
+
+
+def _query(c, heads, dtype, seed=1, size=1.5):
+    import torch
+
+    q = torch.from_numpy(np.random.default_rng(seed).standard_normal((c.tokens, heads, c.d)) * size)
+    return q.to(_type(dtype)).to(c.cuda)
+
+
+def _attend(c, q, scale, out=None, lse=True, max_new=None, max_len=None, accumulate=False, offsets=True, stream=None):
+    import torch
+
+    out = torch.full_like(q, float("nan")) if out is None else out
+    lse = torch.full(q.shape[:2], float("nan"), device=c.cuda) if lse is True else lse
+    max_new = max(c.news + [1]) if max_new is None else max_new
+    max_len = max(c.lens + [max_new]) if max_len is None else max_len
+    need = c.ks.kv4_attention_workspace(c.cache, q.shape[1], len(c.lens), c.tokens, max_new, max_len)
+    ws = torch.full((max(need, 16),), 255, dtype=torch.uint8, device=c.cuda)  # NaN: nothing may be taken from it
+    c.ks.kv4_attention_async(c.cache, c.table, c.seq_lens, q, out, scale, ws,
+                             token_offsets=c.offsets if offsets else None, max_new=max_new, max_len=max_len,
+                             lse=lse, accumulate=accumulate, status=c.status, stream=stream)
+    return out, lse
+
+
+def _check(c, q, scale, out, lse, dtype, weights=None, before=None):
+    """Bounds.  A score is a sum of products code * q, exact in f32, over up to 2 x 8 tensor-core steps of at most
+    2^-23 of the largest partial sum (15 + 8 times sum |q| and the scale: codes are taken from 0 to 15, from -8
+    sum(q)), and of some six more roundings: |dx| <= 22 * 23 * 2^-23 * scale * s_max * sum |q| <= E.  A probability is
+    then within 2 E + 2^-18 (exponentials, sums, the two parts) relatively, 2^-11 more in one f16 part (bf16 results),
+    and the result is rounded once."""
+    import torch
+
+    half = torch.finfo(_type(dtype)).eps / 2
+    out, lse, qn = out.double().cpu().numpy(), lse.double().cpu().numpy(), q.double().cpu().numpy()
+    err = norm = top = 0.0
+    for s in range(len(c.lens)):
+        a, n = c.first[s], c.news[s]
+        want, z, w, size, _ = O.kv4_attention(qn[a:a + n], c.cached(s, "k"), c.cached(s, "v"), scale, n)
+        e = 512 * 2.0**-23 * abs(scale) * c.scale_max * np.abs(qn[a:a + n]).sum(-1)  # [n, heads]
+        rel = 2 * e + 2.0**-18 + (2.0**-11 if dtype == "bf16" else 0)
+        tol = half * np.abs(want) + rel[..., None] * size + 2.0**-24
+        bad = ~(np.abs(out[a:a + n] - want) <= tol)
+        assert not bad.any(), (s, np.argwhere(bad)[:5], out[a:a + n][bad][:5], want[bad][:5])
+        empty = np.isinf(z)
+        assert (np.isneginf(lse[a:a + n]) == empty).all() and (out[a:a + n][empty] == 0).all()
+        with np.errstate(invalid="ignore"):
+            assert (empty | (np.abs(lse[a:a + n] - z) <= e + 2.0**-20 + 2.0**-22 * np.abs(z))).all()
+        top = max([top] + np.abs(z[~empty]).tolist())
+        err, norm = err + ((out[a:a + n] - want) ** 2).sum(), norm + (want**2).sum()
+        if weights is not None:
+            got = c.weights_of(s, weights.double().cpu().numpy())
+            old = c.weights_of(s, before)
+            # f32 sums of the rows' weights, each within 2 E + 2^-18
+            worst = 2 * e.max() + 2.0**-18 if n else 0.0
+            assert (np.abs(got - old - w) <= worst * w + 2.0**-23 * (old + w) * (1 + n)).all(), s
+    # The products' roundings are independent, far below their worst case.  What does not average out: the score x (in
+    # units of log2, rounded to f32 four times: scale * log2(e), the row's factor, the product with it, the difference
+    # to the maximum) is off by up to 4 * 2^-24 |x|, so the probabilities by 2^-22 |x| relatively and, divided by their
+    # sum, by twice that; |x| is about |lse| where it matters (at x = 66, 3e-5).
+    most = half + 2.0**-17 + 2.0**-21 * top + (2.0**-12 if dtype == "bf16" else 0)
+    assert err**0.5 <= most * norm**0.5 + 1e-30
+
+
+# ------------------------------------------------------------------ append, read
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("page,heads", [(16, 3), (64, 8), (256, 33)])
+def test_append_and_read(ks, cuda, dtype, d, group, page, heads):
+    import torch
+
+    lens, news = [1, page + 5, 40, 0, 2 * page], [1, 7, 40, 0, 1]
+    c = Seqs(ks, cuda, lens, news, heads, d, group, page, seed=d + group + page, weights=True, garbage=False)
+    rng = np.random.default_rng(9)
+    x = torch.from_numpy(rng.standard_normal((2, c.tokens + 2, heads, d)) * np.exp(2 * rng.standard_normal(
+        (2, c.tokens + 2, heads, 1)))).to(_type(dtype)).to(cuda)
+    x[0, 0, 0, :group] = 0
+    before, wbefore = c.pool.clone(), c.w.clone()
+    ks.kv4_append_async(c.cache, c.table, c.seq_lens, x[0], x[1], token_offsets=c.offsets, status=c.status)
+    k, v = torch.full_like(x[0], 7), torch.full_like(x[0], 7)
+    ks.kv4_read_async(c.cache, c.table, c.seq_lens, k, v, token_offsets=c.offsets, status=c.status)
+    c.ok()
+    # rows behind the last sequence are left
+    assert (k[c.tokens:] == 7).all() and (v[c.tokens:] == 7).all()
+    want = before.cpu().numpy()
+    wwant = wbefore.cpu().numpy()
+    for values, got in ((0, k), (1, v)):
+        codes, scale = O.kv4_quantize(x[values].double().cpu().numpy(), group)
+        value = torch.from_numpy(O.kv4_value(codes, scale)).to(_type(dtype))
+        assert torch.equal(got[: c.tokens].cpu(), value[: c.tokens])
+        at, half = O.kv4_byte(d, bool(values)), want.shape[-1] // 2 * values
+        for s in range(len(lens)):
+            for j in range(news[s]):
+                pos, i = lens[s] - news[s] + j, c.first[s] + j
+                p, slot = c.pages[s][pos // page], pos % page
+                q = (codes[i] & 15).astype(np.uint8)
+                row = want[p, :, slot // 16]
+                row[:, half + slot % 16 * (d // 2) + at[::2]] = q[:, ::2] | (q[:, 1::2] << 4)
+                per = 2 * (d // group)
+                o = half + 8 * d + slot % 16 * per
+                row[:, o:o + per] = np.ascontiguousarray(scale[i]).view(np.uint8)
+                wwant[p, :, slot] = 0
+    assert (c.pool.cpu().numpy() == want).all()
+    assert (c.w.cpu().numpy() == wwant).all()
+
+
+def test_append_ties_and_strides(ks, cuda):
+    """Quotients on and next to a tie, decided by the exact quotient; strided and unaligned rows."""
+    import torch
+
+    heads, d, group = 2, 64, 32
+    c = Seqs(ks, cuda, [20], [20], heads, d, group, 32, garbage=False)
+    rng = np.random.default_rng(3)
+    x = np.zeros((20, heads, d), np.float32)
+    scale = np.float16(np.exp(rng.standard_normal((20, heads, 2)))).astype(np.float32)
+    tie = (rng.integers(-8, 7, (20, heads, 2, group)) + 0.5).astype(np.float32) * scale[..., None]
+    tie = np.nextafter(tie, np.where(rng.random(tie.shape) < 0.5, np.inf, -np.inf).astype(np.float32)) \
+        * (rng.random(tie.shape) < 0.7) + tie * (rng.random(tie.shape) < 0.2)
+    tie[..., 0] = 7 * scale  # the group's scale, exactly
+    tie = np.clip(tie, -8 * scale[..., None], 7 * scale[..., None])
+    x[:] = tie.reshape(20, heads, d)
+    big = torch.zeros(20 * (heads * d + 3) + 1, device=cuda)
+    k = big[1:].as_strided((20, heads, d), (heads * d + 3, d, 1))  # 4-byte aligned rows
+    k.copy_(torch.from_numpy(x))
+    v = torch.from_numpy(x).to(cuda).transpose(0, 1).contiguous().transpose(0, 1)
+    ks.kv4_append_async(c.cache, c.table, c.seq_lens, k, v, token_offsets=c.offsets, status=c.status)
+    ko = torch.zeros(20, heads, d + 1, device=cuda)[..., 1:]
+    vo = torch.zeros(heads, 20, d, device=cuda).transpose(0, 1)
+    ks.kv4_read_async(c.cache, c.table, c.seq_lens, ko, vo, token_offsets=c.offsets, status=c.status)
+    c.ok()
+    want = torch.from_numpy(O.kv4_value(*O.kv4_quantize(x, group)).astype(np.float32))
+    assert torch.equal(ko.cpu(), want) and torch.equal(vo.cpu(), want)
+
+
+def test_append_not_finite(ks, cuda):
+    import torch
+
+    c = Seqs(ks, cuda, [3], [3], 1, 64, 32, 16, garbage=False)
+    x = torch.ones(3, 1, 64, device=cuda)
+    x[0, 0, 3], x[0, 0, 40], x[1, 0, 5], x[2, 0, 0] = float("nan"), float("inf"), -float("inf"), 1e-30
+    x[2, 0, 32:] = 3e38
+    y = torch.zeros_like(x)
+    ks.kv4_append_async(c.cache, c.table, c.seq_lens, x, torch.ones_like(x), token_offsets=c.offsets, status=c.status)
+    ks.kv4_read_async(c.cache, c.table, c.seq_lens, y, torch.zeros_like(x), token_offsets=c.offsets, status=None)
+    torch.cuda.synchronize()
+    assert c.status.cpu().tolist() == [1, 0]
+    want = O.kv4_value(*O.kv4_quantize(x.double().cpu().numpy(), 32))
+    assert np.isfinite(want).all() and (y.double().cpu().numpy() == want).all()
+    assert y[0, 0, 3] == 0 and y[0, 0, 40] == 7 * 65504 and y[1, 0, 5] == -8 * 65504 and y[2, 0, 33] == 7 * 65504
+    with pytest.raises(ks.KernelSmithError):
+        ks.check(ks.lib().ks_b200_status_check(ks.addr(c.status), None))
+
+
+# --------------------------------------------------------------------- attention
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,group", [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("heads,q_heads", [(2, 2), (1, 4), (2, 10), (1, 8), (1, 12)])
+def test_decode(ks, cuda, dtype, d, group, heads, q_heads):
+    """One new token: lengths around tiles, blocks, pages and chunks."""
+    lens = [1, 2, 15, 16, 17, 31, 33, 64, 100, 255, 257, 700]
+    c = Seqs(ks, cuda, lens, [1] * len(lens), heads, d, group, 32, seed=d + group + q_heads)
+    q = _query(c, q_heads, dtype)
+    out, lse = _attend(c, q, d**-0.5)
+    c.ok()
+    _check(c, q, d**-0.5, out, lse, dtype)
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_pages(ks, cuda, page):
+    lens = [1, page - 1, page, page + 1, 3 * page + 7, 300]
+    for d, group in ((128, 32), (64, 64)):
+        c = Seqs(ks, cuda, lens, [1] * len(lens), 2, d, group, page, seed=page)
+        q = _query(c, 8, "f32")
+        out, lse = _attend(c, q, 0.1, offsets=False)
+        c.ok()
+        _check(c, q, 0.1, out, lse, "f32")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,group", [(64, 32), (128, 32), (128, 128)])
+@pytest.mark.parametrize("q_heads,heads,lens,news", [
+    (4, 1, [5, 40, 70, 0, 9], [2, 3, 1, 0, 9]),  # a prompt, drafts, one token, an idle place
+    (7, 1, [130, 33], [5, 33]),
+    (6, 2, [300, 64], [31, 64]),
+    (2, 2, [700], [17]),
+])
+def test_several_new_tokens(ks, cuda, dtype, d, group, q_heads, heads, lens, news):
+    c = Seqs(ks, cuda, lens, news, heads, d, group, 16, seed=len(lens) + d)
+    q = _query(c, q_heads, dtype)
+    out, lse = _attend(c, q, d**-0.5)
+    c.ok()
+    _check(c, q, d**-0.5, out, lse, dtype)
+
+
+def test_long_and_split(ks, cuda):
+    """Many chunks to a row, one head."""
+    for d, group, dtype in ((128, 64, "f32"), (64, 32, "bf16")):
+        c = Seqs(ks, cuda, [20000, 3, 9001], [1, 1, 2], 1, d, group, 64, seed=5)
+        q = _query(c, 5, dtype)
+        out, lse = _attend(c, q, d**-0.5)
+        c.ok()
+        _check(c, q, d**-0.5, out, lse, dtype)
+
+
+def test_empty_rows_and_rows_behind(ks, cuda):
+    """Sequences without tokens, new tokens before position 0, rows before and behind the sequences, strided rows."""
+    import torch
+
+    lens, news = [0, 3, 50, 0], [2, 5, 1, 0]
+    c = Seqs(ks, cuda, lens, news, 2, 64, 32, 16)
+    c.first = c.first + 1
+    c.offsets = c.offsets + 1
+    big = torch.randn(c.tokens + 3, 6, 64 + 3, device=cuda)
+    q = big[:, :4, :64]
+    out = torch.full((4, c.tokens + 3, 64), 7.0, device=cuda).transpose(0, 1)
+    lse = torch.full((c.tokens + 3, 4), 7.0, device=cuda)
+    c.tokens += 3
+    _attend(c, q, 0.125, out=out, lse=lse, max_len=64)
+    c.ok()
+    assert (out[0] == 7).all() and (out[-2:] == 7).all() and (lse[0] == 7).all() and (lse[-2:] == 7).all()
+    assert (out[1:3] == 0).all() and torch.isneginf(lse[1:3]).all()  # no token
+    assert (out[3:5] == 0).all() and torch.isneginf(lse[3:5]).all()  # before position 0
+    _check(c, q, 0.125, out, lse, "f32")
+
+
+def test_extreme_scores(ks, cuda):
+    """Scores far apart, all equal, negative and zero scale; values of very unlike size; huge and tiny queries."""
+    import torch
+
+    for scale, size in ((1.0, 30.0), (0.0, 1.0), (-0.125, 1.0), (1e-20, 1e18), (1e20, 1e-20)):
+        c = Seqs(ks, cuda, [400, 7], [1, 2], 1, 128, 32, 64, seed=11)
+        q = _query(c, 4, "f32", size=size)
+        out, lse = _attend(c, q, scale)
+        c.ok()
+        _check(c, q, scale, out, lse, "f32")
+    # one token with all the weight and values 2^-18 of the others'
+    c = Seqs(ks, cuda, [320], [1], 1, 64, 32, 64, seed=12)
+    k = torch.zeros(320, 1, 64, device=cuda)
+    v = torch.randn(320, 1, 64, device=cuda) * 2.0**14
+    k[7], v[7] = 4.0, v[7] * 2.0**-18
+    offsets = torch.tensor([0, 320], dtype=torch.int32, device=cuda)
+    ks.kv4_append_async(c.cache, c.table, c.seq_lens, k, v, token_offsets=offsets, status=c.status)
+    c.k[c.pages[0]] = _paged(c, O.kv4_value(*O.kv4_quantize(k.double().cpu().numpy(), 32)))
+    c.v[c.pages[0]] = _paged(c, O.kv4_value(*O.kv4_quantize(v.double().cpu().numpy(), 32)))
+    q = torch.full((1, 2, 64), 1.0, device=cuda)
+    out, lse = _attend(c, q, 1.0)
+    c.ok()
+    _check(c, q, 1.0, out, lse, "f32")
+
+
+def _paged(c, x):
+    full = np.zeros((len(c.pages[0]) * c.page, c.heads, c.d))
+    full[: len(x)] = x
+    return full.reshape(-1, c.page, c.heads, c.d).transpose(0, 2, 1, 3)
+
+
+def test_queries_not_finite_stay_in_their_rows(ks, cuda):
+    import torch
+
+    c = Seqs(ks, cuda, [300], [1], 1, 128, 64, 32)
+    q = _query(c, 8, "f32")
+    good, _ = _attend(c, q, 0.1)
+    bad = q.clone()
+    bad[0, 2, 5], bad[0, 6, 0] = float("nan"), float("inf")
+    out, lse = _attend(c, bad, 0.1)
+    c.ok()
+    rows = [0, 1, 3, 4, 5, 7]
+    assert torch.equal(out[0, rows], good[0, rows])
+    assert torch.isnan(out[0, 2]).all() and torch.isnan(out[0, 6]).all() and torch.isnan(lse[0, [2, 6]]).all()
+
+
+@pytest.mark.parametrize("q_heads,heads,lens,news", [
+    (4, 1, [5, 40, 300, 0], [1, 1, 1, 0]),
+    (3, 3, [17, 600], [1, 1]),
+    (8, 2, [90, 33, 512], [7, 33, 1]),
+])
+@pytest.mark.parametrize("dtype,d,group", [("f32", 128, 32), ("bf16", 64, 64), ("f16", 128, 128)])
+def test_accumulated_weights(ks, cuda, q_heads, heads, lens, news, dtype, d, group):
+    import torch
+
+    c = Seqs(ks, cuda, lens, news, heads, d, group, 16, weights=True)
+    before = c.w.double().cpu().numpy()
+    q = _query(c, q_heads, dtype)
+    out, lse = _attend(c, q, d**-0.5, accumulate=True)
+    c.ok()
+    _check(c, q, d**-0.5, out, lse, dtype, weights=c.w, before=before)
+    used = np.zeros(before.shape, bool)
+    for s, n in enumerate(lens):
+        for i, p in enumerate(c.pages[s]):
+            used[p, :, : min(16, n - i * 16)] = True
+    assert (c.w.double().cpu().numpy()[~used] == before[~used]).all()
+    # in a fixed order: the same again, bit for bit
+    first, again = c.w.clone(), torch.from_numpy(before.astype(np.float32)).to(cuda)
+    c.w.copy_(again)
+    out2, lse2 = _attend(c, q, d**-0.5, accumulate=True)
+    assert torch.equal(c.w, first) and torch.equal(out, out2) and torch.equal(lse, lse2)
+
+
+def test_far_pages(ks, cuda):
+    """A pool of more than 4 GiB, tokens at its end."""
+    import torch
+
+    heads, d, group, page = 8, 128, 32, 256
+    c = Seqs(ks, cuda, [300, 20], [1, 1], heads, d, group, page, weights=True)
+    per = ks.kv4_page_bytes(page, heads, d, group)
+    n = (9 << 29) // per + c.n_pages
+    pool = torch.empty(n, per, dtype=torch.uint8, device=cuda)
+    pool[n - c.n_pages:] = c.pool.reshape(c.n_pages, per)
+    w = torch.zeros(n, heads, page, device=cuda)
+    c.table += (c.table >= 0).int() * (n - c.n_pages)
+    c.cache = ks.Kv4Cache(pool, n, page, heads, d, group, weights=w)
+    q = _query(c, 16, "f32")
+    out, lse = _attend(c, q, 0.1, accumulate=True)
+    c.ok()
+    _check(c, q, 0.1, out, lse, "f32", weights=w[n - c.n_pages:], before=np.zeros((c.n_pages, heads, page)))
+    k = torch.zeros(2, heads, d, device=cuda)
+    ks.kv4_append_async(c.cache, c.table, c.seq_lens, k + 3, k - 5, status=c.status)
+    ko, vo = torch.zeros_like(k), torch.zeros_like(k)
+    ks.kv4_read_async(c.cache, c.table, c.seq_lens, ko, vo, status=c.status)
+    c.ok()
+    assert torch.allclose(ko, k + 3, rtol=2**-10) and torch.allclose(vo, k - 5, rtol=2**-10)
+
+
+def test_streams_and_graphs(ks, cuda):
+    """A captured step follows lengths, table and queries; two graphs with a workspace each on two streams."""
+    import torch
+
+    c = Seqs(ks, cuda, [900, 350], [1, 1], 2, 128, 32, 64, garbage=False)
+    qs = [_query(c, 8, "f32", seed=i) for i in range(2)]
+    graphs, outs, ws = [], [], []
+    need = ks.kv4_attention_workspace(c.cache, 8, 2, 2, 1, 960)
+    assert need > 0
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for i in range(2):
+        out, lse = torch.zeros_like(qs[i]), torch.zeros(2, 8, device=cuda)
+        ws.append(torch.zeros(need, dtype=torch.uint8, device=cuda))
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[i]):
+            ks.kv4_attention_async(c.cache, c.table, c.seq_lens, qs[i], out, 0.1, ws[i], max_len=960, lse=lse,
+                                   status=c.status, stream=streams[i])
+        graphs.append(g)
+        outs.append((out, lse))
+    pages = np.concatenate(c.pages)  # without accumulated weights, sequences may share pages
+    for lens in ([900, 350], [1, 960], [257, 0]):
+        c.lens, c.pages = lens, [pages[: -(-n // 64)] for n in lens]
+        c.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        for s in range(2):
+            c.table[s] = -1
+            c.table[s, : len(c.pages[s])] = torch.from_numpy(c.pages[s].astype(np.int32)).to(cuda)
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        c.ok()
+        for i in range(2):
+            _check(c, qs[i], 0.1, *outs[i], "f32")
+    del graphs
+
+
+def test_bad_descriptors_are_reported(ks, cuda):
+    """Pages outside the pool, lengths beyond the table, offsets beyond the rows: status word 0, nothing outside
+    the buffers is touched, the other sequences are served."""
+    import torch
+
+    def fresh():
+        return Seqs(ks, cuda, [100, 40], [1, 1], 2, 64, 32, 16, weights=True)
+
+    def good(c, q, out, lse, s=1):
+        torch.cuda.synchronize()
+        assert c.status.cpu().tolist() == [1, 0]
+        want, _, _, _, _ = O.kv4_attention(q.double().cpu().numpy()[s:s + 1], c.cached(s, "k"), c.cached(s, "v"),
+                                           0.1, 1)
+        assert np.abs(out.double().cpu().numpy()[s] - want[0]).max() < 1e-3
+
+    for page in (-1, 1 << 20, -(1 << 31)):
+        c = fresh()
+        q = _query(c, 4, "f32")
+        c.table[0, 2] = page
+        out, lse = _attend(c, q, 0.1, accumulate=True)
+        good(c, q, out, lse)
+    for length in (-1, 1 << 30, 200):
+        c = fresh()
+        q = _query(c, 4, "f32")
+        c.seq_lens[0] = length
+        out, lse = _attend(c, q, 0.1, max_len=112)
+        good(c, q, out, lse)
+        assert (out[0] == 0).all()
+        x = torch.randn(2, 2, 64, device=cuda)
+        before = c.pool.clone()
+        ks.kv4_append_async(c.cache, c.table, c.seq_lens, x, x, status=c.status)
+        changed = (c.pool != before).flatten(1).any(1).nonzero().flatten().tolist()
+        assert set(changed) <= set(c.pages[1].tolist())
+    c = fresh()
+    q = _query(c, 4, "f32")
+    c.offsets = torch.tensor([0, 1, 7], dtype=torch.int32, device=cuda)
+    out = torch.full_like(q, 7)
+    _attend(c, q, 0.1, out=out)
+    torch.cuda.synchronize()
+    assert c.status.cpu().tolist() == [1, 0] and (out[1] == 7).all()
+
+
+# ---------------------------------------------------------------------- eviction
+def _evict(c, budget, recent, kept=True, to_lens=None, status=None):
+    import torch
+
+    keep = [min(n, budget) for n in c.lens]
+    each = [-(-n // c.page) for n in keep]
+    used = c.n_pages
+    n = used + sum(each) + 1
+    pool = torch.full((n, *c.pool.shape[1:]), 0xEE, dtype=torch.uint8, device=c.cuda)
+    pool[:used] = c.pool
+    w = torch.full((n, c.heads, c.page), 7.0, device=c.cuda)
+    w[:used] = c.w
+    table = np.full((len(c.lens), max(each + [1]) + 1), -1, np.int32)
+    at = used
+    for s, k in enumerate(each):
+        table[s, :k] = np.arange(at, at + k)
+        at += k
+    cache = c.ks.Kv4Cache(pool, n, c.page, c.heads, c.d, c.group, weights=w)
+    max_len = max(c.lens)
+    kept = torch.full((len(c.lens), c.heads, budget), -1, dtype=torch.int32, device=c.cuda) if kept else None
+    to_lens = torch.full((len(c.lens),), -5, dtype=torch.int32, device=c.cuda) if to_lens is None else to_lens
+    ws = torch.full((c.ks.kv4_evict_workspace(cache, len(c.lens), max_len, budget),), 255, dtype=torch.uint8,
+                    device=c.cuda)
+    to_table = torch.from_numpy(table).to(c.cuda)
+    c.ks.kv4_evict_async(cache, c.table, c.seq_lens, to_table, to_lens, max_len, budget, recent, ws, kept=kept,
+                         status=c.status)
+    return cache, pool, w, table, to_table, to_lens, kept, keep
+
+
+def _kept_of(w, n, budget, recent):
+    """Positions kept of one head's weights w [n]."""
+    if n <= budget:
+        return np.arange(n)
+    old = n - recent
+    key = np.where(np.isnan(w[:old]), -np.inf, w[:old].astype(np.float64))
+    key = np.where(np.isnan(w[:old]), np.finfo(np.float64).min, np.where(np.isneginf(w[:old]), -1e300, key))
+    order = np.argsort(-key, kind="stable")[: budget - recent]
+    return np.concatenate([np.sort(order), np.arange(old, n)])
+
+
+@pytest.mark.parametrize("d,group,page", [(128, 32, 16), (64, 64, 64), (128, 128, 256), (64, 32, 32)])
+@pytest.mark.parametrize("lens,budget,recent", [
+    ([100, 1, 40, 0, 41], 40, 8),
+    ([300, 5000], 33, 33),    # only the newest
+    ([700, 64], 63, 0),       # only the heaviest
+    ([9000], 4099, 17),
+    ([3], 1, 1),
+])
+def test_evict(ks, cuda, d, group, page, lens, budget, recent):
+    import torch
+
+    c = Seqs(ks, cuda, lens, [0] * len(lens), 2, d, group, page, weights=True, seed=budget)
+    ties = torch.from_numpy(np.random.default_rng(1).integers(0, 6, tuple(c.w.shape)).astype(np.float32)).to(cuda)
+    c.w.copy_(torch.where(torch.rand_like(c.w) < 0.5, ties / 5, c.w))
+    c.w[torch.rand_like(c.w) < 0.02] = float("nan")
+    c.w[torch.rand_like(c.w) < 0.02] = -0.0
+    c.w[torch.rand_like(c.w) < 0.01] = float("inf")
+    c.w[torch.rand_like(c.w) < 0.01] = -float("inf")
+    before = c.pool.clone()
+    cache, pool, w, table, to_table, to_lens, kept, keep = _evict(c, budget, recent)
+    c.ok()
+    assert to_lens.tolist() == keep and torch.equal(pool[: c.n_pages], before)
+    old, new = c.w.cpu().numpy(), w.cpu().numpy()
+    src, dst = c.pool.cpu().numpy(), pool.cpu().numpy()
+    per, half = 2 * (d // group), src.shape[-1] // 2
+
+    def row(p, h, page_id, slot):
+        b = p[page_id, h, slot // 16]
+        i = slot % 16
+        return np.concatenate([x for o in (0, half) for x in (b[o + i * (d // 2):o + (i + 1) * (d // 2)],
+                                                              b[o + 8 * d + i * per:o + 8 * d + (i + 1) * per])])
+
+    for s, n in enumerate(lens):
+        for h in range(c.heads):
+            at = c.weights_of(s, old)[h]
+            want = _kept_of(at, n, budget, recent)
+            assert kept[s, h, : keep[s]].tolist() == want.tolist(), (s, h)
+            assert (kept[s, h, keep[s]:] == -1).all()
+            for i in list(range(min(keep[s], 20))) + list(range(max(keep[s] - 20, 0), keep[s])):
+                a, b = c.pages[s][want[i] // page], table[s, i // page]
+                assert (row(src, h, a, want[i] % page) == row(dst, h, b, i % page)).all()
+            got = np.concatenate([new[p, h] for p in table[s] if p >= 0] + [np.zeros(0, np.float32)])
+            np.testing.assert_array_equal(got[: keep[s]], at[want])
+            assert (got[keep[s]:] == 7).all()
+
+
+def test_evict_in_place_lengths_and_no_list(ks, cuda):
+    c = Seqs(ks, cuda, [90, 20, 64], [0] * 3, 3, 64, 32, 16, weights=True)
+    _, _, _, _, _, to_lens, _, keep = _evict(c, 50, 10, kept=False, to_lens=c.seq_lens)
+    c.ok()
+    assert c.seq_lens.tolist() == keep
+
+
+# ------------------------------------------------------------------ all together
+@pytest.mark.parametrize("dtype,d,group,q_heads", [("f32", 128, 32, 8), ("bf16", 64, 64, 6)])
+def test_generation(ks, cuda, dtype, d, group, q_heads):
+    """A prompt, decode steps that accumulate weights, an eviction, more steps: as the definition has them."""
+    import torch
+
+    heads, page, prompts = 2, 16, [70, 30]
+    rng = np.random.default_rng(4)
+    T = _type(dtype)
+    n_pages = 40
+    pool = torch.full((n_pages, ks.kv4_page_bytes(page, heads, d, group)), 0xFF, dtype=torch.uint8, device=cuda)
+    w = torch.full((n_pages, heads, page), float("nan"), device=cuda)
+    cache = ks.Kv4Cache(pool, n_pages, page, heads, d, group, weights=w)
+    ids = rng.permutation(n_pages).astype(np.int32)
+    table = torch.from_numpy(ids[:20].reshape(2, 10).copy()).to(cuda)
+    lens = torch.zeros(2, dtype=torch.int32, device=cuda)
+    status = torch.zeros(2, dtype=torch.int32, device=cuda)
+    ref = [dict(k=[np.zeros((0, d))] * heads, v=[np.zeros((0, d))] * heads, w=[np.zeros(0)] * heads) for _ in range(2)]
+    half = torch.finfo(T).eps / 2
+
+    def step(news):
+        tokens = sum(news)
+        x = [torch.from_numpy(rng.standard_normal((tokens, n, d))).to(T).to(cuda) for n in (q_heads, heads, heads)]
+        offsets = torch.tensor(np.concatenate([[0], np.cumsum(news)]), dtype=torch.int32, device=cuda)
+        lens.add_(torch.tensor(news, dtype=torch.int32, device=cuda))
+        ks.kv4_append_async(cache, table, lens, x[1], x[2], token_offsets=offsets, status=status)
+        out, lse = torch.zeros_like(x[0]), torch.zeros(tokens, q_heads, device=cuda)
+        ws = torch.zeros(max(16, ks.kv4_attention_workspace(cache, q_heads, 2, tokens, max(news), 160)),
+                         dtype=torch.uint8, device=cuda)
+        ks.kv4_attention_async(cache, table, lens, x[0], out, d**-0.5, ws, token_offsets=offsets, max_new=max(news),
+                               max_len=160, lse=lse, accumulate=True, status=status)
+        torch.cuda.synchronize()
+        assert status.tolist() == [0, 0]
+        q, k, v = (t.double().cpu().numpy() for t in x)
+        at = 0
+        for s, n in enumerate(news):
+            r = ref[s]
+            for h in range(heads):
+                for name, y in (("k", k), ("v", v)):
+                    r[name][h] = np.concatenate([r[name][h], O.kv4_value(*O.kv4_quantize(y[at:at + n, h], group))])
+                r["w"][h] = np.concatenate([r["w"][h], np.zeros(n)])
+            g = q_heads // heads
+            for h in range(heads):
+                want, z, add, size, _ = O.kv4_attention(q[at:at + n, h * g:(h + 1) * g], r["k"][h][:, None],
+                                                        r["v"][h][:, None], d**-0.5, n)
+                r["w"][h] = r["w"][h] + add[0]
+                got = out[at:at + n, h * g:(h + 1) * g].double().cpu().numpy()
+                assert (np.abs(got - want) <= half * np.abs(want) + 2.0**-10 * size).all()
+            at += n
+
+    step(prompts)
+    for _ in range(3):
+        step([1, 1])
+    step([2, 4])
+    # the heads keep different tokens
+    to = torch.from_numpy(ids[20:40].reshape(2, 10).copy()).to(cuda)
+    budget, recent = 40, 6
+    kept = torch.full((2, heads, budget), -1, dtype=torch.int32, device=cuda)
+    ws = torch.zeros(ks.kv4_evict_workspace(cache, 2, 160, budget), dtype=torch.uint8, device=cuda)
+    old = lens.tolist()
+    ks.kv4_evict_async(cache, table, lens, to, lens, 160, budget, recent, ws, kept=kept, status=status)
+    torch.cuda.synchronize()
+    assert lens.tolist() == [min(n, budget) for n in old]
+    for s in range(2):
+        for h in range(heads):
+            at = kept[s, h, : lens[s]].tolist()
+            r = ref[s]
+            assert at == sorted(set(at)) and at[-recent:] == list(range(old[s] - recent, old[s]))
+            # f32 sums and the roundings of the scores may swap weights that are nearly the same
+            low = np.sort(r["w"][h][: old[s] - recent])[::-1]
+            if old[s] > budget:
+                assert r["w"][h][at[:-recent]].min() >= low[budget - recent - 1] * (1 - 2.0**-10)
+            r["k"][h], r["v"][h], r["w"][h] = r["k"][h][at], r["v"][h][at], r["w"][h][at]
+    table.copy_(to)
+    for _ in range(3):
+        step([1, 1])
+    step([3, 1])

@@ -221,6 +221,56 @@ struct ImportQ4Launch {
 };
 cudaError_t launch_import_q4_0(const ImportQ4Launch &a, cudaStream_t stream);
 
+// The paged 4-bit key/value cache (layout: ks_kv4.cuh).
+enum DType : int { kF32 = 0, kF16 = 1, kBF16 = 2 };
+struct Kv4View {
+  uint8_t *pool;
+  float *weights;  // [page][kv_head][slot] accumulated attention weights, or null
+  int64_t page_bytes, head_bytes;
+  int block_bytes, page_shift;  // a block of 16 tokens of one head; log2(page_size)
+  int n_pages, kv_heads, head_dim, groups;
+};
+// The sequences of a call: pages, cached tokens and (packed, offsets[s] ..
+// offsets[s + 1]; one each when null) the rows of their newest tokens.
+struct Kv4Batch {
+  const int32_t *table;
+  int64_t table_stride;
+  const int32_t *lens, *offsets;
+  int n_seqs, n_tokens;
+  int max_len;  // no sequence is longer (at most what a row of the table holds)
+};
+// Rows of new tokens, [n_tokens][kv_heads][head_dim] with element strides.
+struct Kv4Rows {
+  void *k, *v;
+  int64_t k_token, k_head, v_token, v_head;
+  int dtype;  // DType
+};
+cudaError_t launch_kv4_append(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, uint32_t *status,
+                              cudaStream_t stream);
+cudaError_t launch_kv4_read(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, uint32_t *status,
+                            cudaStream_t stream);
+struct Kv4Evict {
+  const int32_t *to_table;
+  int64_t to_stride;
+  int32_t *to_lens;
+  int32_t *kept;  // [n_seqs][kv_heads][budget], or null
+  int budget, recent;
+  void *workspace;
+};
+size_t kv4_evict_workspace(const Kv4View &c, int n_seqs, int max_len, int budget);
+cudaError_t launch_kv4_evict(const Kv4View &c, const Kv4Batch &b, const Kv4Evict &e, uint32_t *status,
+                             cudaStream_t stream);
+struct Kv4Attention {
+  const void *q;
+  void *out;
+  int64_t q_token, q_head, out_token, out_head;  // element strides
+  int q_heads, dtype, max_new;
+  float scale;
+  float *lse;  // [n_tokens][q_heads], or null
+  bool accumulate;
+  void *workspace;
+};
+
 // Which kernel family launch_w4a8 / launch_i8 picked for a shape (tests and
 // benchmarks report it): 0 = generic per-element path, 1 = TMA-staged path.
 int w4a8_path(const W4A8Launch &a);

@@ -36,6 +36,9 @@ STATUS_WORDS = 2
 STATUS_BAD_SCALE = 0
 STATUS_TIMEOUT = 1
 IPC_HANDLE_BYTES = 64
+DTYPE_F32 = 0
+DTYPE_F16 = 1
+DTYPE_BF16 = 2
 KS_QUANT_LAYOUT_VERSION = 1  # include/ks_b200.h; lib().ks_b200_quant_layout_version() returns the built value
 
 _vp = c_void_p
@@ -140,6 +143,26 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "ks_b200_quantize_per_token_async": (c_int, [_vp, _sz, _sz, _sz, _vp, _sz, _vp, _vp]),
     "ks_b200_decode_layer_launches": (c_int, [_sz, _sz, _sz]),
+    "ks_b200_kv4_page_bytes": (_sz, [_sz, _sz, _sz, _sz]),
+    "ks_b200_kv4_append_async": (
+        c_int,
+        [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _sz, c_int, _vp, _vp],
+    ),
+    "ks_b200_kv4_read_async": (
+        c_int,
+        [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _sz, c_int, _vp, _vp],
+    ),
+    "ks_b200_kv4_attention_workspace": (_sz, [_vp, _sz, _sz, _sz, _sz, _sz]),
+    "ks_b200_kv4_attention_async": (
+        c_int,
+        [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _sz, _vp, _sz, _sz, _sz, _f, _vp, _sz, _sz, c_int, _vp, c_int,
+         _vp, _sz, _vp, _vp],
+    ),
+    "ks_b200_kv4_evict_workspace": (_sz, [_vp, _sz, _sz, _sz]),
+    "ks_b200_kv4_evict_async": (
+        c_int,
+        [_vp, _vp, _sz, _vp, _sz, _sz, _vp, _sz, _vp, _sz, _sz, _vp, _vp, _sz, _vp, _vp],
+    ),
     # include/ks_b200_ggml.h: the GGML MUL_MAT(Q4_0, f32) adapter
     "ks_b200_ggml_q4_0_create": (c_int, [_vp, _sz, _sz, _sz, _vp, _vp]),
     "ks_b200_ggml_q4_0_destroy": (c_int, [_vp]),
@@ -366,6 +389,109 @@ def matvec_i8_batch_async(xs, ws, ys, w_stride, rows, cols, zx=0, zw=0, w_scales
         lib().ks_b200_matvec_i8_batch_async(
             n, _ptr_array(xs), _ptr_array(ws), _ptr_array(w_scales) if w_scales is not None else None,
             _ptr_array(ys), w_stride, rows, cols, zx, zw, sa, stream_handle(stream),
+        )
+    )
+
+
+_DTYPES = {"torch.float32": DTYPE_F32, "torch.float16": DTYPE_F16, "torch.bfloat16": DTYPE_BF16}
+
+
+def _rows3(t) -> tuple[int, int, int]:
+    """Token and head strides and KS_B200_DTYPE_* of a [tokens, heads, head_dim] tensor."""
+    token, head, last = t.stride()
+    if last != 1:
+        raise ValueError("the last dimension must be contiguous")
+    return token, head, _DTYPES[str(t.dtype)]
+
+
+class Kv4Cache(ctypes.Structure):
+    """ks_b200_kv4_cache (include/ks_b200.h): a pool of pages of 4-bit keys and values on the device,
+    n_pages * kv4_page_bytes(...) bytes, and (or None) the tokens' accumulated attention weights, f32
+    [n_pages, kv_heads, page_size].  The tensors are kept alive with it."""
+
+    _fields_ = [("pool", _vp), ("weights", _vp), ("n_pages", _sz), ("page_size", _sz), ("kv_heads", _sz),
+                ("head_dim", _sz), ("group_size", _sz)]
+
+    def __init__(self, pool, n_pages, page_size, kv_heads, head_dim, group_size, weights=None):
+        super().__init__(addr(pool), addr(weights), n_pages, page_size, kv_heads, head_dim, group_size)
+        self._tensors = (pool, weights)
+
+
+def kv4_page_bytes(page_size, kv_heads, head_dim, group_size) -> int:
+    return lib().ks_b200_kv4_page_bytes(page_size, kv_heads, head_dim, group_size)
+
+
+def kv4_append_async(cache, page_table, seq_lens, k, v, token_offsets=None, status=None, stream=None) -> None:
+    """Quantise the newest tokens of each sequence, k and v [n_tokens, kv_heads, head_dim], into the cache."""
+    kt, kh, dtype = _rows3(k)
+    vt, vh, vtype = _rows3(v)
+    if vtype != dtype or tuple(k.shape) != tuple(v.shape) or tuple(k.shape[1:]) != (cache.kv_heads, cache.head_dim):
+        raise ValueError("k and v must be [n_tokens, kv_heads, head_dim] of one type")
+    check(
+        lib().ks_b200_kv4_append_async(
+            ctypes.byref(cache), addr(page_table), page_table.stride(0), addr(seq_lens), addr(token_offsets),
+            seq_lens.numel(), k.shape[0], addr(k), kt, kh, addr(v), vt, vh, dtype, addr(status),
+            stream_handle(stream),
+        )
+    )
+
+
+def kv4_read_async(cache, page_table, seq_lens, k, v, token_offsets=None, status=None, stream=None) -> None:
+    """Dequantise the newest tokens of each sequence into k and v [n_tokens, kv_heads, head_dim]."""
+    kt, kh, dtype = _rows3(k)
+    vt, vh, vtype = _rows3(v)
+    if vtype != dtype or tuple(k.shape) != tuple(v.shape) or tuple(k.shape[1:]) != (cache.kv_heads, cache.head_dim):
+        raise ValueError("k and v must be [n_tokens, kv_heads, head_dim] of one type")
+    check(
+        lib().ks_b200_kv4_read_async(
+            ctypes.byref(cache), addr(page_table), page_table.stride(0), addr(seq_lens), addr(token_offsets),
+            seq_lens.numel(), k.shape[0], addr(k), kt, kh, addr(v), vt, vh, dtype, addr(status),
+            stream_handle(stream),
+        )
+    )
+
+
+def kv4_attention_workspace(cache, q_heads, n_seqs, n_tokens, max_new, max_len) -> int:
+    return lib().ks_b200_kv4_attention_workspace(ctypes.byref(cache), q_heads, n_seqs, n_tokens, max_new, max_len)
+
+
+def kv4_attention_async(cache, page_table, seq_lens, q, out, scale, workspace, token_offsets=None, max_new=1,
+                        max_len=None, lse=None, accumulate=False, status=None, stream=None) -> None:
+    """Attention of the newest tokens, q and out [n_tokens, q_heads, head_dim], over the cache.  max_len: no
+    sequence is longer (default: what a row of the page table holds); workspace: a device byte tensor."""
+    qt, qh, dtype = _rows3(q)
+    ot, oh, otype = _rows3(out)
+    if otype != dtype or tuple(q.shape) != tuple(out.shape) or q.shape[2] != cache.head_dim:
+        raise ValueError("q and out must be [n_tokens, q_heads, head_dim] of one type")
+    if lse is not None and not (lse.is_contiguous() and tuple(lse.shape) == tuple(q.shape[:2])):
+        raise ValueError("lse must be a contiguous f32 [n_tokens, q_heads]")
+    stride = page_table.stride(0)
+    check(
+        lib().ks_b200_kv4_attention_async(
+            ctypes.byref(cache), addr(page_table), stride, addr(seq_lens), addr(token_offsets), seq_lens.numel(),
+            q.shape[0], max_new, stride * cache.page_size if max_len is None else max_len, addr(q), qt, qh,
+            q.shape[1], scale, addr(out), ot, oh, dtype, addr(lse), int(accumulate), addr(workspace),
+            workspace.numel(), addr(status), stream_handle(stream),
+        )
+    )
+
+
+def kv4_evict_workspace(cache, n_seqs, max_len, budget) -> int:
+    return lib().ks_b200_kv4_evict_workspace(ctypes.byref(cache), n_seqs, max_len, budget)
+
+
+def kv4_evict_async(cache, page_table, seq_lens, to_table, to_lens, max_len, budget, recent, workspace, kept=None,
+                    status=None, stream=None) -> None:
+    """Keep the newest `recent` tokens of each sequence and head and the heaviest others, `budget` in all, in the
+    pages of to_table; kept: None or int32 [n_seqs, kv_heads, budget] for their old positions."""
+    if kept is not None and not (kept.is_contiguous() and tuple(kept.shape) == (seq_lens.numel(), cache.kv_heads,
+                                                                                budget)):
+        raise ValueError("kept must be a contiguous int32 [n_seqs, kv_heads, budget]")
+    check(
+        lib().ks_b200_kv4_evict_async(
+            ctypes.byref(cache), addr(page_table), page_table.stride(0), addr(seq_lens), seq_lens.numel(), max_len,
+            addr(to_table), to_table.stride(0), addr(to_lens), budget, recent, addr(kept), addr(workspace),
+            workspace.numel(), addr(status), stream_handle(stream),
         )
     )
 
