@@ -99,31 +99,29 @@ int rows_ok(const void *p, size_t tokens, size_t token_stride, size_t heads, siz
 }
 
 // How the attention is cut.  Row tiles of 8 while the rows of a key/value head
-// fit, else 16.  Chunks: three times as many CTAs as the GPU holds at once, so
-// that unequal lengths even out, of at least 256 tokens (two tiles to a warp).
-Kv4Plan plan_of(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_new, size_t max_len) {
+// fit, else 16; as many CTAs as the GPU holds at once, but no more than there
+// can be units of work.
+Kv4Plan plan_of(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_new, size_t max_len, int dtype) {
   Kv4Plan p;
   const size_t rows = max_new * group_heads;
   p.rows_tile = rows <= 8 ? 8 : 16;
   p.row_tiles = (int)((rows + p.rows_tile - 1) / p.rows_tile);
-  const size_t tiles = n_seqs * v.kv_heads * p.row_tiles;
-  const size_t ctas = 3 * kPlanSms * (p.rows_tile == 8 ? 3 : 2);
-  size_t chunk = (max_len * tiles + ctas - 1) / ctas;
-  chunk = (chunk + 127) / 128 * 128;
-  if (chunk < 256) chunk = 256;
-  p.chunk = (int)chunk;
-  p.chunks = (int)((max_len + chunk - 1) / chunk);
+  const size_t units = n_seqs * v.kv_heads * p.row_tiles * ((max_len + kUnitTokens - 1) / kUnitTokens);
+  const size_t ctas = kPlanSms * kv4_ctas_per_sm(p.rows_tile / 8, dtype == KS_B200_DTYPE_F32 ? 2 : 1);
+  p.ctas = (int)(units < ctas ? units : ctas);
   return p;
 }
 
 bool attention_sizes_ok(const Kv4View &v, size_t q_heads, size_t n_seqs, size_t max_new, size_t max_len) {
   return q_heads > 0 && q_heads % v.kv_heads == 0 && q_heads <= kMost && n_seqs > 0 && n_seqs <= 65535 && max_new > 0 &&
-         max_len > 0 && max_new <= max_len && max_len <= kMost - 1024 && max_new * (q_heads / v.kv_heads) <= kMost / 2;
+         max_len > 0 && max_new <= max_len && max_len <= kMost - 1024 && max_new <= kMost / q_heads &&
+         n_seqs * max_new <= (size_t)1 << 40 && n_seqs * max_new * q_heads <= ((size_t)1 << 50) / (max_len / 128 + 1);
 }
 
-size_t attention_bytes(const Kv4View &v, const Kv4Plan &p, size_t n_seqs) {
-  if (p.chunks <= 1) return 0;
-  return n_seqs * v.kv_heads * p.row_tiles * (size_t)p.chunks * p.rows_tile * (v.head_dim + 2) * 4;
+// The counters, then two parts of every CTA: for any type (f16 and bf16 have the most CTAs).
+size_t attention_bytes(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_new, size_t max_len) {
+  const Kv4Plan p = plan_of(v, group_heads, n_seqs, max_new, max_len, KS_B200_DTYPE_F16);
+  return 4 * (kAttnCounters + 2 * (size_t)p.ctas * p.rows_tile * (v.head_dim + 2));
 }
 
 }  // namespace
@@ -185,7 +183,7 @@ extern "C" size_t ks_b200_kv4_attention_workspace(const ks_b200_kv4_cache *cache
   (void)n_tokens;
   Kv4View v{};
   if (view_of(cache, &v) != KS_OK || !attention_sizes_ok(v, q_heads, n_seqs, max_new, max_len)) return 0;
-  return attention_bytes(v, plan_of(v, q_heads / v.kv_heads, n_seqs, max_new, max_len), n_seqs);
+  return attention_bytes(v, q_heads / v.kv_heads, n_seqs, max_new, max_len);
 }
 
 extern "C" int ks_b200_kv4_attention_async(const ks_b200_kv4_cache *cache, const int32_t *page_table,
@@ -217,9 +215,9 @@ extern "C" int ks_b200_kv4_attention_async(const ks_b200_kv4_cache *cache, const
   if (!attention_sizes_ok(k.c, q_heads, n_seqs, max_new, (size_t)k.b.max_len))
     return fail(KS_ERR_UNSUPPORTED, "too many rows or tokens for one call");
   k.group_heads = (int)(q_heads / k.c.kv_heads);
-  k.p = plan_of(k.c, k.group_heads, n_seqs, max_new, (size_t)k.b.max_len);
-  const size_t need = attention_bytes(k.c, k.p, n_seqs);
-  if (need && (!workspace || misaligned(workspace, 16) || workspace_bytes < need))
+  k.p = plan_of(k.c, k.group_heads, n_seqs, max_new, (size_t)k.b.max_len, dtype);
+  const size_t need = attention_bytes(k.c, k.group_heads, n_seqs, max_new, (size_t)k.b.max_len);
+  if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
     return fail(KS_ERR_WORKSPACE, "workspace smaller than ks_b200_kv4_attention_workspace, or not 16-byte aligned");
   k.a.q = q;
   k.a.out = out;
