@@ -645,7 +645,7 @@ int ks_b200_kv4_read_async(const ks_b200_kv4_cache *cache,
  * (max_new <= max_len <= page_table_stride * page_size): they size the launch.
  * out may not overlap q.  workspace: device memory, 16-byte aligned,
  * ks_b200_kv4_attention_workspace(...) bytes for these sizes, zero-filled
- * before its first use (its first 4096 bytes are 0 again after each call, so
+ * before its first use (its first 8192 bytes are 0 again after each call, so
  * calls of any sizes may follow one another in it), not shared by calls that
  * may run at the same time (two graphs that replay at the same time need one
  * each).  After a call whose status reports a timeout, zero it again.

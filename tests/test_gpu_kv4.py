@@ -99,11 +99,11 @@ def _attend(c, q, scale, out=None, lse=True, max_new=None, max_len=None, accumul
     max_len = max(c.lens + [max_new]) if max_len is None else max_len
     need = c.ks.kv4_attention_workspace(c.cache, q.shape[1], len(c.lens), c.tokens, max_new, max_len)
     ws = torch.full((need,), 255, dtype=torch.uint8, device=c.cuda)  # NaN: nothing may be taken from it
-    ws[:4096] = 0
+    ws[:8192] = 0
     c.ks.kv4_attention_async(c.cache, c.table, c.seq_lens, q, out, scale, ws,
                              token_offsets=c.offsets if offsets else None, max_new=max_new, max_len=max_len,
                              lse=lse, accumulate=accumulate, status=c.status, stream=stream)
-    assert not ws[:4096].any()  # ready for the next call
+    assert not ws[:8192].any()  # ready for the next call
     return out, lse
 
 

@@ -54,7 +54,11 @@ namespace ksb {
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
 constexpr int kTileBlocks = 2, kTileTokens = kTileBlocks * kKv4Block;
 constexpr int kUnitTokens = kAttnWarps * kTileTokens;
-constexpr int kAttnCounters = 1024;  // words at the start of the workspace, one per CTA, 0 between calls
+constexpr int kJoin = 16;  // parts that are joined at once
+// Words at the start of the workspace, 0 between calls: three per CTA, of the
+// item that begins in its stretch (finished groups of parts), of that item's
+// first group of parts and of a later group, which begins at this CTA.
+constexpr int kAttnCtas = 680, kAttnCounters = 2048;
 
 // How a call is cut: the same on the host, for the workspace, and in the kernel.
 struct Kv4Plan {
@@ -97,6 +101,16 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
       "%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// d = a * b + c, the rows' constants of a lane's four accumulators
+__device__ __forceinline__ void mma_f16_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1, const float4 &c) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, "
+      "%12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
 }
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -157,8 +171,8 @@ struct Kv4Smem {
   static constexpr int kRing = kAttnWarps * kStages * kStage;
   static constexpr int kMerge = kAttnWarps * 8 * NT * (D + 2) * 4;  // over the ring, once it is drained
   static constexpr int kQ = kRing > kMerge ? kRing : kMerge;        // NT x D/32 x QS fragments of 512 bytes
-  static constexpr int kCorr = kQ + NT * (D / 32) * QS * 512;       // NT x NG x QS x 8 f32
-  static constexpr int kFactor = kCorr + NT * NG * QS * 8 * 4;      // 8 NT f32
+  static constexpr int kCorr = kQ + NT * (D / 32) * QS * 512;       // NT x NG x QS x 4 float4
+  static constexpr int kFactor = kCorr + NT * NG * QS * 64;        // 8 NT f32
   static constexpr int kLse = kFactor + 8 * NT * 4;                 // 8 NT f32
   static constexpr int kPages = kLse + 8 * NT * 4;                  // pages of a stage's blocks
   static constexpr int kBar = kPages + kAttnWarps * kStages * 8;    // mbarriers
@@ -238,9 +252,11 @@ __device__ __forceinline__ void load_queries(const Kv4AttnArgs &k, const Kv4Seq 
           make_uint4(part[p][0], part[p][1], part[p][2], part[p][3]);
 #pragma unroll
       for (int o = 1; o < 4 * W; o *= 2) sum[p] += __shfl_xor_sync(0xffffffffu, sum[p], o);
-      if (t == 0 && w % W == 0)  // codes + 8 stand for 2^-20 of their value
-        reinterpret_cast<float *>(smem + S::kCorr)[(((n >> 3) * NG + w / W) * QS + p) * 8 + (n & 7)] =
-            sum[p] * (-8.0f * 0x1p-20f);
+      if (t == 0 && w % W == 0) {  // codes + 8 stand for 2^-20 of their value; rows 2t, 2t + 1, twice
+        float *c = reinterpret_cast<float *>(smem + S::kCorr) + (((n >> 3) * NG + w / W) * QS + p) * 16 +
+                   (n & 7) / 2 * 4 + (n & 1);
+        c[0] = c[2] = sum[p] * (-8.0f * 0x1p-20f);
+      }
     }
     if (w == 0 && t == 0)  // not 0: times -inf, that would be NaN
       reinterpret_cast<float *>(smem + S::kFactor)[n] =
@@ -281,18 +297,12 @@ __device__ __forceinline__ void tile_scores(const char *buf, const char *smem, f
 #pragma unroll
   for (int gr = 0; gr < NG; ++gr) {
     float acc[kTileBlocks][NT][QS][4];
+    float4 start[NT][QS];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int p = 0; p < QS; ++p) {
-        const float2 c =
-            *reinterpret_cast<const float2 *>(smem + S::kCorr + (((nt * NG + gr) * QS + p) * 8 + 2 * t) * 4);
-#pragma unroll
-        for (int b = 0; b < kTileBlocks; ++b) {
-          acc[b][nt][p][0] = acc[b][nt][p][2] = c.x;
-          acc[b][nt][p][1] = acc[b][nt][p][3] = c.y;
-        }
-      }
+      for (int p = 0; p < QS; ++p)
+        start[nt][p] = reinterpret_cast<const float4 *>(smem + S::kCorr)[((nt * NG + gr) * QS + p) * 4 + t];
 #pragma unroll
     for (int w = gr * W; w < (gr + 1) * W; ++w) {
       uint32_t q[NT][QS][4];
@@ -310,7 +320,10 @@ __device__ __forceinline__ void tile_scores(const char *buf, const char *smem, f
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int p = 0; p < QS; ++p) {
-            mma_f16(acc[b][nt][p], u[0], v[0], u[1], v[1], q[nt][p][0], q[nt][p][1]);
+            if (w == gr * W)
+              mma_f16_from(acc[b][nt][p], u[0], v[0], u[1], v[1], q[nt][p][0], q[nt][p][1], start[nt][p]);
+            else
+              mma_f16(acc[b][nt][p], u[0], v[0], u[1], v[1], q[nt][p][0], q[nt][p][1]);
             mma_f16(acc[b][nt][p], u[2], v[2], u[3], v[3], q[nt][p][2], q[nt][p][3]);
           }
       }
@@ -338,22 +351,22 @@ struct Kv4Units {
     per = (q.len + kUnitTokens - 1) / kUnitTokens;
     if (!WEIGHTS) per = max(per, 1);
   }
-  __device__ int64_t all() const { return (int64_t)per * items; }
+  __device__ int all() const { return per * items; }
 };
 
 // Sum over the CTA, and over its threads before this one.
-__device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t *total, int64_t *shared) {
+__device__ __forceinline__ int cta_scan(int v, int *total, int *shared) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t sum = v;
+  int sum = v;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
-    const int64_t n = __shfl_up_sync(0xffffffffu, sum, o);
+    const int n = __shfl_up_sync(0xffffffffu, sum, o);
     if (lane >= o) sum += n;
   }
   __syncthreads();
   if (lane == 31) shared[warp] = sum;
   __syncthreads();
-  int64_t before = 0, all = 0;
+  int before = 0, all = 0;
 #pragma unroll
   for (int w = 0; w < kAttnWarps; ++w) {
     if (w < warp) before += shared[w];
@@ -361,6 +374,60 @@ __device__ __forceinline__ int64_t cta_scan(int64_t v, int64_t *total, int64_t *
   }
   *total = all;
   return before + sum - v;
+}
+
+// Joins the parts of CTAs first, first + step, .. (count of them) of the item
+// that CTA c0 began: outputs x, maxima m and sums l of this thread's four
+// elements of a row, I times (row and element by thread as in the kernel).
+template <int D, int R, int I>
+__device__ __forceinline__ void join_parts(const Kv4AttnArgs &k, int c0, int first, int count, int step,
+                                           float4 (&x)[I], float (&m)[I], float (&l)[I]) {
+  constexpr int B = 8 / I > 2 ? 8 / I : 2;  // parts in flight
+#pragma unroll
+  for (int i = 0; i < I; ++i) {
+    x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    m[i] = -INFINITY;
+    l[i] = 0.0f;
+  }
+  for (int at = 0; at < count; at += B) {
+    float4 y[I][B];
+    float pm[I][B], pl[I][B];
+#pragma unroll
+    for (int b = 0; b < B; ++b)
+#pragma unroll
+      for (int i = 0; i < I; ++i) {
+        const int e = threadIdx.x + i * kAttnThreads, n = e / (D / 4), d = e % (D / 4) * 4;
+        pm[i][b] = -INFINITY;
+        pl[i][b] = 0.0f;
+        y[i][b] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (at + b < count) {
+          const int c = first + (at + b) * step;
+          const float *in = kv4_partial(k, c, c == c0);
+          pm[i][b] = __ldcg(in + R * D + n);
+          pl[i][b] = __ldcg(in + R * D + R + n);
+          y[i][b] = __ldcg(reinterpret_cast<const float4 *>(in + n * D + d));
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < I; ++i) {
+      float to = m[i];
+#pragma unroll
+      for (int b = 0; b < B; ++b) to = fmaxf(to, pm[i][b]);
+      const float base = to == -INFINITY ? 0.0f : to, f = fast_exp2(m[i] - base);
+      m[i] = to;
+      l[i] *= f;
+      x[i].x *= f, x[i].y *= f, x[i].z *= f, x[i].w *= f;
+#pragma unroll
+      for (int b = 0; b < B; ++b) {
+        const float w = fast_exp2(pm[i][b] - base);
+        l[i] = fmaf(pl[i][b], w, l[i]);
+        x[i].x = fmaf(y[i][b].x, w, x[i].x);
+        x[i].y = fmaf(y[i][b].y, w, x[i].y);
+        x[i].z = fmaf(y[i][b].z, w, x[i].z);
+        x[i].w = fmaf(y[i][b].w, w, x[i].w);
+      }
+    }
+  }
 }
 
 // WEIGHTS: adds the attention weights of every token to the cache's, given the rows' lse.
@@ -371,7 +438,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
   constexpr int R = 8 * NT, kStages = S::kStages;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  int64_t *share = reinterpret_cast<int64_t *>(smem + S::kShare);
+  int *share = reinterpret_cast<int *>(smem + S::kShare);
 
   uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBar) + warp * kStages;
   if (lane == 0) {
@@ -381,34 +448,31 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
   char *ring = smem + warp * kStages * S::kStage;
   int2 *stage_pages = reinterpret_cast<int2 *>(smem + S::kPages) + warp * kStages;
 
-  // this CTA's stretch of the units, and the sequence that it begins in
-  int64_t mine = 0, total = 0;
+  // this CTA's stretch of the units (the first `extra` CTAs have one more), and the sequence that it begins in
+  int mine = 0, total = 0;
   for (int s = tid; s < k.b.n_seqs; s += kAttnThreads) mine += Kv4Units<WEIGHTS>(k, kv4_seq(k.b, s, k.status)).all();
-  int64_t before = cta_scan(mine, &total, share);
-  if (total == 0) return;
-  const int64_t ctas = min((int64_t)gridDim.x, total);
-  if (blockIdx.x >= ctas) return;
-  const int64_t first_unit = total * blockIdx.x / ctas, end_unit = total * (blockIdx.x + 1) / ctas;
+  int before = cta_scan(mine, &total, share);
+  const int ctas = min((int)gridDim.x, total), cta = blockIdx.x;
+  if (cta >= ctas) return;
+  const int each = total / ctas, extra = total - each * ctas;
+  const int first_unit = each * cta + min(cta, extra), end_unit = first_unit + each + (cta < extra);
   __syncthreads();
-  int seq;
-  int64_t seq_unit;  // first unit of the sequence
+  int seq = k.b.n_seqs, seq_unit = 0;  // the sequence, its first unit
   if (k.b.n_seqs <= kAttnThreads) {
     if (first_unit >= before && first_unit < before + mine) {
       share[0] = tid;
       share[1] = before;
     }
     __syncthreads();
-    seq = (int)share[0];
+    seq = share[0];
     seq_unit = share[1];
   } else {
-    int64_t passed = 0;
-    seq = k.b.n_seqs;
-    seq_unit = 0;
+    int passed = 0;
     for (int base = 0; base < k.b.n_seqs; base += kAttnThreads) {
       const int s = base + tid;
-      const int64_t u = s < k.b.n_seqs ? Kv4Units<WEIGHTS>(k, kv4_seq(k.b, s, nullptr)).all() : 0;
-      int64_t some;
-      const int64_t at = passed + cta_scan(u, &some, share);
+      const int u = s < k.b.n_seqs ? Kv4Units<WEIGHTS>(k, kv4_seq(k.b, s, nullptr)).all() : 0;
+      int some;
+      const int at = passed + cta_scan(u, &some, share);
       if (first_unit >= passed + some) {
         passed += some;
         continue;
@@ -419,7 +483,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
         share[1] = at;
       }
       __syncthreads();
-      seq = (int)share[0];
+      seq = share[0];
       seq_unit = share[1];
       break;
     }
@@ -429,7 +493,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
   uint32_t phase = 0;
   bool lost = false;
 
-  for (int64_t unit = first_unit; unit < end_unit && seq < k.b.n_seqs;) {
+  for (int unit = first_unit; unit < end_unit && seq < k.b.n_seqs;) {
     const Kv4Seq q = kv4_seq(k.b, seq, nullptr);
     const Kv4Units<WEIGHTS> units(k, q);
     if (unit >= seq_unit + units.all()) {
@@ -441,9 +505,9 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
     const int rows = min(q.n_new, k.a.max_new) * k.group_heads;
     const int past = q.len - q.n_new + 1;  // tokens that the first new one sees
     // the part of one item that falls into the stretch
-    const int item = (int)((unit - seq_unit) / units.per), from = (int)((unit - seq_unit) % units.per);
-    const int upto = (int)min((int64_t)units.per, from + (end_unit - unit));
-    const int64_t item_unit = unit - from;
+    const int item = (unit - seq_unit) / units.per, from = (unit - seq_unit) - item * units.per;
+    const int upto = min(units.per, from + (end_unit - unit));
+    const int item_unit = unit - from;
     unit += upto - from;
     const int row_tiles = WEIGHTS ? 1 : units.items / k.c.kv_heads;
     const int head = item / row_tiles;
@@ -456,32 +520,37 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       const int begin = from * kUnitTokens, end = min(upto * kUnitTokens, seen);
       const int tiles = max((end - begin + kTileTokens - 1) / kTileTokens, 0);
       const int count = (tiles - warp + kAttnWarps - 1) / kAttnWarps;  // this warp's; <= 0: none
-      // pages of the next 32 of this warp's tiles, a tile to a lane
-      int page0 = 0, page1 = 0, fetched = 0;
+      // a lane knows where one of the next 32 of this warp's tiles stands, and starts its copy
+      constexpr int N = WEIGHTS ? S::kBlock / 2 : S::kBlock;  // of a block: its keys alone, or all
+      const uint8_t *src0 = nullptr, *src1 = nullptr;
+      int blocks = 0, fetched = 0;
+      int2 pages = make_int2(0, 0);
       auto fetch = [&]() {
         if (!(fetched & 31)) {
           const int at = begin + (warp + (fetched + lane) * kAttnWarps) * kTileTokens;
-          if (at < end) page0 = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, at, k.status), 0);
-          page1 = page0;
-          if (k.c.page_shift == 4 && at + kKv4Block < end)
-            page1 = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, at + kKv4Block, k.status), 0);
+          blocks = min(kTileBlocks, (end - at + kKv4Block - 1) / kKv4Block);
+          if (at < end) {
+            const int slot = at & ((1 << k.c.page_shift) - 1);
+            pages.x = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, at, k.status), 0);
+            src0 = kv4_block(k.c, pages.x, head, slot);
+            pages.y = pages.x;
+            src1 = src0 + S::kBlock;
+            if (k.c.page_shift == 4 && blocks > 1) {
+              pages.y = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, at + kKv4Block, k.status), 0);
+              src1 = kv4_block(k.c, pages.y, head, 0);
+            }
+          }
         }
-        const int at = begin + (warp + fetched * kAttnWarps) * kTileTokens, slot = at & ((1 << k.c.page_shift) - 1);
-        const int p0 = __shfl_sync(0xffffffffu, page0, fetched & 31), p1 = __shfl_sync(0xffffffffu, page1, fetched & 31);
-        if (lane == 0) {
-          constexpr int N = WEIGHTS ? S::kBlock / 2 : S::kBlock;  // keys alone, or all
+        if (lane == (fetched & 31)) {
           char *to = ring + stage_in * S::kStage;
           uint64_t *bar = &bars[stage_in];
-          const int blocks = min(kTileBlocks, (end - at + kKv4Block - 1) / kKv4Block);
-          if (WEIGHTS) stage_pages[stage_in] = make_int2(p0, p1);
+          if (WEIGHTS) stage_pages[stage_in] = pages;
           mbar_arrive_expect_tx(bar, (uint32_t)(blocks * N));
-          const uint8_t *src = kv4_block(k.c, p0, head, slot);
           if (!WEIGHTS && k.c.page_shift > 4) {  // the tile lies within a page
-            bulk_g2s(to, src, (uint32_t)(blocks * N), bar);
+            bulk_g2s(to, src0, (uint32_t)(blocks * N), bar);
           } else {
-            bulk_g2s(to, src, N, bar);
-            if (blocks > 1)
-              bulk_g2s(to + S::kBlock, k.c.page_shift > 4 ? src + S::kBlock : kv4_block(k.c, p1, head, 0), N, bar);
+            bulk_g2s(to, src0, N, bar);
+            if (blocks > 1) bulk_g2s(to + S::kBlock, src1, N, bar);
           }
         }
         stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
@@ -503,9 +572,11 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       }
       __syncthreads();
 
-      // base: what the exponentials of rows 2t, 2t + 1 refer to (the running maximum at its last rise, in powers of
-      // two; lse in the weights' pass), limit: where it has to rise
-      float factor[NT][2], base[NT][2], limit[NT][2], sum[NT][2];
+      // In powers of two: top, the maximum of rows 2t, 2t + 1 at its last rise, limit, where it has to rise again, and
+      // base, what the exponentials refer to: top - lift, where 2^lift brings the largest value scale into
+      // [2^10, 2^11), so that products with probabilities up to 2^4 stay below f16's largest.  (lse in the weights'
+      // pass.)  Outputs and sums are both in units of 2^base.
+      float factor[NT][2], base[NT][2], top[NT][2], sum[NT][2];
       int sees[NT][2];  // tokens that these rows see
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -514,7 +585,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
           const int n = nt * 8 + 2 * t + e, r = row0 + n;
           factor[nt][e] = reinterpret_cast<const float *>(smem + S::kFactor)[n];
           base[nt][e] = WEIGHTS ? reinterpret_cast<const float *>(smem + S::kLse)[n] : 0.0f;
-          limit[nt][e] = -INFINITY;
+          top[nt][e] = -INFINITY;
           sum[nt][e] = 0.0f;
           sees[nt][e] = min(r < rows ? min(past + r / k.group_heads, q.len) : q.len, end);
         }
@@ -527,7 +598,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
 #pragma unroll
           for (int m = 0; m < D / 16; ++m) o[nt][m][0] = o[nt][m][1] = o[nt][m][2] = o[nt][m][3] = 0.0f;
       }
-      float v_limit = 0.0f, v_up = 1.0f, v_down = 1.0f;  // value scales up to v_limit fit, times v_up; o is times v_up
+      float lift = 0.0f;
+      __half2 scale_limit = __floats2half2_rn(0.0f, 0.0f);  // value scales up to this one fit
 
       for (int i = 0; i < count; ++i) {
         const int at = begin + (warp + i * kAttnWarps) * kTileTokens;
@@ -551,7 +623,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
         }
 
         if constexpr (WEIGHTS) {
-          const int2 pages = stage_pages[stage_out];
+          const int2 pages_of = stage_pages[stage_out];
 #pragma unroll
           for (int b = 0; b < kTileBlocks; ++b) {
             float w[2] = {0.0f, 0.0f};
@@ -566,7 +638,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
               w[e] += __shfl_xor_sync(0xffffffffu, w[e], 2);
               const int tok = at + b * kKv4Block + kv4_token(g) + 8 * e;
               if (t == 0 && tok < end)
-                k.c.weights[(((int64_t)(b ? pages.y : pages.x) * k.c.kv_heads + head) << k.c.page_shift) +
+                k.c.weights[(((int64_t)(b ? pages_of.y : pages_of.x) * k.c.kv_heads + head) << k.c.page_shift) +
                             (tok & ((1 << k.c.page_shift) - 1))] += w[e];
             }
           }
@@ -580,7 +652,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
               float m = fmaxf(p[0][nt][e], p[0][nt][e + 2]);
 #pragma unroll
               for (int b = 1; b < kTileBlocks; ++b) m = fmaxf(m, fmaxf(p[b][nt][e], p[b][nt][e + 2]));
-              rise |= m * factor[nt][e] > limit[nt][e];
+              rise |= m * factor[nt][e] > top[nt][e] + 4.0f;
             }
           if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
@@ -593,11 +665,10 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
                 m *= factor[nt][e];
 #pragma unroll
                 for (int x = 4; x < 32; x *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-                const float old = limit[nt][e] == -INFINITY ? -INFINITY : base[nt][e];  // nothing seen so far
-                m = fmaxf(m, old);
-                const float to = m == -INFINITY ? 0.0f : m, f = fast_exp2(old - to);
-                base[nt][e] = to;
-                limit[nt][e] = m == -INFINITY ? m : m + 4.0f;
+                m = fmaxf(m, top[nt][e]);
+                const float f = m == -INFINITY ? 1.0f : fast_exp2(top[nt][e] - m);
+                top[nt][e] = m;
+                base[nt][e] = m == -INFINITY ? 0.0f : m - lift;
                 sum[nt][e] *= f;
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
@@ -605,6 +676,56 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
                   o[nt][d][e + 2] *= f;
                 }
               }
+          }
+          // value scales of this lane's tokens; what stands behind the last token is not a scale
+          float sv[kTileBlocks][2][NG];
+          __half2 big = __floats2half2_rn(0.0f, 0.0f);
+#pragma unroll
+          for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int tok = kv4_token(g) + 8 * e;
+              const char *at_scales = buf + b * S::kBlock + S::kBlock / 2 + 8 * D + tok * 2 * NG;
+              const bool there = whole || at + b * kKv4Block + tok < end;
+              __half2 h[NG > 1 ? NG / 2 : 1];
+              if constexpr (NG == 1) {
+                h[0] = __half2half2(*reinterpret_cast<const __half *>(at_scales));
+              } else {
+                uint32_t w[NG / 2];
+                lds<NG * 2>(at_scales, w);
+#pragma unroll
+                for (int x = 0; x < NG / 2; ++x) h[x] = *reinterpret_cast<const __half2 *>(&w[x]);
+              }
+#pragma unroll
+              for (int x = 0; x < (NG + 1) / 2; ++x) {
+                if (!there) h[x] = __floats2half2_rn(0.0f, 0.0f);
+                big = __hmax2(big, h[x]);
+                const float2 f = __half22float2(h[x]);
+                sv[b][e][2 * x] = f.x;
+                if constexpr (NG > 1) sv[b][e][2 * x + 1] = f.y;
+              }
+            }
+          if (__any_sync(0xffffffffu, !__hble2(big, scale_limit))) {
+            float all = fmaxf(__low2float(big), __high2float(big));
+#pragma unroll
+            for (int x = 4; x < 32; x *= 2) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
+            const int power = ilogbf(all);
+            const float to = (float)(10 - power), f = ldexpf(1.0f, (int)(to - lift));
+            const float most = ldexpf(2.0f, power) * (1.0f - 0x1p-11f);
+            scale_limit = __floats2half2_rn(most, most);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                base[nt][e] -= to - lift;
+                sum[nt][e] *= f;
+#pragma unroll
+                for (int d = 0; d < D / 16; ++d) {
+                  o[nt][d][e] *= f;
+                  o[nt][d][e + 2] *= f;
+                }
+              }
+            lift = to;
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -615,38 +736,6 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
                 p[b][nt][e] = fast_exp2(fmaf(p[b][nt][e], factor[nt][e & 1], -base[nt][e & 1]));
                 sum[nt][e & 1] += p[b][nt][e];
               }
-          // value scales of this lane's tokens
-          float sv[kTileBlocks][2][NG], big = 0.0f;
-#pragma unroll
-          for (int b = 0; b < kTileBlocks; ++b)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int tok = kv4_token(g) + 8 * e;
-              load_scales<NG>(buf + b * S::kBlock + S::kBlock / 2 + 8 * D + tok * 2 * NG, sv[b][e]);
-              const bool there = whole || at + b * kKv4Block + tok < end;  // what stands behind the last token is not
-#pragma unroll
-              for (int gr = 0; gr < NG; ++gr) {
-                sv[b][e][gr] = there ? sv[b][e][gr] : 0.0f;
-                big = fmaxf(big, sv[b][e][gr]);
-              }
-            }
-          if (__any_sync(0xffffffffu, big > v_limit)) {
-#pragma unroll
-            for (int x = 4; x < 32; x *= 2) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, x));
-            // the largest in [2^10, 2^11): with probabilities up to 2^4 below f16's largest; scales are normal in f32
-            const uint32_t power = __float_as_uint(big) >> 23;
-            const float old = v_down;
-            v_up = __uint_as_float((264u - power) << 23);
-            v_down = __uint_as_float((power - 10u) << 23);
-            const float f = v_limit == 0.0f ? 1.0f : old * v_up;
-            v_limit = __uint_as_float(((power + 1u) << 23) - 1u);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) o[nt][d][e] *= f;
-          }
 
           // value codes: a 32-bit word has this lane's pairs of four 16-element slices
           uint32_t v[kTileBlocks][4][D / 64];
@@ -666,7 +755,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
               for (int b = 0; b < kTileBlocks; ++b)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const float f = sv[b][e][m / M] * v_up;
+                  const float f = sv[b][e][m / M];
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt) {
                     const float x0 = p[b][nt][2 * e] * f, x1 = p[b][nt][2 * e + 1] * f;
@@ -734,9 +823,9 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
 #pragma unroll
             for (int m = 0; m < D / 16; ++m)
               *reinterpret_cast<float2 *>(part + (warp * R + n) * D + 16 * m + 2 * g) =
-                  make_float2(o[nt][m][e] * v_down, o[nt][m][e + 2] * v_down);
+                  make_float2(o[nt][m][e], o[nt][m][e + 2]);
             if (g == 0) {
-              stat[warp * 2 * R + n] = limit[nt][e] == -INFINITY ? -INFINITY : base[nt][e];
+              stat[warp * 2 * R + n] = top[nt][e] == -INFINITY ? -INFINITY : base[nt][e];
               stat[warp * 2 * R + R + n] = sum[nt][e];
             }
           }
@@ -754,7 +843,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
             k.a.lse[token * k.a.q_heads + h] = some ? (m + log2f(l)) * 0.693147180559945309f : -INFINITY;
         };
         const bool ends = upto == units.per;
-        float *out = kv4_partial(k, blockIdx.x, from == 0);
+        float *out = kv4_partial(k, cta, from == 0);
         for (int i = tid; i < R * D / 4; i += kAttnThreads) {
           const int n = i / (D / 4), d = i % (D / 4) * 4;
           if (row0 + n >= rows) break;
@@ -786,45 +875,54 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
         }
         if (from != 0 || !ends) {
           // the CTAs that the item's first and last unit fall to
-          auto cta_of = [&](int64_t u) {
-            int64_t c = u * ctas / total;
-            while (total * (c + 1) / ctas <= u) ++c;
-            while (total * c / ctas > u) --c;
-            return (int)c;
+          auto cta_of = [&](int u) {
+            const int more = extra * (each + 1);
+            return u < more ? u / (each + 1) : extra + (u - more) / each;
           };
           const int c0 = cta_of(item_unit), c1 = cta_of(item_unit + units.per - 1);
           uint32_t *counters = static_cast<uint32_t *>(k.a.workspace);
-          __threadfence();
-          __syncthreads();
-          if (tid == 0) {
-            const uint32_t done = atomicAdd(&counters[c0], 1u);
-            share[0] = done == (uint32_t)(c1 - c0);
-            if (share[0]) counters[c0] = 0;
-          }
-          __syncthreads();
-          if (share[0]) {  // the last: all parts are there
+          // whether this CTA is the last of `of` to arrive; all that the others wrote is then visible
+          auto last_of = [&](uint32_t *counter, int of) {
             __threadfence();
-            for (int i = tid; i < R * D / 4; i += kAttnThreads) {
-              const int n = i / (D / 4), d = i % (D / 4) * 4;
-              if (row0 + n >= rows) break;
-              float m = -INFINITY;
-#pragma unroll 4
-              for (int c = c0; c <= c1; ++c) m = fmaxf(m, __ldcg(kv4_partial(k, c, c == c0) + R * D + n));
-              const float to = m == -INFINITY ? 0.0f : m;
-              float l = 0.0f;
-              float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-              for (int c = c0; c <= c1; ++c) {
-                const float *in = kv4_partial(k, c, c == c0);
-                const float f = fast_exp2(__ldcg(in + R * D + n) - to);
-                const float4 y = __ldcg(reinterpret_cast<const float4 *>(in + n * D + d));
-                l = fmaf(__ldcg(in + R * D + R + n), f, l);
-                x.x = fmaf(y.x, f, x.x);
-                x.y = fmaf(y.y, f, x.y);
-                x.z = fmaf(y.z, f, x.z);
-                x.w = fmaf(y.w, f, x.w);
+            __syncthreads();
+            if (tid == 0) {
+              const bool last = atomicAdd(counter, 1u) == (uint32_t)of - 1u;
+              if (last) *counter = 0;
+              share[0] = last;
+            }
+            __syncthreads();
+            const bool last = share[0];
+            if (last) __threadfence();
+            return last;
+          };
+          // up to kJoin parts at once, then the groups' results, which take the place of their first parts
+          constexpr int I = R * D / 4 / kAttnThreads;
+          float4 x[I];
+          float m[I], l[I];
+          const int parts = c1 - c0 + 1, group = (cta - c0) / kJoin, head_cta = c0 + group * kJoin;
+          const int in_group = min(kJoin, parts - group * kJoin), groups = (parts + kJoin - 1) / kJoin;
+          bool last = last_of(counters + (group ? 2 : 1) * kAttnCtas + head_cta, in_group);
+          if (last) join_parts<D, R, I>(k, c0, head_cta, in_group, 1, x, m, l);
+          if (last && groups > 1) {
+            float *to = kv4_partial(k, head_cta, head_cta == c0);
+            __syncthreads();  // all have read the first part
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+              const int e = tid + i * kAttnThreads, n = e / (D / 4), d = e % (D / 4) * 4;
+              *reinterpret_cast<float4 *>(to + n * D + d) = x[i];
+              if (d == 0) {
+                to[R * D + n] = m[i];
+                to[R * D + R + n] = l[i];
               }
-              store(n, d, x, m, l);
+            }
+            last = last_of(counters + c0, groups);
+            if (last) join_parts<D, R, I>(k, c0, c0, groups, kJoin, x, m, l);
+          }
+          if (last) {
+#pragma unroll
+            for (int i = 0; i < I; ++i) {
+              const int e = tid + i * kAttnThreads, n = e / (D / 4), d = e % (D / 4) * 4;
+              if (row0 + n < rows) store(n, d, x[i], m[i], l[i]);
             }
           }
         }

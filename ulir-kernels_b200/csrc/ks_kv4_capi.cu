@@ -108,6 +108,7 @@ Kv4Plan plan_of(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_
   p.row_tiles = (int)((rows + p.rows_tile - 1) / p.rows_tile);
   const size_t units = n_seqs * v.kv_heads * p.row_tiles * ((max_len + kUnitTokens - 1) / kUnitTokens);
   const size_t ctas = kPlanSms * kv4_ctas_per_sm(p.rows_tile / 8, dtype == KS_B200_DTYPE_F32 ? 2 : 1);
+  static_assert(kPlanSms * 4 <= kAttnCtas && 3 * kAttnCtas <= kAttnCounters, "three counters to a CTA");
   p.ctas = (int)(units < ctas ? units : ctas);
   return p;
 }
@@ -115,7 +116,8 @@ Kv4Plan plan_of(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_
 bool attention_sizes_ok(const Kv4View &v, size_t q_heads, size_t n_seqs, size_t max_new, size_t max_len) {
   return q_heads > 0 && q_heads % v.kv_heads == 0 && q_heads <= kMost && n_seqs > 0 && n_seqs <= 65535 && max_new > 0 &&
          max_len > 0 && max_new <= max_len && max_len <= kMost - 1024 && max_new <= kMost / q_heads &&
-         n_seqs * max_new <= (size_t)1 << 40 && n_seqs * max_new * q_heads <= ((size_t)1 << 50) / (max_len / 128 + 1);
+         // units of work, a row tile of at least 8 rows and 128 tokens each, are counted in 31 bits
+         n_seqs * v.kv_heads <= kMost / (max_new * (q_heads / v.kv_heads) / 8 + 1) / (max_len / kUnitTokens + 1);
 }
 
 // The counters, then two parts of every CTA: for any type (f16 and bf16 have the most CTAs).
