@@ -7,9 +7,8 @@
 //           positive finite f16 values (1 if every element is 0)
 //   code  = clamp(rne(v / scale), -8, 7)
 // the rule of the Q4_0 importer with f16 scales.  Both roundings are decided
-// by the exact quotient: the scale's by one division in 64 bits, a code's by
-// the sign of v - x * scale where the f32 quotient x falls on a tie.  NaN
-// counts as 0 and an infinity as beyond every code; both are reported.
+// by the exact quotient.  NaN counts as 0 and an infinity as beyond every code;
+// both are reported.
 
 #include "ks_kv4.cuh"
 
@@ -17,227 +16,278 @@ namespace ksb {
 
 namespace {
 
-// The sequence whose rows hold packed row i (-1: none).  32-ary search, the
-// whole warp on one i.
+// The sequence whose rows hold packed row i (-1: none), by bisection.
 __device__ __forceinline__ int kv4_find_seq(const Kv4Batch &b, int i) {
   if (!b.offsets) return i < b.n_seqs ? i : -1;
   if (i < b.offsets[0] || i >= b.offsets[b.n_seqs]) return -1;
-  const int lane = threadIdx.x & 31;
-  int lo = 0, n = b.n_seqs;
-  while (n > 1) {
-    const int step = (n + 31) >> 5;
-    const int at = lane * step;
-    const unsigned le = __ballot_sync(0xffffffffu, at < n && b.offsets[lo + at] <= i);
-    const int c = le ? 31 - __clz(le) : 0;
-    lo += c * step;
-    n = min(step, n - c * step);
+  int lo = 0, hi = b.n_seqs;  // offsets[lo] <= i < offsets[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (b.offsets[mid] <= i)
+      lo = mid;
+    else
+      hi = mid;
   }
   return lo;
 }
 
-// Eight elements of one token and head per lane.  keys: lane l of head_dim / 8
-// has elements 8l .. 8l + 7, one word of the row's codes.  values: lane l =
-// g * (head_dim / 64) + a has elements 16 (4a + k) + 2g + {0, 1}, k = 0..3,
-// again one word.
+// Four threads have one token's keys or values of one head, D / 4 elements
+// each, which are D / 8 bytes in a row of the codes and 8 elements of every 32:
+//   keys    thread t: elements 32 w + 8 t .. + 7 of each w
+//   values  thread t: elements 16 i + 4 t .. + 3 of each i
+// Run r of a thread is the consecutive elements that one load or store moves.
 template <int D, bool V>
-__device__ __forceinline__ int kv4_element(int l, int k) {  // first element of pair k
-  if constexpr (!V) return 8 * l + 2 * k;
-  constexpr int A = D / 64;
-  return 16 * (4 * (l % A) + k) + 2 * (l / A);
-}
-template <int D, bool V>
-__device__ __forceinline__ int kv4_word(int l) {  // byte of that word in the row
-  if constexpr (!V) return (l & 3) * (D / 8) + (l >> 2) * 4;
-  return l * 4;
-}
+struct Kv4Runs {
+  static constexpr int kLength = V ? 4 : 8, kRuns = D / 4 / kLength;
+  static __device__ __forceinline__ int first(int t, int r) { return r * 4 * kLength + t * kLength; }
+  // Where element e of a thread's D / 4 (in order of the runs) has its nibble among the thread's words.
+  static __host__ __device__ constexpr int word(int e) { return V ? (e % 4 / 2) * (D / 64) + e / 4 / 4 : e / 8; }
+  static __host__ __device__ constexpr int shift(int e) { return V ? (e / 4 % 4) * 8 + (e % 2) * 4 : (e % 8) * 4; }
+};
 
-template <typename T>
-__device__ __forceinline__ void load_pair(const T *p, bool vec, float &a, float &b) {
+template <typename T, int N>
+__device__ __forceinline__ void load_run(const T *p, bool vec, float *v) {
+  constexpr int kBytes = N * sizeof(T);
   if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      const float2 v = *reinterpret_cast<const float2 *>(p);
-      a = v.x;
-      b = v.y;
-    } else {
-      const uint32_t v = *reinterpret_cast<const uint32_t *>(p);
-      const T x = reinterpret_cast<const T *>(&v)[0], y = reinterpret_cast<const T *>(&v)[1];
-      a = kv4_load(&x);
-      b = kv4_load(&y);
-    }
+    T x[N];
+    if constexpr (kBytes == 8)
+      *reinterpret_cast<uint2 *>(x) = *reinterpret_cast<const uint2 *>(p);
+    else
+#pragma unroll
+      for (int k = 0; k < kBytes / 16; ++k)
+        reinterpret_cast<uint4 *>(x)[k] = reinterpret_cast<const uint4 *>(p)[k];
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = kv4_load(&x[k]);
   } else {
-    a = kv4_load(p);
-    b = kv4_load(p + 1);
+#pragma unroll
+    for (int k = 0; k < N; ++k) v[k] = kv4_load(p + k);
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void store_pair(T *p, bool vec, float a, float b) {
-  T x, y;
-  kv4_store(&x, a);
-  kv4_store(&y, b);
+template <typename T, int N>
+__device__ __forceinline__ void store_run(T *p, bool vec, const float *v) {
+  constexpr int kBytes = N * sizeof(T);
+  T x[N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) kv4_store(&x[k], v[k]);
   if (vec) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float2 *>(p) = make_float2(a, b);
-    } else {
-      T v[2] = {x, y};
-      *reinterpret_cast<uint32_t *>(p) = *reinterpret_cast<uint32_t *>(v);
-    }
+    if constexpr (kBytes == 8)
+      *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(x);
+    else
+#pragma unroll
+      for (int k = 0; k < kBytes / 16; ++k)
+        reinterpret_cast<uint4 *>(p)[k] = reinterpret_cast<const uint4 *>(x)[k];
   } else {
-    p[0] = x;
-    p[1] = y;
+#pragma unroll
+    for (int k = 0; k < N; ++k) p[k] = x[k];
   }
 }
 
-// max(hi / 7, -lo / 8) in f16: one division and one rounding of the exact
-// quotient (a double holds enough bits of it that f16 rounds as from it).
+template <int BYTES>
+__device__ __forceinline__ void copy_words(void *to, const void *from) {
+  if constexpr (BYTES == 16)
+    *static_cast<uint4 *>(to) = *static_cast<const uint4 *>(from);
+  else
+    *static_cast<uint2 *>(to) = *static_cast<const uint2 *>(from);
+}
+
+// max(hi / 7, -lo / 8) in f16, as rounded from the exact quotient: where the
+// f32 quotient stands between two f16 values it may have been rounded there,
+// and below 2^-14 f16's steps are wider; the division is then made in 64 bits
+// (enough of them that f16 rounds as from the exact quotient).
 __device__ __forceinline__ __half kv4_scale(float lo, float hi) {
-  const double r = fmax((double)hi / 7.0, -(double)lo * 0.125);
-  if (r == 0.0) return __float2half_rn(1.0f);
-  return __double2half(fmin(fmax(r, 0x1p-24), 65504.0));
+  const float a = __fdiv_rn(hi, 7.0f), r = fmaxf(a, -lo * 0.125f);
+  if (hi == 0.0f && lo == 0.0f) return __float2half_rn(1.0f);
+  if (r >= 0x1p-14f && (__float_as_uint(a) & 0x1FFFu) != 0x1000u) return __float2half_rn(fminf(r, 65504.0f));
+  const double x = fmax((double)hi / 7.0, -(double)lo * 0.125);
+  return __double2half(fmin(fmax(x, 0x1p-24), 65504.0));
 }
 
-// clamp(rne(v / s), -8, 7) of the exact quotient, as a nibble.
-__device__ __forceinline__ uint32_t kv4_code(float v, float s) {
-  const float x = fminf(fmaxf(__fdiv_rn(v, s), -9.0f), 8.0f);
-  float q = rintf(x);
-  const float low = floorf(x);
-  if (x - low == 0.5f) {  // the f32 quotient is a tie: is the exact one beside it?
-    const float r = __fmaf_rn(-x, s, v);
-    if (r != 0.0f) q = r > 0.0f ? low + 1.0f : low;
+// clamp(rne(v / s), -8, 7) of the exact quotient, as a nibble in the lowest
+// bits of the result; inv = 1 / s.  v * inv is within 2^-20 of v / s, so only
+// next to a tie is the quotient itself needed, and where that falls on the tie
+// in f32 the sign of v - x * s says on which side it lies.
+__device__ __forceinline__ uint32_t kv4_code(float v, float s, float inv) {
+  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
+  float x = fminf(fmaxf(v * inv, -8.0f), 7.0f);
+  float y = __fadd_rn(x, kMagic);
+  if (fabsf(x - __fsub_rn(y, kMagic)) > 0.5f - 0x1p-14f) {
+    x = fminf(fmaxf(__fdiv_rn(v, s), -8.5f), 7.5f);
+    float q = rintf(x);
+    const float low = floorf(x), r = __fmaf_rn(-x, s, v);
+    if (x - low == 0.5f && r != 0.0f) q = r > 0.0f ? low + 1.0f : low;
+    y = __fadd_rn(fminf(fmaxf(q, -8.0f), 7.0f), kMagic);
   }
-  q = fminf(fmaxf(q, -8.0f), 7.0f);
-  return (uint32_t)((int)q) & 0xFu;
+  return __float_as_uint(y) & 15u;
 }
 
-// One CTA per (row of new tokens, keys or values); head_dim / 8 lanes per head.
-template <typename T, int D, bool V>
-__device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Batch &b, const T *x, int64_t token_stride,
-                                            int64_t head_stride, uint32_t *status) {
-  constexpr int L = D / 8, A = D / 64;
-  const int i = blockIdx.x, l = threadIdx.x % L;
-  const unsigned lanes = (L == 32 ? 0xffffffffu : ((1u << L) - 1u)) << ((threadIdx.x & 31) & ~(L - 1));
-  const int seq = kv4_find_seq(b, i);
-  if (seq < 0) return;
-  const Kv4Seq q = kv4_seq(b, seq, status);
-  const int pos = q.len - q.n_new + (i - q.first);
-  if (pos < 0 || i - q.first >= q.n_new) {  // more new tokens than the sequence has
-    set_status(status, kStatusBadScale);
-    return;
-  }
-  const int page = kv4_page(c, b.table, b.table_stride, seq, pos, status);
-  if (page < 0) return;
-  const int slot = pos & ((1 << c.page_shift) - 1);
-  const int group = D / c.groups;
-  for (int head = threadIdx.x / L; head < c.kv_heads; head += blockDim.x / L) {
-    const T *src = x + i * token_stride + head * head_stride;
-    const bool vec = (reinterpret_cast<uintptr_t>(src) & (2 * sizeof(T) - 1)) == 0;
-    float v[8];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) load_pair(src + kv4_element<D, V>(l, k), vec, v[2 * k], v[2 * k + 1]);
-    bool odd = false;
-    float hi[2] = {0.0f, 0.0f}, lo[2] = {0.0f, 0.0f};  // of elements 0..3 and 4..7
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      odd |= !isfinite(v[k]);
-      if (isnan(v[k])) v[k] = 0.0f;
-      hi[k / 4] = fmaxf(hi[k / 4], v[k]);
-      lo[k / 4] = fminf(lo[k / 4], v[k]);
-    }
-    if (odd) set_status(status, kStatusBadScale);
-    // over the lanes that share the group
-    if (!V || group >= 64) {
-      hi[0] = hi[1] = fmaxf(hi[0], hi[1]);
-      lo[0] = lo[1] = fminf(lo[0], lo[1]);
-    }
-    const int first = V ? A : 1, last = V ? 4 * A : group / 16;
-    auto share = [&](int o) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        hi[h] = fmaxf(hi[h], __shfl_xor_sync(lanes, hi[h], o));
-        lo[h] = fminf(lo[h], __shfl_xor_sync(lanes, lo[h], o));
+constexpr int kRowThreads = 256, kRowTokens = 32;  // tokens of a CTA, at most
+
+struct Kv4Place {
+  int page, slot;  // page -1: the row is left out
+};
+
+// Where the CTA's rows first .. first + tokens - 1 stand in the cache, one thread each.
+__device__ __forceinline__ void find_places(const Kv4View &c, const Kv4Batch &b, int first, int tokens,
+                                            Kv4Place *places, uint32_t *status) {
+  if ((int)threadIdx.x < tokens) {
+    const int i = first + threadIdx.x;
+    Kv4Place p{-1, 0};
+    const int seq = kv4_find_seq(b, i);
+    if (seq >= 0) {
+      const Kv4Seq q = kv4_seq(b, seq, status);
+      const int pos = q.len - q.n_new + (i - q.first);
+      if (pos < 0 || i - q.first >= q.n_new) {  // more new tokens than the sequence has
+        set_status(status, kStatusBadScale);
+      } else {
+        p.page = kv4_page(c, b.table, b.table_stride, seq, pos, status);
+        p.slot = pos & ((1 << c.page_shift) - 1);
       }
-    };
-    for (int o = first; o <= last; o *= 2) share(o);
-    if (V && group == 128) share(1);
-    const __half s[2] = {kv4_scale(lo[0], hi[0]), kv4_scale(lo[1], hi[1])};
-    const float sf[2] = {__half2float(s[0]), __half2float(s[1])};
-    uint32_t word = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) word |= kv4_code(v[k], sf[k / 4]) << (4 * k);
-    uint8_t *half = kv4_block(c, page, head, slot) + (V ? c.block_bytes / 2 : 0);
-    *reinterpret_cast<uint32_t *>(half + (slot & 15) * (D / 2) + kv4_word<D, V>(l)) = word;
-    __half *scales = reinterpret_cast<__half *>(half + 8 * D) + (slot & 15) * c.groups;
-    if (!V) {
-      if (l % (group / 8) == 0) scales[8 * l / group] = s[0];
-    } else if (l < A) {
-      if (group == 32) scales[2 * l] = s[0], scales[2 * l + 1] = s[1];
-      if (group == 64) scales[l] = s[0];
-      if (group == 128 && l == 0) scales[0] = s[0];
     }
-    if (!V && c.weights && l == 0) c.weights[(((int64_t)page * c.kv_heads + head) << c.page_shift) + slot] = 0.0f;
+    places[threadIdx.x] = p;
   }
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_append_kernel(Kv4View c, Kv4Batch b, Kv4Rows r, uint32_t *status) {
-  if (blockIdx.y == 0)
-    append_rows<T, D, false>(c, b, static_cast<const T *>(r.k), r.k_token, r.k_head, status);
-  else
-    append_rows<T, D, true>(c, b, static_cast<const T *>(r.v), r.v_token, r.v_head, status);
+  __syncthreads();
 }
 
 template <typename T, int D, bool V>
-__device__ __forceinline__ void read_rows(const Kv4View &c, const Kv4Batch &b, T *x, int64_t token_stride,
-                                          int64_t head_stride, uint32_t *status) {
-  constexpr int L = D / 8;
-  const int i = blockIdx.x, l = threadIdx.x % L;
-  const int seq = kv4_find_seq(b, i);
-  if (seq < 0) return;
-  const Kv4Seq q = kv4_seq(b, seq, status);
-  const int pos = q.len - q.n_new + (i - q.first);
-  if (pos < 0 || i - q.first >= q.n_new) {
-    set_status(status, kStatusBadScale);
-    return;
-  }
-  const int page = kv4_page(c, b.table, b.table_stride, seq, pos, status);
-  if (page < 0) return;
-  const int slot = pos & ((1 << c.page_shift) - 1);
-  const int group = D / c.groups;
-  for (int head = threadIdx.x / L; head < c.kv_heads; head += blockDim.x / L) {
-    const uint8_t *half = kv4_block(c, page, head, slot) + (V ? c.block_bytes / 2 : 0);
-    const uint32_t word =
-        *reinterpret_cast<const uint32_t *>(half + (slot & 15) * (D / 2) + kv4_word<D, V>(l)) ^ 0x88888888u;
-    const __half *scales = reinterpret_cast<const __half *>(half + 8 * D) + (slot & 15) * c.groups;
-    T *dst = x + i * token_stride + head * head_stride;
-    const bool vec = (reinterpret_cast<uintptr_t>(dst) & (2 * sizeof(T) - 1)) == 0;
+__device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *places, int first_row, int tokens,
+                                            const T *x, int64_t token_stride, int64_t head_stride, uint32_t *status) {
+  using R = Kv4Runs<D, V>;
+  constexpr int E = D / 4, G32 = D / 32;  // elements of a thread, groups of 32
+  const int group = D / c.groups, t = threadIdx.x & 3;
+  const unsigned lanes = 15u << (threadIdx.x & 28);
+  bool odd = false;
+  for (int i = threadIdx.x >> 2; i < tokens * c.kv_heads; i += kRowThreads / 4) {
+    const int token = i / c.kv_heads, head = i - token * c.kv_heads;
+    const T *src = x + (int64_t)(first_row + token) * token_stride + head * head_stride;
+    const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+    float v[E];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int e = kv4_element<D, V>(l, k);
-      const float s = __half2float(scales[e / group]);
-      const float lo = (float)((word >> (8 * k)) & 15u) - 8.0f, hi = (float)((word >> (8 * k + 4)) & 15u) - 8.0f;
-      store_pair(dst + e, vec, lo * s, hi * s);  // exact in f32
+    for (int r = 0; r < R::kRuns; ++r) load_run<T, R::kLength>(src + R::first(t, r), vec, v + r * R::kLength);
+    const Kv4Place p = places[token];
+    if (p.page < 0) continue;
+    // extremes of the thread's 8 elements of every 32 (e / 8 for both orders), then over the four threads
+    float lo[G32], hi[G32];
+#pragma unroll
+    for (int g = 0; g < G32; ++g) {
+      lo[g] = hi[g] = 0.0f;
+#pragma unroll
+      for (int e = 8 * g; e < 8 * g + 8; ++e) {
+        odd |= !isfinite(v[e]);
+        v[e] = isnan(v[e]) ? 0.0f : v[e];
+        lo[g] = fminf(lo[g], v[e]);
+        hi[g] = fmaxf(hi[g], v[e]);
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < G32; ++g)
+#pragma unroll
+      for (int o = 1; o < 4; o *= 2) {
+        lo[g] = fminf(lo[g], __shfl_xor_sync(lanes, lo[g], o));
+        hi[g] = fmaxf(hi[g], __shfl_xor_sync(lanes, hi[g], o));
+      }
+    if (group >= 64)
+#pragma unroll
+      for (int g = 0; g < G32; g += 2) {
+        lo[g] = lo[g + 1] = fminf(lo[g], lo[g + 1]);
+        hi[g] = hi[g + 1] = fmaxf(hi[g], hi[g + 1]);
+      }
+    if (group == 128) {
+      const float l = fminf(lo[0], lo[G32 - 1]), h = fmaxf(hi[0], hi[G32 - 1]);
+#pragma unroll
+      for (int g = 0; g < G32; ++g) lo[g] = l, hi[g] = h;
+    }
+    // thread t makes the scale of group of 32 t, all take it from there
+    float l = lo[0], h = hi[0];
+#pragma unroll
+    for (int g = 1; g < G32; ++g)
+      if (t == g) l = lo[g], h = hi[g];
+    const __half mine = kv4_scale(l, h);
+    const float scale = __half2float(mine), inverse = __fdiv_rn(1.0f, scale);
+    uint32_t words[D / 32];
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w) words[w] = 0;
+#pragma unroll
+    for (int g = 0; g < G32; ++g) {
+      const float s = __shfl_sync(lanes, scale, g, 4), inv = __shfl_sync(lanes, inverse, g, 4);
+#pragma unroll
+      for (int e = 8 * g; e < 8 * g + 8; ++e) words[R::word(e)] |= kv4_code(v[e], s, inv) << R::shift(e);
+    }
+    uint8_t *half = kv4_block(c, p.page, head, p.slot) + (V ? c.block_bytes / 2 : 0);
+    copy_words<D / 8>(half + (p.slot & 15) * (D / 2) + t * (D / 8), words);
+    const int each = group / 32;
+    if (t < G32 && t % each == 0)
+      reinterpret_cast<__half *>(half + 8 * D)[(p.slot & 15) * c.groups + t / each] = mine;
+    if (!V && c.weights && t == 0)
+      c.weights[(((int64_t)p.page * c.kv_heads + head) << c.page_shift) + p.slot] = 0.0f;
+  }
+  if (odd) set_status(status, kStatusBadScale);
+}
+
+template <typename T, int D, bool V>
+__device__ __forceinline__ void read_rows(const Kv4View &c, const Kv4Place *places, int first_row, int tokens, T *x,
+                                          int64_t token_stride, int64_t head_stride) {
+  using R = Kv4Runs<D, V>;
+  const int group = D / c.groups, t = threadIdx.x & 3;
+#pragma unroll 2
+  for (int i = threadIdx.x >> 2; i < tokens * c.kv_heads; i += kRowThreads / 4) {
+    const int token = i / c.kv_heads, head = i - token * c.kv_heads;
+    const Kv4Place p = places[token];
+    if (p.page < 0) continue;
+    const uint8_t *half = kv4_block(c, p.page, head, p.slot) + (V ? c.block_bytes / 2 : 0);
+    uint32_t words[D / 32];
+    copy_words<D / 8>(words, half + (p.slot & 15) * (D / 2) + t * (D / 8));
+    const __half *scales = reinterpret_cast<const __half *>(half + 8 * D) + (p.slot & 15) * c.groups;
+    float s[D / 32];
+#pragma unroll
+    for (int g = 0; g < D / 32; ++g) s[g] = __half2float(scales[32 * g / group]);
+    T *dst = x + (int64_t)(first_row + token) * token_stride + head * head_stride;
+    const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+#pragma unroll
+    for (int r = 0; r < R::kRuns; ++r) {
+      float v[R::kLength];
+#pragma unroll
+      for (int k = 0; k < R::kLength; ++k) {
+        const int e = r * R::kLength + k;
+        // the code in the top bits, its sign with it: an exact multiple of 2^28
+        const int code = (int)(words[R::word(e)] << (28 - R::shift(e))) >> 28;
+        v[k] = (float)code * s[e / 8];  // exact in f32
+      }
+      store_run<T, R::kLength>(dst + R::first(t, r), vec, v);
     }
   }
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) kv4_read_kernel(Kv4View c, Kv4Batch b, Kv4Rows r, uint32_t *status) {
-  if (blockIdx.y == 0)
-    read_rows<T, D, false>(c, b, static_cast<T *>(r.k), r.k_token, r.k_head, status);
-  else
-    read_rows<T, D, true>(c, b, static_cast<T *>(r.v), r.v_token, r.v_head, status);
+template <typename T, int D, bool READ>
+__global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(Kv4View c, Kv4Batch b, Kv4Rows r, int cta_tokens,
+                                                               uint32_t *status) {
+  __shared__ Kv4Place places[kRowTokens];
+  const int first = blockIdx.x * cta_tokens, tokens = min(cta_tokens, b.n_tokens - first);
+  find_places(c, b, first, tokens, places, status);
+  if constexpr (READ) {
+    if (blockIdx.y == 0)
+      read_rows<T, D, false>(c, places, first, tokens, static_cast<T *>(r.k), r.k_token, r.k_head);
+    else
+      read_rows<T, D, true>(c, places, first, tokens, static_cast<T *>(r.v), r.v_token, r.v_head);
+  } else {
+    if (blockIdx.y == 0)
+      append_rows<T, D, false>(c, places, first, tokens, static_cast<const T *>(r.k), r.k_token, r.k_head, status);
+    else
+      append_rows<T, D, true>(c, places, first, tokens, static_cast<const T *>(r.v), r.v_token, r.v_head, status);
+  }
 }
 
+// Tokens of a CTA: enough for its threads (four to a head) four times over,
+// fewer where that would leave SMs without a CTA.
 template <bool READ, int D>
 cudaError_t launch_rows(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, uint32_t *status, cudaStream_t stream) {
-  const dim3 grid((unsigned)b.n_tokens, 2);
-  const int want = (c.kv_heads * (D / 8) + 31) / 32 * 32, threads = want < 256 ? want : 256;
+  int tokens = 4 * kRowThreads / 4 / c.kv_heads;
+  tokens = tokens < 1 ? 1 : tokens > kRowTokens ? kRowTokens : tokens;
+  while (tokens > 1 && (b.n_tokens + tokens - 1) / tokens < 148) tokens /= 2;
+  const dim3 grid((unsigned)((b.n_tokens + tokens - 1) / tokens), 2);
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    if (READ)
-      kv4_read_kernel<T, D><<<grid, threads, 0, stream>>>(c, b, r, status);
-    else
-      kv4_append_kernel<T, D><<<grid, threads, 0, stream>>>(c, b, r, status);
+    kv4_rows_kernel<T, D, READ><<<grid, kRowThreads, 0, stream>>>(c, b, r, tokens, status);
   };
   if (r.dtype == kF32) go(0.0f);
   if (r.dtype == kF16) go(__half());

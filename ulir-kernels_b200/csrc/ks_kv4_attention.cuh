@@ -47,6 +47,8 @@
 // bits) is well below the result's own rounding.
 #pragma once
 
+#include <atomic>
+
 #include "ks_kv4.cuh"
 
 namespace ksb {
@@ -935,32 +937,37 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
 }
 
 template <typename T, int D, int NG, int NT, int QS, int PS, bool WEIGHTS>
-cudaError_t launch_kv4_attention_pass(const Kv4AttnArgs &k, cudaStream_t stream) {
+cudaError_t launch_kv4_attention_pass(const Kv4AttnArgs &k, cudaStream_t stream, int device) {
   constexpr int bytes = Kv4Smem<D, NG, NT, QS>::kBytes;
   auto *f = kv4_attention_kernel<T, D, NG, NT, QS, PS, WEIGHTS>;
-  cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e != cudaSuccess) return e;
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel may have that much shared memory
+  const uint64_t bit = (uint64_t)1 << (device & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    const cudaError_t e = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess) return e;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
   f<<<(unsigned)k.p.ctas, kAttnThreads, bytes, stream>>>(k);
   return cudaGetLastError();
 }
 
 template <typename T, int D, int NG, int NT, int QS, int PS>
-cudaError_t launch_kv4_attention_all(const Kv4AttnArgs &k, cudaStream_t stream) {
-  cudaError_t e = launch_kv4_attention_pass<T, D, NG, NT, QS, PS, false>(k, stream);
-  if (e == cudaSuccess && k.a.accumulate) e = launch_kv4_attention_pass<T, D, NG, NT, QS, PS, true>(k, stream);
+cudaError_t launch_kv4_attention_all(const Kv4AttnArgs &k, cudaStream_t stream, int device) {
+  cudaError_t e = launch_kv4_attention_pass<T, D, NG, NT, QS, PS, false>(k, stream, device);
+  if (e == cudaSuccess && k.a.accumulate) e = launch_kv4_attention_pass<T, D, NG, NT, QS, PS, true>(k, stream, device);
   return e;
 }
 
 // One translation unit per type: QS and PS as the precision note says.
 template <typename T, int QS, int PS>
-cudaError_t launch_kv4_attention_typed(const Kv4AttnArgs &k, cudaStream_t stream) {
+cudaError_t launch_kv4_attention_typed(const Kv4AttnArgs &k, cudaStream_t stream, int device) {
   const int key = k.c.head_dim * 100 + k.c.groups * 10 + k.p.rows_tile / 8;
   switch (key) {
 #define KS_KV4_CASE(D, NG)                                                   \
   case D * 100 + NG * 10 + 1:                                                \
-    return launch_kv4_attention_all<T, D, NG, 1, QS, PS>(k, stream);         \
+    return launch_kv4_attention_all<T, D, NG, 1, QS, PS>(k, stream, device);         \
   case D * 100 + NG * 10 + 2:                                                \
-    return launch_kv4_attention_all<T, D, NG, 2, QS, PS>(k, stream);
+    return launch_kv4_attention_all<T, D, NG, 2, QS, PS>(k, stream, device);
     KS_KV4_CASE(128, 4)
     KS_KV4_CASE(128, 2)
     KS_KV4_CASE(128, 1)
@@ -972,8 +979,8 @@ cudaError_t launch_kv4_attention_typed(const Kv4AttnArgs &k, cudaStream_t stream
   }
 }
 
-cudaError_t launch_kv4_attention_f32(const Kv4AttnArgs &k, cudaStream_t stream);
-cudaError_t launch_kv4_attention_f16(const Kv4AttnArgs &k, cudaStream_t stream);
-cudaError_t launch_kv4_attention_bf16(const Kv4AttnArgs &k, cudaStream_t stream);
+cudaError_t launch_kv4_attention_f32(const Kv4AttnArgs &k, cudaStream_t stream, int device);
+cudaError_t launch_kv4_attention_f16(const Kv4AttnArgs &k, cudaStream_t stream, int device);
+cudaError_t launch_kv4_attention_bf16(const Kv4AttnArgs &k, cudaStream_t stream, int device);
 
 }  // namespace ksb

@@ -4,8 +4,8 @@
 
 namespace ksb {
 
-cudaError_t launch_kv4_attention_bf16(const Kv4AttnArgs &k, cudaStream_t stream) {
-  return launch_kv4_attention_typed<__nv_bfloat16, 1, 1>(k, stream);
+cudaError_t launch_kv4_attention_bf16(const Kv4AttnArgs &k, cudaStream_t stream, int device) {
+  return launch_kv4_attention_typed<__nv_bfloat16, 1, 1>(k, stream, device);
 }
 
 }  // namespace ksb

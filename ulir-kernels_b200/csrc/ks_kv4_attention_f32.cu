@@ -4,8 +4,8 @@
 
 namespace ksb {
 
-cudaError_t launch_kv4_attention_f32(const Kv4AttnArgs &k, cudaStream_t stream) {
-  return launch_kv4_attention_typed<float, 2, 2>(k, stream);
+cudaError_t launch_kv4_attention_f32(const Kv4AttnArgs &k, cudaStream_t stream, int device) {
+  return launch_kv4_attention_typed<float, 2, 2>(k, stream, device);
 }
 
 }  // namespace ksb

@@ -235,9 +235,12 @@ extern "C" int ks_b200_kv4_attention_async(const ks_b200_kv4_cache *cache, const
   k.a.workspace = workspace;
   k.status = status;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == KS_B200_DTYPE_F32   ? launch_kv4_attention_f32(k, s)
-                        : dtype == KS_B200_DTYPE_F16 ? launch_kv4_attention_f16(k, s)
-                                                     : launch_kv4_attention_bf16(k, s);
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  e = dtype == KS_B200_DTYPE_F32   ? launch_kv4_attention_f32(k, s, device)
+      : dtype == KS_B200_DTYPE_F16 ? launch_kv4_attention_f16(k, s, device)
+                                   : launch_kv4_attention_bf16(k, s, device);
   return e == cudaSuccess ? KS_OK : cuda_fail(e, "kernel launch");
 }
 

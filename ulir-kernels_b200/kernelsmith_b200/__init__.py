@@ -393,15 +393,22 @@ def matvec_i8_batch_async(xs, ws, ys, w_stride, rows, cols, zx=0, zw=0, w_scales
     )
 
 
-_DTYPES = {"torch.float32": DTYPE_F32, "torch.float16": DTYPE_F16, "torch.bfloat16": DTYPE_BF16}
+class _Dtypes(dict):
+    """KS_B200_DTYPE_* by torch dtype, looked up by name once (torch itself is not imported here)."""
+
+    def __missing__(self, dtype):
+        names = {"torch.float32": DTYPE_F32, "torch.float16": DTYPE_F16, "torch.bfloat16": DTYPE_BF16}
+        if str(dtype) not in names:
+            raise ValueError(f"{dtype} is not float32, float16 or bfloat16")
+        return self.setdefault(dtype, names[str(dtype)])
 
 
-def _rows3(t) -> tuple[int, int, int]:
-    """Token and head strides and KS_B200_DTYPE_* of a [tokens, heads, head_dim] tensor."""
-    token, head, last = t.stride()
-    if last != 1:
-        raise ValueError("the last dimension must be contiguous")
-    return token, head, _DTYPES[str(t.dtype)]
+_DTYPES = _Dtypes()
+
+
+# The kv4 calls stand in a decode loop, so they take what they need from their tensors once and directly.
+def _at(t):
+    return None if t is None else t.data_ptr()
 
 
 class Kv4Cache(ctypes.Structure):
@@ -415,85 +422,80 @@ class Kv4Cache(ctypes.Structure):
     def __init__(self, pool, n_pages, page_size, kv_heads, head_dim, group_size, weights=None):
         super().__init__(addr(pool), addr(weights), n_pages, page_size, kv_heads, head_dim, group_size)
         self._tensors = (pool, weights)
+        self._row = (kv_heads, head_dim)
+        self._address = ctypes.addressof(self)
 
 
 def kv4_page_bytes(page_size, kv_heads, head_dim, group_size) -> int:
     return lib().ks_b200_kv4_page_bytes(page_size, kv_heads, head_dim, group_size)
 
 
+def _kv4_rows(call, cache, page_table, seq_lens, k, v, token_offsets, status, stream) -> None:
+    kt, kh, k1 = k.stride()
+    vt, vh, v1 = v.stride()
+    shape = k.shape
+    if k.dtype != v.dtype or shape != v.shape or shape[1:] != cache._row or k1 != 1 or v1 != 1:
+        raise ValueError("k and v must be [n_tokens, kv_heads, head_dim] of one type, the last dimension contiguous")
+    rc = call(cache._address, page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(), _at(token_offsets),
+              seq_lens.numel(), shape[0], k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DTYPES[k.dtype], _at(status),
+              stream_handle(stream))
+    if rc:
+        check(rc)
+
+
 def kv4_append_async(cache, page_table, seq_lens, k, v, token_offsets=None, status=None, stream=None) -> None:
     """Quantise the newest tokens of each sequence, k and v [n_tokens, kv_heads, head_dim], into the cache."""
-    kt, kh, dtype = _rows3(k)
-    vt, vh, vtype = _rows3(v)
-    if vtype != dtype or tuple(k.shape) != tuple(v.shape) or tuple(k.shape[1:]) != (cache.kv_heads, cache.head_dim):
-        raise ValueError("k and v must be [n_tokens, kv_heads, head_dim] of one type")
-    check(
-        lib().ks_b200_kv4_append_async(
-            ctypes.byref(cache), addr(page_table), page_table.stride(0), addr(seq_lens), addr(token_offsets),
-            seq_lens.numel(), k.shape[0], addr(k), kt, kh, addr(v), vt, vh, dtype, addr(status),
-            stream_handle(stream),
-        )
-    )
+    _kv4_rows(lib().ks_b200_kv4_append_async, cache, page_table, seq_lens, k, v, token_offsets, status, stream)
 
 
 def kv4_read_async(cache, page_table, seq_lens, k, v, token_offsets=None, status=None, stream=None) -> None:
     """Dequantise the newest tokens of each sequence into k and v [n_tokens, kv_heads, head_dim]."""
-    kt, kh, dtype = _rows3(k)
-    vt, vh, vtype = _rows3(v)
-    if vtype != dtype or tuple(k.shape) != tuple(v.shape) or tuple(k.shape[1:]) != (cache.kv_heads, cache.head_dim):
-        raise ValueError("k and v must be [n_tokens, kv_heads, head_dim] of one type")
-    check(
-        lib().ks_b200_kv4_read_async(
-            ctypes.byref(cache), addr(page_table), page_table.stride(0), addr(seq_lens), addr(token_offsets),
-            seq_lens.numel(), k.shape[0], addr(k), kt, kh, addr(v), vt, vh, dtype, addr(status),
-            stream_handle(stream),
-        )
-    )
+    _kv4_rows(lib().ks_b200_kv4_read_async, cache, page_table, seq_lens, k, v, token_offsets, status, stream)
 
 
 def kv4_attention_workspace(cache, q_heads, n_seqs, n_tokens, max_new, max_len) -> int:
-    return lib().ks_b200_kv4_attention_workspace(ctypes.byref(cache), q_heads, n_seqs, n_tokens, max_new, max_len)
+    return lib().ks_b200_kv4_attention_workspace(cache._address, q_heads, n_seqs, n_tokens, max_new, max_len)
 
 
 def kv4_attention_async(cache, page_table, seq_lens, q, out, scale, workspace, token_offsets=None, max_new=1,
                         max_len=None, lse=None, accumulate=False, status=None, stream=None) -> None:
     """Attention of the newest tokens, q and out [n_tokens, q_heads, head_dim], over the cache.  max_len: no
-    sequence is longer (default: what a row of the page table holds); workspace: a device byte tensor."""
-    qt, qh, dtype = _rows3(q)
-    ot, oh, otype = _rows3(out)
-    if otype != dtype or tuple(q.shape) != tuple(out.shape) or q.shape[2] != cache.head_dim:
-        raise ValueError("q and out must be [n_tokens, q_heads, head_dim] of one type")
-    if lse is not None and not (lse.is_contiguous() and tuple(lse.shape) == tuple(q.shape[:2])):
+    sequence is longer (default: what a row of the page table holds); workspace: a device byte tensor, zero-filled
+    before its first use."""
+    qt, qh, q1 = q.stride()
+    ot, oh, o1 = out.stride()
+    n_tokens, q_heads, head_dim = shape = q.shape
+    if q.dtype != out.dtype or shape != out.shape or head_dim != cache._row[1] or q1 != 1 or o1 != 1:
+        raise ValueError("q and out must be [n_tokens, q_heads, head_dim] of one type, the last dimension contiguous")
+    if lse is not None and (lse.shape != shape[:2] or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous f32 [n_tokens, q_heads]")
     stride = page_table.stride(0)
-    check(
-        lib().ks_b200_kv4_attention_async(
-            ctypes.byref(cache), addr(page_table), stride, addr(seq_lens), addr(token_offsets), seq_lens.numel(),
-            q.shape[0], max_new, stride * cache.page_size if max_len is None else max_len, addr(q), qt, qh,
-            q.shape[1], scale, addr(out), ot, oh, dtype, addr(lse), int(accumulate), addr(workspace),
-            workspace.numel(), addr(status), stream_handle(stream),
-        )
-    )
+    rc = lib().ks_b200_kv4_attention_async(
+        cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), seq_lens.numel(),
+        n_tokens, max_new, stride * cache.page_size if max_len is None else max_len, q.data_ptr(), qt, qh, q_heads,
+        scale, out.data_ptr(), ot, oh, _DTYPES[q.dtype], _at(lse), 1 if accumulate else 0, workspace.data_ptr(),
+        workspace.numel(), _at(status), stream_handle(stream))
+    if rc:
+        check(rc)
 
 
 def kv4_evict_workspace(cache, n_seqs, max_len, budget) -> int:
-    return lib().ks_b200_kv4_evict_workspace(ctypes.byref(cache), n_seqs, max_len, budget)
+    return lib().ks_b200_kv4_evict_workspace(cache._address, n_seqs, max_len, budget)
 
 
 def kv4_evict_async(cache, page_table, seq_lens, to_table, to_lens, max_len, budget, recent, workspace, kept=None,
                     status=None, stream=None) -> None:
     """Keep the newest `recent` tokens of each sequence and head and the heaviest others, `budget` in all, in the
     pages of to_table; kept: None or int32 [n_seqs, kv_heads, budget] for their old positions."""
-    if kept is not None and not (kept.is_contiguous() and tuple(kept.shape) == (seq_lens.numel(), cache.kv_heads,
-                                                                                budget)):
+    n_seqs = seq_lens.numel()
+    if kept is not None and (kept.shape != (n_seqs, cache._row[0], budget) or not kept.is_contiguous()):
         raise ValueError("kept must be a contiguous int32 [n_seqs, kv_heads, budget]")
-    check(
-        lib().ks_b200_kv4_evict_async(
-            ctypes.byref(cache), addr(page_table), page_table.stride(0), addr(seq_lens), seq_lens.numel(), max_len,
-            addr(to_table), to_table.stride(0), addr(to_lens), budget, recent, addr(kept), addr(workspace),
-            workspace.numel(), addr(status), stream_handle(stream),
-        )
-    )
+    rc = lib().ks_b200_kv4_evict_async(
+        cache._address, page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(), n_seqs, max_len,
+        to_table.data_ptr(), to_table.stride(0), to_lens.data_ptr(), budget, recent, _at(kept), workspace.data_ptr(),
+        workspace.numel(), _at(status), stream_handle(stream))
+    if rc:
+        check(rc)
 
 
 __all__ = [name for name in dir() if not name.startswith("_")]
