@@ -259,7 +259,7 @@ struct Kv4Evict {
 };
 size_t kv4_evict_workspace(const Kv4View &c, int n_seqs, int max_len, int budget);
 cudaError_t launch_kv4_evict(const Kv4View &c, const Kv4Batch &b, const Kv4Evict &e, uint32_t *status,
-                             cudaStream_t stream);
+                             cudaStream_t stream, int device);
 struct Kv4Attention {
   const void *q;
   void *out;

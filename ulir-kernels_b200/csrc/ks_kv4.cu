@@ -10,6 +10,8 @@
 // by the exact quotient.  NaN counts as 0 and an infinity as beyond every code;
 // both are reported.
 
+#include <atomic>
+
 #include "ks_kv4.cuh"
 
 namespace ksb {
@@ -103,22 +105,13 @@ __device__ __forceinline__ __half kv4_scale(float lo, float hi) {
   return __double2half(fmin(fmax(x, 0x1p-24), 65504.0));
 }
 
-// clamp(rne(v / s), -8, 7) of the exact quotient, as a nibble in the lowest
-// bits of the result; inv = 1 / s.  v * inv is within 2^-20 of v / s, so only
-// next to a tie is the quotient itself needed, and where that falls on the tie
-// in f32 the sign of v - x * s says on which side it lies.
-__device__ __forceinline__ uint32_t kv4_code(float v, float s, float inv) {
-  constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
-  float x = fminf(fmaxf(v * inv, -8.0f), 7.0f);
-  float y = __fadd_rn(x, kMagic);
-  if (fabsf(x - __fsub_rn(y, kMagic)) > 0.5f - 0x1p-14f) {
-    x = fminf(fmaxf(__fdiv_rn(v, s), -8.5f), 7.5f);
-    float q = rintf(x);
-    const float low = floorf(x), r = __fmaf_rn(-x, s, v);
-    if (x - low == 0.5f && r != 0.0f) q = r > 0.0f ? low + 1.0f : low;
-    y = __fadd_rn(fminf(fmaxf(q, -8.0f), 7.0f), kMagic);
-  }
-  return __float_as_uint(y) & 15u;
+// clamp(rne(v / s), -8, 7) of the exact quotient: where the f32 quotient falls
+// on a tie, the sign of v - x * s says on which side the exact one lies.
+__device__ __forceinline__ float kv4_code(float v, float s) {
+  const float x = fminf(fmaxf(__fdiv_rn(v, s), -8.5f), 7.5f), low = floorf(x), r = __fmaf_rn(-x, s, v);
+  float q = rintf(x);
+  if (x - low == 0.5f && r != 0.0f) q = r > 0.0f ? low + 1.0f : low;
+  return fminf(fmaxf(q, -8.0f), 7.0f);
 }
 
 constexpr int kRowThreads = 256, kRowTokens = 32;  // tokens of a CTA, at most
@@ -149,16 +142,48 @@ __device__ __forceinline__ void find_places(const Kv4View &c, const Kv4Batch &b,
   __syncthreads();
 }
 
-template <typename T, int D, bool V>
+// Of x[0 .. 2N), the lane keeps the extremes of its own and its partner's (lane ^ o) upper or lower N, in x[0 .. N).
+template <int N, bool MAX, int SIZE>
+__device__ __forceinline__ void hand_over(float (&x)[SIZE], int o, bool upper, unsigned lanes) {
+#pragma unroll
+  for (int g = 0; g < N; ++g) {
+    const float give = upper ? x[g] : x[g + N], keep = upper ? x[g + N] : x[g];
+    const float got = __shfl_xor_sync(lanes, give, o);
+    x[g] = MAX ? fmaxf(keep, got) : fminf(keep, got);
+  }
+}
+
+// Goes over the rows (token, head) of a CTA, kRowThreads / 4 at a time, without dividing each time.
+struct RowWalk {
+  int token, head, step_token, step_head, heads;
+  __device__ RowWalk(int row, int kv_heads) : heads(kv_heads) {
+    token = row / heads;
+    head = row - token * heads;
+    step_token = kRowThreads / 4 / heads;
+    step_head = kRowThreads / 4 - step_token * heads;
+  }
+  __device__ __forceinline__ void next() {
+    token += step_token;
+    head += step_head;
+    if (head >= heads) {
+      head -= heads;
+      ++token;
+    }
+  }
+};
+
+template <typename T, int D, int NG, bool V>
 __device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *places, int first_row, int tokens,
                                             const T *x, int64_t token_stride, int64_t head_stride, uint32_t *status) {
   using R = Kv4Runs<D, V>;
   constexpr int E = D / 4, G32 = D / 32;  // elements of a thread, groups of 32
-  const int group = D / c.groups, t = threadIdx.x & 3;
+  constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer, ties to even
+  constexpr int group = D / NG;
+  const int t = threadIdx.x & 3;
   const unsigned lanes = 15u << (threadIdx.x & 28);
   bool odd = false;
-  for (int i = threadIdx.x >> 2; i < tokens * c.kv_heads; i += kRowThreads / 4) {
-    const int token = i / c.kv_heads, head = i - token * c.kv_heads;
+  for (RowWalk at(threadIdx.x >> 2, c.kv_heads); at.token < tokens; at.next()) {
+    const int token = at.token, head = at.head;
     const T *src = x + (int64_t)(first_row + token) * token_stride + head * head_stride;
     const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
     float v[E];
@@ -166,133 +191,192 @@ __device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *pl
     for (int r = 0; r < R::kRuns; ++r) load_run<T, R::kLength>(src + R::first(t, r), vec, v + r * R::kLength);
     const Kv4Place p = places[token];
     if (p.page < 0) continue;
-    // extremes of the thread's 8 elements of every 32 (e / 8 for both orders), then over the four threads
-    float lo[G32], hi[G32];
+    // extremes of the thread's 8 elements of every 32 (e / 8 for both orders; NaN is passed over)
+    float lo[G32], hi[G32], zero = 0.0f;
 #pragma unroll
     for (int g = 0; g < G32; ++g) {
       lo[g] = hi[g] = 0.0f;
 #pragma unroll
       for (int e = 8 * g; e < 8 * g + 8; ++e) {
-        odd |= !isfinite(v[e]);
-        v[e] = isnan(v[e]) ? 0.0f : v[e];
+        zero = fmaf(v[e], 0.0f, zero);  // NaN if one is not finite
         lo[g] = fminf(lo[g], v[e]);
         hi[g] = fmaxf(hi[g], v[e]);
       }
     }
+    // over the four threads: each step hands the other half of the groups to the partner, thread t ends with group of
+    // 32 t (t % 2 where there are two), makes the scale of its group and all take it from there
+    if constexpr (G32 == 4) {
+      hand_over<2, false>(lo, 2, t & 2, lanes);
+      hand_over<2, true>(hi, 2, t & 2, lanes);
+    } else {
 #pragma unroll
-    for (int g = 0; g < G32; ++g)
-#pragma unroll
-      for (int o = 1; o < 4; o *= 2) {
-        lo[g] = fminf(lo[g], __shfl_xor_sync(lanes, lo[g], o));
-        hi[g] = fmaxf(hi[g], __shfl_xor_sync(lanes, hi[g], o));
+      for (int g = 0; g < 2; ++g) {
+        lo[g] = fminf(lo[g], __shfl_xor_sync(lanes, lo[g], 2));
+        hi[g] = fmaxf(hi[g], __shfl_xor_sync(lanes, hi[g], 2));
       }
-    if (group >= 64)
-#pragma unroll
-      for (int g = 0; g < G32; g += 2) {
-        lo[g] = lo[g + 1] = fminf(lo[g], lo[g + 1]);
-        hi[g] = hi[g + 1] = fmaxf(hi[g], hi[g + 1]);
-      }
-    if (group == 128) {
-      const float l = fminf(lo[0], lo[G32 - 1]), h = fmaxf(hi[0], hi[G32 - 1]);
-#pragma unroll
-      for (int g = 0; g < G32; ++g) lo[g] = l, hi[g] = h;
     }
-    // thread t makes the scale of group of 32 t, all take it from there
+    hand_over<1, false>(lo, 1, t & 1, lanes);
+    hand_over<1, true>(hi, 1, t & 1, lanes);
     float l = lo[0], h = hi[0];
 #pragma unroll
-    for (int g = 1; g < G32; ++g)
-      if (t == g) l = lo[g], h = hi[g];
+    for (int o = 1; 32 * o < group; o *= 2) {
+      l = fminf(l, __shfl_xor_sync(lanes, l, o));
+      h = fmaxf(h, __shfl_xor_sync(lanes, h, o));
+    }
     const __half mine = kv4_scale(l, h);
     const float scale = __half2float(mine), inverse = __fdiv_rn(1.0f, scale);
-    uint32_t words[D / 32];
+    // Codes are q = rne(v * (1 / s)), at most one beside rne(v / s) and that only next to a tie: then the remainder
+    // v - q * s (exact) is at least half of s.  Held scales (v / s may leave [-8.5, 7.5]) and values that are not
+    // finite go through the quotient.  A word is q + 8 in base 16, exact in f32 four codes at a time.
+    const bool plain = zero == 0.0f;
+    odd |= !plain;
+    float sums[D / 32][2];
 #pragma unroll
-    for (int w = 0; w < D / 32; ++w) words[w] = 0;
+    for (int w = 0; w < D / 32; ++w) sums[w][0] = sums[w][1] = 8388608.0f + 34952.0f;  // 2^23 + 0x8888
 #pragma unroll
     for (int g = 0; g < G32; ++g) {
-      const float s = __shfl_sync(lanes, scale, g, 4), inv = __shfl_sync(lanes, inverse, g, 4);
+      const float s = __shfl_sync(lanes, scale, g, 4), inv = __shfl_sync(lanes, inverse, g, 4), half = 0.5f * s;
+      float q[8], off = -1.0f;
 #pragma unroll
-      for (int e = 8 * g; e < 8 * g + 8; ++e) words[R::word(e)] |= kv4_code(v[e], s, inv) << R::shift(e);
+      for (int e = 0; e < 8; ++e) {
+        q[e] = __fsub_rn(__fadd_rn(v[8 * g + e] * inv, kMagic), kMagic);
+        off = fmaxf(off, fabsf(__fmaf_rn(-q[e], s, v[8 * g + e])) - half);
+      }
+      if (!plain || s >= 65504.0f || s < 0x1p-14f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[e] = kv4_code(isnan(v[8 * g + e]) ? 0.0f : v[8 * g + e], s);
+      } else if (off >= 0.0f) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float r = __fmaf_rn(-q[e], s, v[8 * g + e]);
+          const bool is_odd = __float_as_uint(q[e] + kMagic) & 1u;
+          if (fabsf(r) > half || (fabsf(r) == half && is_odd)) q[e] += copysignf(1.0f, r);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int n = R::shift(8 * g + e) / 4;
+        constexpr float kBase[4] = {1.0f, 16.0f, 256.0f, 4096.0f};
+        float &sum = sums[R::word(8 * g + e)][n / 4];
+        sum = fmaf(q[e], kBase[n % 4], sum);
+      }
     }
+    uint32_t words[D / 32];
+#pragma unroll
+    for (int w = 0; w < D / 32; ++w)
+      words[w] = prmt(__float_as_uint(sums[w][0]), __float_as_uint(sums[w][1]), 0x5410) ^ 0x88888888u;
     uint8_t *half = kv4_block(c, p.page, head, p.slot) + (V ? c.block_bytes / 2 : 0);
     copy_words<D / 8>(half + (p.slot & 15) * (D / 2) + t * (D / 8), words);
-    const int each = group / 32;
-    if (t < G32 && t % each == 0)
-      reinterpret_cast<__half *>(half + 8 * D)[(p.slot & 15) * c.groups + t / each] = mine;
+    constexpr int each = group / 32;
+    if (t < G32 && t % each == 0) reinterpret_cast<__half *>(half + 8 * D)[(p.slot & 15) * NG + t / each] = mine;
     if (!V && c.weights && t == 0)
       c.weights[(((int64_t)p.page * c.kv_heads + head) << c.page_shift) + p.slot] = 0.0f;
   }
   if (odd) set_status(status, kStatusBadScale);
 }
 
-template <typename T, int D, bool V>
+// The 8 codes of a word, in order of the nibbles.
+__device__ __forceinline__ void word_codes(uint32_t w, float (&f)[8]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    // 1024 + (code + 8), as f16, of nibbles k and k + 4
+    const uint32_t u = and_xor(w >> (4 * k), 0x000F000Fu, 0x64086408u);
+    const __half2 h = __hsub2(*reinterpret_cast<const __half2 *>(&u), __floats2half2_rn(1032.0f, 1032.0f));
+    const float2 x = __half22float2(h);
+    f[k] = x.x;
+    f[k + 4] = x.y;
+  }
+}
+
+template <typename T, int D, int NG, bool V>
 __device__ __forceinline__ void read_rows(const Kv4View &c, const Kv4Place *places, int first_row, int tokens, T *x,
                                           int64_t token_stride, int64_t head_stride) {
   using R = Kv4Runs<D, V>;
-  const int group = D / c.groups, t = threadIdx.x & 3;
-#pragma unroll 2
-  for (int i = threadIdx.x >> 2; i < tokens * c.kv_heads; i += kRowThreads / 4) {
-    const int token = i / c.kv_heads, head = i - token * c.kv_heads;
-    const Kv4Place p = places[token];
-    if (p.page < 0) continue;
-    const uint8_t *half = kv4_block(c, p.page, head, p.slot) + (V ? c.block_bytes / 2 : 0);
-    uint32_t words[D / 32];
-    copy_words<D / 8>(words, half + (p.slot & 15) * (D / 2) + t * (D / 8));
-    const __half *scales = reinterpret_cast<const __half *>(half + 8 * D) + (p.slot & 15) * c.groups;
-    float s[D / 32];
+  const int t = threadIdx.x & 3;
+  constexpr int N = 2;  // rows whose loads are under way together
+  for (RowWalk at(threadIdx.x >> 2, c.kv_heads); at.token < tokens;) {
+    uint32_t words[N][D / 32];
+    float s[N][D / 32];
+    T *dst[N];
 #pragma unroll
-    for (int g = 0; g < D / 32; ++g) s[g] = __half2float(scales[32 * g / group]);
-    T *dst = x + (int64_t)(first_row + token) * token_stride + head * head_stride;
-    const bool vec = (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+    for (int n = 0; n < N; ++n, at.next()) {
+      const int token = at.token, head = at.head;
+      dst[n] = nullptr;
+      if (token >= tokens || places[token].page < 0) continue;
+      const Kv4Place p = places[token];
+      const uint8_t *half = kv4_block(c, p.page, head, p.slot) + (V ? c.block_bytes / 2 : 0);
+      copy_words<D / 8>(words[n], half + (p.slot & 15) * (D / 2) + t * (D / 8));
+      float sc[NG];
+      load_scales<NG>(half + 8 * D + (p.slot & 15) * 2 * NG, sc);
 #pragma unroll
-    for (int r = 0; r < R::kRuns; ++r) {
-      float v[R::kLength];
+      for (int g = 0; g < D / 32; ++g) s[n][g] = sc[g * NG / (D / 32)];
+      dst[n] = x + (int64_t)(first_row + token) * token_stride + head * head_stride;
+    }
 #pragma unroll
-      for (int k = 0; k < R::kLength; ++k) {
-        const int e = r * R::kLength + k;
-        // the code in the top bits, its sign with it: an exact multiple of 2^28
-        const int code = (int)(words[R::word(e)] << (28 - R::shift(e))) >> 28;
-        v[k] = (float)code * s[e / 8];  // exact in f32
+    for (int n = 0; n < N; ++n) {
+      if (!dst[n]) continue;
+      float f[D / 32][8];
+#pragma unroll
+      for (int w = 0; w < D / 32; ++w) word_codes(words[n][w], f[w]);
+      const bool vec = (reinterpret_cast<uintptr_t>(dst[n]) & 15) == 0;
+#pragma unroll
+      for (int r = 0; r < R::kRuns; ++r) {
+        float v[R::kLength];
+#pragma unroll
+        for (int k = 0; k < R::kLength; ++k) {
+          const int e = r * R::kLength + k;
+          v[k] = f[R::word(e)][R::shift(e) / 4] * s[n][e / 8];  // exact in f32
+        }
+        store_run<T, R::kLength>(dst[n] + R::first(t, r), vec, v);
       }
-      store_run<T, R::kLength>(dst + R::first(t, r), vec, v);
     }
   }
 }
 
-template <typename T, int D, bool READ>
-__global__ void __launch_bounds__(kRowThreads) kv4_rows_kernel(Kv4View c, Kv4Batch b, Kv4Rows r, int cta_tokens,
-                                                               uint32_t *status) {
+template <typename T, int D, int NG, bool READ>
+__global__ void __launch_bounds__(kRowThreads, READ ? 4 : 3) kv4_rows_kernel(Kv4View c, Kv4Batch b, Kv4Rows r,
+                                                                              int cta_tokens, uint32_t *status) {
   __shared__ Kv4Place places[kRowTokens];
   const int first = blockIdx.x * cta_tokens, tokens = min(cta_tokens, b.n_tokens - first);
   find_places(c, b, first, tokens, places, status);
   if constexpr (READ) {
     if (blockIdx.y == 0)
-      read_rows<T, D, false>(c, places, first, tokens, static_cast<T *>(r.k), r.k_token, r.k_head);
+      read_rows<T, D, NG, false>(c, places, first, tokens, static_cast<T *>(r.k), r.k_token, r.k_head);
     else
-      read_rows<T, D, true>(c, places, first, tokens, static_cast<T *>(r.v), r.v_token, r.v_head);
+      read_rows<T, D, NG, true>(c, places, first, tokens, static_cast<T *>(r.v), r.v_token, r.v_head);
   } else {
     if (blockIdx.y == 0)
-      append_rows<T, D, false>(c, places, first, tokens, static_cast<const T *>(r.k), r.k_token, r.k_head, status);
+      append_rows<T, D, NG, false>(c, places, first, tokens, static_cast<const T *>(r.k), r.k_token, r.k_head, status);
     else
-      append_rows<T, D, true>(c, places, first, tokens, static_cast<const T *>(r.v), r.v_token, r.v_head, status);
+      append_rows<T, D, NG, true>(c, places, first, tokens, static_cast<const T *>(r.v), r.v_token, r.v_head, status);
   }
 }
 
 // Tokens of a CTA: enough for its threads (four to a head) four times over,
 // fewer where that would leave SMs without a CTA.
-template <bool READ, int D>
+template <bool READ, int D, int NG>
 cudaError_t launch_rows(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, uint32_t *status, cudaStream_t stream) {
   int tokens = 4 * kRowThreads / 4 / c.kv_heads;
   tokens = tokens < 1 ? 1 : tokens > kRowTokens ? kRowTokens : tokens;
   while (tokens > 1 && (b.n_tokens + tokens - 1) / tokens < 148) tokens /= 2;
   const dim3 grid((unsigned)((b.n_tokens + tokens - 1) / tokens), 2);
-  auto go = [&](auto zero) {
-    using T = decltype(zero);
-    kv4_rows_kernel<T, D, READ><<<grid, kRowThreads, 0, stream>>>(c, b, r, tokens, status);
-  };
-  if (r.dtype == kF32) go(0.0f);
-  if (r.dtype == kF16) go(__half());
-  if (r.dtype == kBF16) go(__nv_bfloat16());
+  if (r.dtype == kF32)
+    kv4_rows_kernel<float, D, NG, READ><<<grid, kRowThreads, 0, stream>>>(c, b, r, tokens, status);
+  else if (r.dtype == kF16)
+    kv4_rows_kernel<__half, D, NG, READ><<<grid, kRowThreads, 0, stream>>>(c, b, r, tokens, status);
+  else
+    kv4_rows_kernel<__nv_bfloat16, D, NG, READ><<<grid, kRowThreads, 0, stream>>>(c, b, r, tokens, status);
   return cudaGetLastError();
+}
+
+template <bool READ>
+cudaError_t launch_rows(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, uint32_t *status, cudaStream_t stream) {
+  if (c.head_dim == 64)
+    return c.groups == 1 ? launch_rows<READ, 64, 1>(c, b, r, status, stream)
+                         : launch_rows<READ, 64, 2>(c, b, r, status, stream);
+  return c.groups == 1   ? launch_rows<READ, 128, 1>(c, b, r, status, stream)
+         : c.groups == 2 ? launch_rows<READ, 128, 2>(c, b, r, status, stream)
+                         : launch_rows<READ, 128, 4>(c, b, r, status, stream);
 }
 
 // ------------------------------------------------------------------ eviction
@@ -303,7 +387,8 @@ cudaError_t launch_rows(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, u
 // is kept by four 8-bit passes over the weights as order-preserving integers
 // and lists the positions in order; a second moves the tokens.  The first
 // writes only the workspace, so to_lens may be the sequences' own lengths.
-constexpr int kSelectThreads = 512;
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectShared = 200 * 1024;  // keys that fit stay in shared memory
 
 struct EvictWorkspace {
   uint32_t *keys;  // [seq][head][max_len]
@@ -326,7 +411,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sums over the CTA of two counts below 2^16 each, packed.
+// Exclusive sums over the CTA (also of two counts below 2^16 each, packed).
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *total, uint32_t *shared) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   uint32_t sum = v;
@@ -348,9 +433,11 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *total, uint
   return before + sum - v;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4View c, Kv4Batch b, Kv4Evict e,
+__global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4View c, Kv4Batch b, Kv4Evict e, bool shared,
                                                                     uint32_t *status) {
-  __shared__ uint32_t hist[256], scan[kSelectThreads / 32], found[2];
+  constexpr int kBins = 2048;
+  __shared__ uint32_t hist[kBins], scan[kSelectThreads / 32], found[2];
+  extern __shared__ uint32_t shared_keys[];
   const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
   int len = b.lens[seq];
   if (len < 0 || len > b.max_len) {
@@ -360,7 +447,7 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4View c, K
   const EvictWorkspace ws =
       evict_workspace(e.workspace, (int64_t)b.n_seqs * c.kv_heads, b.max_len, e.budget);
   const int64_t row = (int64_t)seq * c.kv_heads + head;
-  uint32_t *keys = ws.keys + row * b.max_len;
+  uint32_t *keys = shared ? shared_keys : ws.keys + row * b.max_len;
   int32_t *list = ws.list + row * e.budget;
   const int count = min(len, e.budget);
   if (head == 0 && tid == 0) ws.count[seq] = count;
@@ -371,47 +458,47 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4View c, K
   const int old = len - e.recent, want = e.budget - e.recent;
   for (int i = tid; i < e.recent; i += kSelectThreads) list[want + i] = old + i;
   if (want == 0) return;
+  for (int i = tid; i < kBins; i += kSelectThreads) hist[i] = 0;
+  __syncthreads();
+#pragma unroll 4
   for (int i = tid; i < old; i += kSelectThreads) {
     const int page = kv4_page(c, b.table, b.table_stride, seq, i, status);
     const int slot = i & ((1 << c.page_shift) - 1);
-    keys[i] = page < 0 ? 0u : weight_key(c.weights[(((int64_t)page * c.kv_heads + head) << c.page_shift) + slot]);
+    const uint32_t k =
+        page < 0 ? 0u : weight_key(c.weights[(((int64_t)page * c.kv_heads + head) << c.page_shift) + slot]);
+    keys[i] = k;
+    atomicAdd(&hist[k >> 21], 1u);
   }
-  // the want-th largest key, byte by byte: `rank` of the keys with this prefix are still wanted
+  // the want-th largest key, digit by digit: `rank` of the keys with this prefix are still wanted
   uint32_t prefix = 0;
   int rank = want;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelectThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = tid; i < old; i += kSelectThreads) {
-      const uint32_t k = keys[i];
-      if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(k >> shift) & 255u], 1u);
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bins = pass == 2 ? 1024 : kBins;
+    if (pass > 0) {
+      for (int i = tid; i < bins; i += kSelectThreads) hist[i] = 0;
+      __syncthreads();
+      const int known = pass == 1 ? 21 : 10;
+      for (int i = tid; i < old; i += kSelectThreads) {
+        const uint32_t k = keys[i];
+        if (k >> known == prefix >> known) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
+      }
     }
     __syncthreads();
-    if (tid < 32) {  // lane l has bins 255 - 8l .. 248 - 8l
-      uint32_t n[8], sum = 0;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) sum += n[k] = hist[255 - 8 * tid - k];
-      uint32_t upto = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o *= 2) {
-        const uint32_t m = __shfl_up_sync(0xffffffffu, upto, o);
-        if (tid >= o) upto += m;
-      }
-      uint32_t before = upto - sum;
-      if (before < (uint32_t)rank && upto >= (uint32_t)rank) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if (before < (uint32_t)rank && before + n[k] >= (uint32_t)rank) {
-            found[0] = 255u - 8 * tid - k;
-            found[1] = before;
-          }
-          before += n[k];
-        }
-      }
+    // thread t has the bins bins - 1 - 2t and below it, from the largest down
+    const int top = bins - 1 - 2 * tid;
+    const uint32_t n0 = top >= 0 ? hist[top] : 0u, n1 = top >= 1 ? hist[top - 1] : 0u;
+    uint32_t all;
+    const uint32_t before = block_scan(n0 + n1, &all, scan);
+    if (before < (uint32_t)rank && before + n0 + n1 >= (uint32_t)rank) {
+      const bool second = before + n0 < (uint32_t)rank;
+      found[0] = (uint32_t)(top - second);
+      found[1] = before + (second ? n0 : 0u);
     }
     __syncthreads();
     prefix |= found[0] << shift;
     rank -= (int)found[1];
+    __syncthreads();
   }
   // `rank` tokens with exactly that key are kept, those of the lowest positions
   constexpr int kEach = 8;
@@ -444,43 +531,79 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4View c, K
   }
 }
 
-// Moves tokens, eight lanes each: the codes in 16-byte pieces (head_dim / 32
-// of keys and as many of values, a lane each), the scales and the weight by
-// three of the lanes.
-constexpr int kMoveThreads = 256, kMoveTokens = kMoveThreads / 8;
+// Moves 128 tokens of a head: a thread each for where they are and go, their
+// weight and list entry, then eight lanes to a token for the codes in 16-byte
+// pieces (head_dim / 32 of keys and as many of values) and the scales, all of a
+// thread's loads before its stores.
+constexpr int kMoveThreads = 256, kMoveTokens = 128;
 
+template <int D>
 __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(Kv4View c, Kv4Batch b, Kv4Evict e, uint32_t *status) {
-  const int head = blockIdx.y, seq = blockIdx.z, l = threadIdx.x & 7;
-  const int to = blockIdx.x * kMoveTokens + (threadIdx.x >> 3);
+  __shared__ uint8_t *rows[kMoveTokens][2];  // source and destination: the token's row of key codes
+  __shared__ int slots[kMoveTokens];         // their slots in the blocks, 16 * source + destination; -1: none
+  const int head = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x, base = blockIdx.x * kMoveTokens;
   const EvictWorkspace ws =
       evict_workspace(e.workspace, (int64_t)b.n_seqs * c.kv_heads, b.max_len, e.budget);
   const int count = ws.count[seq];
-  if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0) e.to_lens[seq] = count;
-  if (to >= count) return;
-  const int64_t row = ((int64_t)seq * c.kv_heads + head) * e.budget;
-  const int from = ws.list[row + to];
-  if (e.kept && l == 0) e.kept[row + to] = from;
-  const int src = kv4_page(c, b.table, b.table_stride, seq, from, status);
-  const int dst = kv4_page(c, e.to_table, e.to_stride, seq, to, status);
-  if (src < 0 || dst < 0) return;
-  const int mask = (1 << c.page_shift) - 1, s = from & mask, t = to & mask;
-  const uint8_t *sb = kv4_block(c, src, head, s);
-  uint8_t *db = kv4_block(c, dst, head, t);
-  const int codes = c.head_dim / 2, half = c.block_bytes / 2, pieces = codes / 16;
-  if (l < 2 * pieces) {
-    const int o = (l < pieces ? 0 : half) + (l % pieces) * 16;
-    *reinterpret_cast<uint4 *>(db + o + (t & 15) * codes) =
-        *reinterpret_cast<const uint4 *>(sb + o + (s & 15) * codes);
+  if (blockIdx.x == 0 && head == 0 && tid == 0) e.to_lens[seq] = count;
+  if (base >= count) return;
+  if (tid < kMoveTokens) {
+    int slot = -1;
+    const int to = base + tid;
+    if (to < count) {
+      const int64_t row = ((int64_t)seq * c.kv_heads + head) * e.budget;
+      const int from = ws.list[row + to];
+      if (e.kept) e.kept[row + to] = from;
+      const int src = kv4_page(c, b.table, b.table_stride, seq, from, status);
+      const int dst = kv4_page(c, e.to_table, e.to_stride, seq, to, status);
+      if (src >= 0 && dst >= 0) {
+        const int mask = (1 << c.page_shift) - 1, s = from & mask, t = to & mask;
+        rows[tid][0] = kv4_block(c, src, head, s) + (s & 15) * (D / 2);
+        rows[tid][1] = kv4_block(c, dst, head, t) + (t & 15) * (D / 2);
+        slot = (s & 15) * 16 + (t & 15);
+        c.weights[(((int64_t)dst * c.kv_heads + head) << c.page_shift) + t] =
+            c.weights[(((int64_t)src * c.kv_heads + head) << c.page_shift) + s];
+      }
+    }
+    slots[tid] = slot;
   }
-  if (l < 2) {
-    const int o = l * half + 16 * codes;
-    const __half *ss = reinterpret_cast<const __half *>(sb + o) + (s & 15) * c.groups;
-    __half *ds = reinterpret_cast<__half *>(db + o) + (t & 15) * c.groups;
-    for (int g = 0; g < c.groups; ++g) ds[g] = ss[g];
+  __syncthreads();
+  constexpr int kPieces = D / 32, kEach = kMoveTokens * 8 / kMoveThreads;
+  const int l = tid & 7, half = c.block_bytes / 2, piece = (l < kPieces ? 0 : half) + (l % kPieces) * 16;
+  const bool code = l < 2 * kPieces;
+  uint4 data[kEach];
+  uint2 scale[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = (tid >> 3) + k * (kMoveThreads / 8), slot = slots[i];
+    if (slot < 0) continue;
+    const uint8_t *src = rows[i][0];
+    if (code) data[k] = *reinterpret_cast<const uint4 *>(src + piece);
+    if (l < 2) {  // behind the block's 16 rows of codes
+      const uint8_t *from = src - (slot >> 4) * (D / 2) + 8 * D + l * half + (slot >> 4) * 2 * c.groups;
+      if (c.groups == 4)
+        scale[k] = *reinterpret_cast<const uint2 *>(from);
+      else if (c.groups == 2)
+        scale[k].x = *reinterpret_cast<const uint32_t *>(from);
+      else
+        scale[k].x = *reinterpret_cast<const uint16_t *>(from);
+    }
   }
-  if (l == 2) {
-    c.weights[(((int64_t)dst * c.kv_heads + head) << c.page_shift) + t] =
-        c.weights[(((int64_t)src * c.kv_heads + head) << c.page_shift) + s];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    const int i = (tid >> 3) + k * (kMoveThreads / 8), slot = slots[i];
+    if (slot < 0) continue;
+    uint8_t *dst = rows[i][1];
+    if (code) *reinterpret_cast<uint4 *>(dst + piece) = data[k];
+    if (l < 2) {
+      uint8_t *to = dst - (slot & 15) * (D / 2) + 8 * D + l * half + (slot & 15) * 2 * c.groups;
+      if (c.groups == 4)
+        *reinterpret_cast<uint2 *>(to) = scale[k];
+      else if (c.groups == 2)
+        *reinterpret_cast<uint32_t *>(to) = scale[k].x;
+      else
+        *reinterpret_cast<uint16_t *>(to) = (uint16_t)scale[k].x;
+    }
   }
 }
 
@@ -488,14 +611,12 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(Kv4View c, Kv4Ba
 
 cudaError_t launch_kv4_append(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, uint32_t *status,
                               cudaStream_t stream) {
-  return c.head_dim == 128 ? launch_rows<false, 128>(c, b, r, status, stream)
-                           : launch_rows<false, 64>(c, b, r, status, stream);
+  return launch_rows<false>(c, b, r, status, stream);
 }
 
 cudaError_t launch_kv4_read(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, uint32_t *status,
                             cudaStream_t stream) {
-  return c.head_dim == 128 ? launch_rows<true, 128>(c, b, r, status, stream)
-                           : launch_rows<true, 64>(c, b, r, status, stream);
+  return launch_rows<true>(c, b, r, status, stream);
 }
 
 size_t kv4_evict_workspace(const Kv4View &c, int n_seqs, int max_len, int budget) {
@@ -504,13 +625,27 @@ size_t kv4_evict_workspace(const Kv4View &c, int n_seqs, int max_len, int budget
 }
 
 cudaError_t launch_kv4_evict(const Kv4View &c, const Kv4Batch &b, const Kv4Evict &e, uint32_t *status,
-                             cudaStream_t stream) {
-  kv4_select_kernel<<<dim3((unsigned)c.kv_heads, (unsigned)b.n_seqs), kSelectThreads, 0, stream>>>(c, b, e, status);
+                             cudaStream_t stream, int device) {
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel may have that much shared memory
+  const uint64_t bit = (uint64_t)1 << (device & 63);
+  if (!(ready.load(std::memory_order_relaxed) & bit)) {
+    const cudaError_t err =
+        cudaFuncSetAttribute(kv4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectShared);
+    if (err != cudaSuccess) return err;
+    ready.fetch_or(bit, std::memory_order_relaxed);
+  }
+  const int64_t bytes = (int64_t)b.max_len * 4;
+  const bool shared = bytes <= kSelectShared;
+  kv4_select_kernel<<<dim3((unsigned)c.kv_heads, (unsigned)b.n_seqs), kSelectThreads, shared ? (size_t)bytes : 0,
+                      stream>>>(c, b, e, shared, status);
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   const int most = e.budget < b.max_len ? e.budget : b.max_len;
   const dim3 grid((unsigned)((most + kMoveTokens - 1) / kMoveTokens), (unsigned)c.kv_heads, (unsigned)b.n_seqs);
-  kv4_move_kernel<<<grid, kMoveThreads, 0, stream>>>(c, b, e, status);
+  if (c.head_dim == 128)
+    kv4_move_kernel<128><<<grid, kMoveThreads, 0, stream>>>(c, b, e, status);
+  else
+    kv4_move_kernel<64><<<grid, kMoveThreads, 0, stream>>>(c, b, e, status);
   return cudaGetLastError();
 }
 

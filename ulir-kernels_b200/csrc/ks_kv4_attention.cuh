@@ -121,44 +121,6 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   return d;
 }
 
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&h);
-}
-__device__ __forceinline__ float2 unpack_f16(uint32_t v) {
-  return __half22float2(*reinterpret_cast<const __half2 *>(&v));
-}
-
-template <int BYTES>
-__device__ __forceinline__ void lds(const void *p, uint32_t (&w)[BYTES / 4]) {
-  if constexpr (BYTES == 16) {
-    const uint4 v = *static_cast<const uint4 *>(p);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-  } else if constexpr (BYTES == 8) {
-    const uint2 v = *static_cast<const uint2 *>(p);
-    w[0] = v.x, w[1] = v.y;
-  } else {
-    w[0] = *static_cast<const uint32_t *>(p);
-  }
-}
-
-// The NG scales of one token.
-template <int NG>
-__device__ __forceinline__ void load_scales(const void *p, float (&s)[NG]) {
-  const __half *h = static_cast<const __half *>(p);
-  if constexpr (NG == 1) {
-    s[0] = __half2float(h[0]);
-  } else {
-    uint32_t w[NG / 2];
-    lds<NG * 2>(p, w);
-#pragma unroll
-    for (int k = 0; k < NG / 2; ++k) {
-      const float2 v = unpack_f16(w[k]);
-      s[2 * k] = v.x, s[2 * k + 1] = v.y;
-    }
-  }
-}
-
 // Row g of the products' token side is token kv4_token(g) of the block: any
 // order serves, and with 0 1 3 2 4 5 7 6 the 16-byte loads of the keys (two
 // rows, 64 bytes apart or an odd multiple of it, to a quarter warp) meet no

@@ -278,6 +278,9 @@ extern "C" int ks_b200_kv4_evict_async(const ks_b200_kv4_cache *cache, const int
   if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
     return fail(KS_ERR_WORKSPACE, "workspace smaller than ks_b200_kv4_evict_workspace, or not 16-byte aligned");
   const Kv4Evict e{to_table, (int64_t)to_table_stride, to_lens, kept, (int)budget, (int)recent, workspace};
-  const cudaError_t err = launch_kv4_evict(v, b, e, status, static_cast<cudaStream_t>(stream));
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return cuda_fail(err, "cudaGetDevice");
+  err = launch_kv4_evict(v, b, e, status, static_cast<cudaStream_t>(stream), device);
   return err == cudaSuccess ? KS_OK : cuda_fail(err, "kernel launch");
 }
