@@ -15,7 +15,9 @@
 // output, f32) in the workspace; the last of them to finish joins the parts in
 // their order, so results do not depend on which one that is.  Within a CTA
 // four warps take turns at tiles of 32 tokens, each through a ring of its own
-// in shared memory that bulk copies fill.
+// in shared memory that its lanes fill by asynchronous 16-byte copies (a bulk
+// copy for each tile, issued by one lane, held its warp up for some 400 cycles
+// of about 3000 that it spends on a tile, ten of these copies for about 60).
 //
 // Products.  Both run on the tensor cores with the tokens' codes as the A
 // operand, made in registers, and the query rows as the 8-wide N side, so that
@@ -115,6 +117,10 @@ __device__ __forceinline__ void mma_f16_from(float (&d)[4], uint32_t a0, uint32_
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x), "f"(c.y), "f"(c.z), "f"(c.w));
 }
 
+__device__ __forceinline__ void copy16_async(void *to, const void *from) {
+  asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(smem_u32(to)), "l"(from) : "memory");
+}
+
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t d;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
@@ -138,9 +144,7 @@ struct Kv4Smem {
   static constexpr int kCorr = kQ + NT * (D / 32) * QS * 512;       // NT x NG x QS x 4 float4
   static constexpr int kFactor = kCorr + NT * NG * QS * 64;        // 8 NT f32
   static constexpr int kLse = kFactor + 8 * NT * 4;                 // 8 NT f32
-  static constexpr int kPages = kLse + 8 * NT * 4;                  // pages of a stage's blocks
-  static constexpr int kBar = kPages + kAttnWarps * kStages * 8;    // mbarriers
-  static constexpr int kShare = kBar + kAttnWarps * kStages * 8;    // 8 words
+  static constexpr int kShare = kLse + 8 * NT * 4;                  // 8 words
   static constexpr int kBytes = kShare + 32;
 };
 
@@ -404,14 +408,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   int *share = reinterpret_cast<int *>(smem + S::kShare);
 
-  uint64_t *bars = reinterpret_cast<uint64_t *>(smem + S::kBar) + warp * kStages;
-  if (lane == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(&bars[s], 1);
-    fence_mbarrier_init();
-  }
   char *ring = smem + warp * kStages * S::kStage;
-  int2 *stage_pages = reinterpret_cast<int2 *>(smem + S::kPages) + warp * kStages;
-
   // this CTA's stretch of the units (the first `extra` CTAs have one more), and the sequence that it begins in
   int mine = 0, total = 0;
   for (int s = tid; s < k.b.n_seqs; s += kAttnThreads) mine += Kv4Units<WEIGHTS>(k, kv4_seq(k.b, s, k.status)).all();
@@ -453,10 +450,6 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
     }
   }
 
-  int stage_in = 0, stage_out = 0;  // of the next tile to fetch, to use
-  uint32_t phase = 0;
-  bool lost = false;
-
   for (int unit = first_unit; unit < end_unit && seq < k.b.n_seqs;) {
     const Kv4Seq q = kv4_seq(k.b, seq, nullptr);
     const Kv4Units<WEIGHTS> units(k, q);
@@ -484,43 +477,39 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       const int begin = from * kUnitTokens, end = min(upto * kUnitTokens, seen);
       const int tiles = max((end - begin + kTileTokens - 1) / kTileTokens, 0);
       const int count = (tiles - warp + kAttnWarps - 1) / kAttnWarps;  // this warp's; <= 0: none
-      // a lane knows where one of the next 32 of this warp's tiles stands, and starts its copy
-      constexpr int N = WEIGHTS ? S::kBlock / 2 : S::kBlock;  // of a block: its keys alone, or all
-      const uint8_t *src0 = nullptr, *src1 = nullptr;
-      int blocks = 0, fetched = 0;
-      int2 pages = make_int2(0, 0);
+      // a lane knows the pages of one of the next 32 of this warp's tiles
+      int fetched = 0, stage_in = 0, page0 = 0, page1 = 0;
       auto fetch = [&]() {
-        if (!(fetched & 31)) {
-          const int at = begin + (warp + (fetched + lane) * kAttnWarps) * kTileTokens;
-          blocks = min(kTileBlocks, (end - at + kKv4Block - 1) / kKv4Block);
-          if (at < end) {
-            const int slot = at & ((1 << k.c.page_shift) - 1);
-            pages.x = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, at, k.status), 0);
-            src0 = kv4_block(k.c, pages.x, head, slot);
-            pages.y = pages.x;
-            src1 = src0 + S::kBlock;
-            if (k.c.page_shift == 4 && blocks > 1) {
-              pages.y = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, at + kKv4Block, k.status), 0);
-              src1 = kv4_block(k.c, pages.y, head, 0);
-            }
+        if (fetched < count) {
+          if (!(fetched & 31)) {
+            const int at = begin + (warp + (fetched + lane) * kAttnWarps) * kTileTokens;
+            if (at < end) page0 = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, at, k.status), 0);
+            if (k.c.page_shift == 4 && at + kKv4Block < end)
+              page1 = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, at + kKv4Block, k.status), 0);
           }
-        }
-        if (lane == (fetched & 31)) {
+          const int at = begin + (warp + fetched * kAttnWarps) * kTileTokens, slot = at & ((1 << k.c.page_shift) - 1);
+          constexpr int N = WEIGHTS ? S::kBlock / 2 : S::kBlock;  // of a block: its keys alone, or all
+          const uint8_t *src = kv4_block(k.c, __shfl_sync(0xffffffffu, page0, fetched & 31), head, slot);
           char *to = ring + stage_in * S::kStage;
-          uint64_t *bar = &bars[stage_in];
-          if (WEIGHTS) stage_pages[stage_in] = pages;
-          mbar_arrive_expect_tx(bar, (uint32_t)(blocks * N));
-          if (!WEIGHTS && k.c.page_shift > 4) {  // the tile lies within a page
-            bulk_g2s(to, src0, (uint32_t)(blocks * N), bar);
-          } else {
-            bulk_g2s(to, src0, N, bar);
-            if (blocks > 1) bulk_g2s(to + S::kBlock, src1, N, bar);
+#pragma unroll
+          for (int b = 0; b < kTileBlocks; ++b) {
+            if (b > 0) {  // the tile lies within a page, or its second block is the first of another
+              src += S::kBlock;
+              if (k.c.page_shift == 4)
+                src = kv4_block(k.c, __shfl_sync(0xffffffffu, page1, fetched & 31), head, 0);
+              if (at + b * kKv4Block >= end) break;
+            }
+#pragma unroll
+            for (int c = 0; c < N; c += 512)
+              if (c + 512 <= N || c + lane * 16 < N)
+                copy16_async(to + b * S::kBlock + c + lane * 16, src + c + lane * 16);
           }
+          stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+          ++fetched;
         }
-        stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
-        ++fetched;
+        asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      for (int i = 0; i < min(count, kStages); ++i) fetch();
+      for (int i = 0; i < kStages; ++i) fetch();
 
       if (WEIGHTS) __syncthreads();  // the previous rows' fragments have been read
       load_queries<T, D, NG, NT, QS>(k, q, head, row0, rows, smem);
@@ -536,11 +525,12 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       }
       __syncthreads();
 
-      // In powers of two: top, the maximum of rows 2t, 2t + 1 at its last rise, limit, where it has to rise again, and
+      // In powers of two: top, the maximum of rows 2t, 2t + 1 at its last rise (limit: the score, without the row's
+      // factor, at which it has to rise again), and
       // base, what the exponentials refer to: top - lift, where 2^lift brings the largest value scale into
       // [2^10, 2^11), so that products with probabilities up to 2^4 stay below f16's largest.  (lse in the weights'
       // pass.)  Outputs and sums are both in units of 2^base.
-      float factor[NT][2], base[NT][2], top[NT][2], sum[NT][2];
+      float factor[NT][2], base[NT][2], top[NT][2], limit[NT][2], sum[NT][2];
       int sees[NT][2];  // tokens that these rows see
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -549,7 +539,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
           const int n = nt * 8 + 2 * t + e, r = row0 + n;
           factor[nt][e] = reinterpret_cast<const float *>(smem + S::kFactor)[n];
           base[nt][e] = WEIGHTS ? reinterpret_cast<const float *>(smem + S::kLse)[n] : 0.0f;
-          top[nt][e] = -INFINITY;
+          top[nt][e] = limit[nt][e] = -INFINITY;
           sum[nt][e] = 0.0f;
           sees[nt][e] = min(r < rows ? min(past + r / k.group_heads, q.len) : q.len, end);
         }
@@ -565,14 +555,11 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       float lift = 0.0f;
       __half2 scale_limit = __floats2half2_rn(0.0f, 0.0f);  // value scales up to this one fit
 
-      for (int i = 0; i < count; ++i) {
+      for (int i = 0, stage_out = 0; i < count; ++i, stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1) {
         const int at = begin + (warp + i * kAttnWarps) * kTileTokens;
-        const char *buf = ring + stage_out * S::kStage;
-        if (!mbar_wait(&bars[stage_out], phase)) {
-          set_status(k.status, kStatusTimeout);
-          lost = true;
-          break;
-        }
+        char *buf = ring + stage_out * S::kStage;
+        asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+        __syncwarp();  // every lane's copies are there
         float p[kTileBlocks][NT][4];
         tile_scores<D, NG, NT, QS>(buf, smem, p);
         const bool whole = at + kTileTokens <= all_see;
@@ -587,7 +574,6 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
         }
 
         if constexpr (WEIGHTS) {
-          const int2 pages_of = stage_pages[stage_out];
 #pragma unroll
           for (int b = 0; b < kTileBlocks; ++b) {
             float w[2] = {0.0f, 0.0f};
@@ -601,87 +587,76 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
               w[e] += __shfl_xor_sync(0xffffffffu, w[e], 1);
               w[e] += __shfl_xor_sync(0xffffffffu, w[e], 2);
               const int tok = at + b * kKv4Block + kv4_token(g) + 8 * e;
-              if (t == 0 && tok < end)
-                k.c.weights[(((int64_t)(b ? pages_of.y : pages_of.x) * k.c.kv_heads + head) << k.c.page_shift) +
-                            (tok & ((1 << k.c.page_shift) - 1))] += w[e];
+              if (t == 0 && tok < end) {
+                const int page = kv4_page(k.c, k.b.table, k.b.table_stride, seq, tok, nullptr);
+                if (page >= 0)
+                  k.c.weights[(((int64_t)page * k.c.kv_heads + head) << k.c.page_shift) +
+                              (tok & ((1 << k.c.page_shift) - 1))] += w[e];
+              }
             }
           }
         } else {
-          // does a score exceed its row's limit?
+          // does a score exceed its row's limit, or a value scale what fits?
           bool rise = false;
+          float m[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              float m = fmaxf(p[0][nt][e], p[0][nt][e + 2]);
+              m[nt][e] = fmaxf(p[0][nt][e], p[0][nt][e + 2]);
 #pragma unroll
-              for (int b = 1; b < kTileBlocks; ++b) m = fmaxf(m, fmaxf(p[b][nt][e], p[b][nt][e + 2]));
-              rise |= m * factor[nt][e] > top[nt][e] + 4.0f;
+              for (int b = 1; b < kTileBlocks; ++b) m[nt][e] = fmaxf(m[nt][e], fmaxf(p[b][nt][e], p[b][nt][e + 2]));
+              rise |= m[nt][e] > limit[nt][e];
             }
-          if (__any_sync(0xffffffffu, rise)) {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                float m = fmaxf(p[0][nt][e], p[0][nt][e + 2]);
-#pragma unroll
-                for (int b = 1; b < kTileBlocks; ++b) m = fmaxf(m, fmaxf(p[b][nt][e], p[b][nt][e + 2]));
-                m *= factor[nt][e];
-#pragma unroll
-                for (int x = 4; x < 32; x *= 2) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-                m = fmaxf(m, top[nt][e]);
-                const float f = m == -INFINITY ? 1.0f : fast_exp2(top[nt][e] - m);
-                top[nt][e] = m;
-                base[nt][e] = m == -INFINITY ? 0.0f : m - lift;
-                sum[nt][e] *= f;
-#pragma unroll
-                for (int d = 0; d < D / 16; ++d) {
-                  o[nt][d][e] *= f;
-                  o[nt][d][e + 2] *= f;
-                }
-              }
+          if (!whole) {  // what stands behind the last token is not a scale
+            if (lane < kTileTokens && at + lane >= end)
+              for (int gr = 0; gr < NG; ++gr)
+                reinterpret_cast<__half *>(buf + (lane >> 4) * S::kBlock + S::kBlock / 2 + 8 * D)[(lane & 15) * NG + gr] =
+                    __ushort_as_half(0);
+            __syncwarp();
           }
-          // value scales of this lane's tokens; what stands behind the last token is not a scale
-          float sv[kTileBlocks][2][NG];
-          __half2 big = __floats2half2_rn(0.0f, 0.0f);
+          __half2 h[kTileBlocks][2][(NG + 1) / 2], big = __floats2half2_rn(0.0f, 0.0f);
 #pragma unroll
           for (int b = 0; b < kTileBlocks; ++b)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int tok = kv4_token(g) + 8 * e;
-              const char *at_scales = buf + b * S::kBlock + S::kBlock / 2 + 8 * D + tok * 2 * NG;
-              const bool there = whole || at + b * kKv4Block + tok < end;
-              __half2 h[NG > 1 ? NG / 2 : 1];
+              const char *from = buf + b * S::kBlock + S::kBlock / 2 + 8 * D + (kv4_token(g) + 8 * e) * 2 * NG;
               if constexpr (NG == 1) {
-                h[0] = __half2half2(*reinterpret_cast<const __half *>(at_scales));
+                h[b][e][0] = __half2half2(*reinterpret_cast<const __half *>(from));
               } else {
                 uint32_t w[NG / 2];
-                lds<NG * 2>(at_scales, w);
+                lds<NG * 2>(from, w);
 #pragma unroll
-                for (int x = 0; x < NG / 2; ++x) h[x] = *reinterpret_cast<const __half2 *>(&w[x]);
+                for (int x = 0; x < NG / 2; ++x) h[b][e][x] = *reinterpret_cast<const __half2 *>(&w[x]);
               }
 #pragma unroll
-              for (int x = 0; x < (NG + 1) / 2; ++x) {
-                if (!there) h[x] = __floats2half2_rn(0.0f, 0.0f);
-                big = __hmax2(big, h[x]);
-                const float2 f = __half22float2(h[x]);
-                sv[b][e][2 * x] = f.x;
-                if constexpr (NG > 1) sv[b][e][2 * x + 1] = f.y;
-              }
+              for (int x = 0; x < (NG + 1) / 2; ++x) big = __hmax2(big, h[b][e][x]);
             }
-          if (__any_sync(0xffffffffu, !__hble2(big, scale_limit))) {
+          if (__any_sync(0xffffffffu, rise || !__hble2(big, scale_limit))) {
             float all = fmaxf(__low2float(big), __high2float(big));
 #pragma unroll
             for (int x = 4; x < 32; x *= 2) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
-            const int power = ilogbf(all);
-            const float to = (float)(10 - power), f = ldexpf(1.0f, (int)(to - lift));
-            const float most = ldexpf(2.0f, power) * (1.0f - 0x1p-11f);
-            scale_limit = __floats2half2_rn(most, most);
+            float up = 0.0f;  // of lift
+            if (all > __low2float(scale_limit)) {
+              const int power = ilogbf(all);
+              const float most = ldexpf(2.0f, power) * (1.0f - 0x1p-11f);
+              scale_limit = __floats2half2_rn(most, most);
+              up = (float)(10 - power) - lift;
+              lift += up;
+            }
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                base[nt][e] -= to - lift;
+                float x = m[nt][e] * factor[nt][e];
+#pragma unroll
+                for (int y = 4; y < 32; y *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, y));
+                x = fmaxf(x, top[nt][e]);
+                // sums and outputs so far are in units of 2^(top - lift)
+                const float f = x == -INFINITY ? 1.0f : fast_exp2(top[nt][e] - x + up);
+                top[nt][e] = x;
+                base[nt][e] = x == -INFINITY ? 0.0f : x - lift;
+                limit[nt][e] = x == -INFINITY ? x : (x + 4.0f) / factor[nt][e];
                 sum[nt][e] *= f;
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
@@ -689,7 +664,6 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
                   o[nt][d][e + 2] *= f;
                 }
               }
-            lift = to;
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -719,7 +693,9 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
               for (int b = 0; b < kTileBlocks; ++b)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                  const float f = sv[b][e][m / M];
+                  constexpr int kTwo = NG > 1 ? 2 : 1;
+                  const __half2 pair = h[b][e][m / M / kTwo];
+                  const float f = m / M % kTwo ? __high2float(pair) : __low2float(pair);
 #pragma unroll
                   for (int nt = 0; nt < NT; ++nt) {
                     const float x0 = p[b][nt][2 * e] * f, x1 = p[b][nt][2 * e + 1] * f;
@@ -762,12 +738,9 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
               for (int e = 0; e < 4; ++e) o[nt][m][e] = kWide ? o[nt][m][e] + acc[nt][e] : acc[nt][e];
           }
         }
-        stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1;
-        phase ^= stage_out == 0;
         __syncwarp();  // every lane has read the stage
-        if (fetched < count) fetch();
+        fetch();
       }
-      if (lost) return;  // reported; the results are lost, the workspace with them
       if constexpr (!WEIGHTS) {
         // join the warps: the ring is drained, each writes its part over it
 #pragma unroll
@@ -890,9 +863,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
             }
           }
         }
-        // the next copies come after these accesses of the ring
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
+        __syncthreads();  // the next copies come after these accesses of the ring
       }
     }
   }
