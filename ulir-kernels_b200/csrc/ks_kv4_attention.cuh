@@ -477,34 +477,47 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       const int begin = from * kUnitTokens, end = min(upto * kUnitTokens, seen);
       const int tiles = max((end - begin + kTileTokens - 1) / kTileTokens, 0);
       const int count = (tiles - warp + kAttnWarps - 1) / kAttnWarps;  // this warp's; <= 0: none
-      // a lane knows the pages of one of the next 32 of this warp's tiles
-      int fetched = 0, stage_in = 0, page0 = 0, page1 = 0;
+      // A lane knows where one of the next 32 of this warp's tiles stands; where that tile is whole and within a page,
+      // the same copies fetch it each time.
+      constexpr int N = WEIGHTS ? S::kBlock / 2 : S::kBlock;  // of a block: its keys alone, or all
+      int fetched = 0, page0 = 0, page1 = 0;
+      char *to = ring + lane * 16;
+      const uint8_t *mine_at = nullptr;
       auto fetch = [&]() {
         if (fetched < count) {
+          const int at = begin + (warp + fetched * kAttnWarps) * kTileTokens;
           if (!(fetched & 31)) {
-            const int at = begin + (warp + (fetched + lane) * kAttnWarps) * kTileTokens;
-            if (at < end) page0 = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, at, k.status), 0);
-            if (k.c.page_shift == 4 && at + kKv4Block < end)
-              page1 = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, at + kKv4Block, k.status), 0);
-          }
-          const int at = begin + (warp + fetched * kAttnWarps) * kTileTokens, slot = at & ((1 << k.c.page_shift) - 1);
-          constexpr int N = WEIGHTS ? S::kBlock / 2 : S::kBlock;  // of a block: its keys alone, or all
-          const uint8_t *src = kv4_block(k.c, __shfl_sync(0xffffffffu, page0, fetched & 31), head, slot);
-          char *to = ring + stage_in * S::kStage;
-#pragma unroll
-          for (int b = 0; b < kTileBlocks; ++b) {
-            if (b > 0) {  // the tile lies within a page, or its second block is the first of another
-              src += S::kBlock;
-              if (k.c.page_shift == 4)
-                src = kv4_block(k.c, __shfl_sync(0xffffffffu, page1, fetched & 31), head, 0);
-              if (at + b * kKv4Block >= end) break;
+            const int lane_at = at + lane * kAttnWarps * kTileTokens;
+            if (lane_at < end) {
+              page0 = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, lane_at, k.status), 0);
+              mine_at = kv4_block(k.c, page0, head, lane_at & ((1 << k.c.page_shift) - 1));
             }
-#pragma unroll
-            for (int c = 0; c < N; c += 512)
-              if (c + 512 <= N || c + lane * 16 < N)
-                copy16_async(to + b * S::kBlock + c + lane * 16, src + c + lane * 16);
+            if (k.c.page_shift == 4 && lane_at + kKv4Block < end)
+              page1 = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, lane_at + kKv4Block, k.status), 0);
           }
-          stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+          const uint8_t *src = reinterpret_cast<const uint8_t *>(
+                                   __shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(mine_at), fetched & 31)) +
+                               lane * 16;
+          if (k.c.page_shift > 4 && at + kTileTokens <= end) {
+            constexpr int kPieces = WEIGHTS ? kTileBlocks : 1, kBytes = WEIGHTS ? N : S::kStage;
+#pragma unroll
+            for (int b = 0; b < kPieces; ++b)
+#pragma unroll
+              for (int c = 0; c < kBytes; c += 512)
+                if (c + 512 <= kBytes || c + lane * 16 < kBytes)
+                  copy16_async(to + b * S::kBlock + c, src + b * S::kBlock + c);
+          } else {
+#pragma unroll 1
+            for (int b = 0; b < kTileBlocks && at + b * kKv4Block < end; ++b) {
+              if (b > 0)
+                src = k.c.page_shift > 4
+                          ? src + S::kBlock
+                          : kv4_block(k.c, __shfl_sync(0xffffffffu, page1, fetched & 31), head, 0) + lane * 16;
+#pragma unroll 1
+              for (int c = 0; c + lane * 16 < N; c += 512) copy16_async(to + b * S::kBlock + c, src + c);
+            }
+          }
+          to = to + S::kStage == ring + lane * 16 + kStages * S::kStage ? ring + lane * 16 : to + S::kStage;
           ++fetched;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
