@@ -148,47 +148,55 @@ struct Kv4Smem {
   static constexpr int kBytes = kShare + 32;
 };
 
-// Reads the tile's query rows into B fragments.  A thread has the 8 elements
-// 32w + 8t .. of one row, the ones that lane (row, t) multiplies with the words
-// of a token's keys: halves (0, 4) and (2, 6), with the factor 16, and (1, 5)
-// and (3, 7).  A row is scaled by the power of two that brings its largest
-// element into [2^10, 2^11), and has the sign of the scale.
-template <typename T, int D, int NG, int NT, int QS>
+// The tile's query rows as B fragments.  A thread has the 8 elements 32w + 8t ..
+// of one row (of each 128 / (D / 8) rows), the ones that lane (row, t)
+// multiplies with the words of a token's keys: halves (0, 4) and (2, 6), with
+// the factor 16, and (1, 5) and (3, 7).  A row is scaled by the power of two
+// that brings its largest element into [2^10, 2^11), and has the sign of the
+// scale.
+template <int D, int NT>
+constexpr int kQuerySets = (NT * D + kAttnThreads - 1) / kAttnThreads;  // rows of a thread
+
+template <typename T, int D, int NT>
 __device__ __forceinline__ void load_queries(const Kv4AttnArgs &k, const Kv4Seq &q, int head, int row0, int rows,
-                                             char *smem) {
+                                             T (&x)[kQuerySets<D, NT>][8]) {
+  constexpr int PER = D / 8;  // threads of a row
+#pragma unroll
+  for (int set = 0; set < kQuerySets<D, NT>; ++set) {
+    const int i = set * kAttnThreads + threadIdx.x, n = i / PER, r = row0 + n;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[set][e] = T(0.0f);
+    if (n < 8 * NT && r < rows) {
+      const int j = r / k.group_heads, h = head * k.group_heads + r % k.group_heads;
+      const T *src = static_cast<const T *>(k.a.q) + (int64_t)(q.first + j) * k.a.q_token + h * k.a.q_head + i % PER * 8;
+      if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
+#pragma unroll
+        for (int e = 0; e < (int)sizeof(T) / 2; ++e)
+          reinterpret_cast<uint4 *>(x[set])[e] = reinterpret_cast<const uint4 *>(src)[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[set][e] = src[e];
+      }
+    }
+  }
+}
+
+template <typename T, int D, int NG, int NT, int QS>
+__device__ __forceinline__ void place_queries(const Kv4AttnArgs &k, int row0, int rows,
+                                              const T (&x)[kQuerySets<D, NT>][8], char *smem) {
   using S = Kv4Smem<D, NG, NT, QS>;
   constexpr int PER = D / 8;      // threads of a row
   constexpr int W = D / 32 / NG;  // words of a group
-  const int tid = threadIdx.x;
   const float sign = k.a.scale < 0.0f ? -1.0f : k.a.scale == 0.0f ? 0.0f : 1.0f;
 #pragma unroll
-  for (int base = 0; base < 8 * NT * PER; base += kAttnThreads) {
-    const int i = base + tid, n = i / PER, w = (i % PER) >> 2, t = i & 3;  // (8 NT PER is a multiple of 64)
-    if (8 * NT * PER % kAttnThreads && i >= 8 * NT * PER) break;           // whole warps
+  for (int set = 0; set < kQuerySets<D, NT>; ++set) {
+    const int i = set * kAttnThreads + threadIdx.x, n = i / PER, w = (i % PER) >> 2, t = i & 3, r = row0 + n;
+    if (8 * NT * PER % kAttnThreads && n >= 8 * NT) break;  // whole warps
     float v[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-    const int r = row0 + n;
-    if (r < rows) {
-      const int j = r / k.group_heads, h = head * k.group_heads + r % k.group_heads;
-      const T *src = static_cast<const T *>(k.a.q) + (int64_t)(q.first + j) * k.a.q_token + h * k.a.q_head + 32 * w +
-                     8 * t;
-      if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
-        T x[8];
-#pragma unroll
-        for (int e = 0; e < (int)sizeof(T) / 2; ++e)
-          reinterpret_cast<uint4 *>(x)[e] = reinterpret_cast<const uint4 *>(src)[e];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = kv4_load(&x[e]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = kv4_load(src + e);
-      }
-    }
     float top = 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      v[e] *= sign;
+      v[e] = kv4_load(&x[set][e]) * sign;
       top = fmaxf(top, fabsf(v[e]));
     }
 #pragma unroll
@@ -409,44 +417,99 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
   int *share = reinterpret_cast<int *>(smem + S::kShare);
 
   char *ring = smem + warp * kStages * S::kStage;
-  // this CTA's stretch of the units (the first `extra` CTAs have one more), and the sequence that it begins in
-  int mine = 0, total = 0;
-  for (int s = tid; s < k.b.n_seqs; s += kAttnThreads) mine += Kv4Units<WEIGHTS>(k, kv4_seq(k.b, s, k.status)).all();
-  int before = cta_scan(mine, &total, share);
-  const int ctas = min((int)gridDim.x, total), cta = blockIdx.x;
-  if (cta >= ctas) return;
-  const int each = total / ctas, extra = total - each * ctas;
-  const int first_unit = each * cta + min(cta, extra), end_unit = first_unit + each + (cta < extra);
-  __syncthreads();
-  int seq = k.b.n_seqs, seq_unit = 0;  // the sequence, its first unit
-  if (k.b.n_seqs <= kAttnThreads) {
-    if (first_unit >= before && first_unit < before + mine) {
-      share[0] = tid;
-      share[1] = before;
+  // This CTA's stretch of the units (the first `extra` CTAs have one more), and the sequence that it begins in; or,
+  // where that takes no more than three units longer, one of the `parts` of one item: a stretch over two items costs
+  // some three units' time between them.
+  int ctas, first_unit, end_unit, each = 0, extra = 0, seq = k.b.n_seqs, seq_unit = 0, parts = 0, part = 0;
+  const int cta = blockIdx.x;
+  if (k.b.n_seqs <= 32) {  // every warp by itself, a sequence to a lane
+    int per = 1, items = 0;
+    if (lane < k.b.n_seqs) {
+      const Kv4Units<WEIGHTS> u(k, kv4_seq(k.b, lane, k.status));
+      per = u.per, items = u.items;
     }
-    __syncthreads();
-    seq = share[0];
-    seq_unit = share[1];
-  } else {
-    int passed = 0;
-    for (int base = 0; base < k.b.n_seqs; base += kAttnThreads) {
-      const int s = base + tid;
-      const int u = s < k.b.n_seqs ? Kv4Units<WEIGHTS>(k, kv4_seq(k.b, s, nullptr)).all() : 0;
-      int some;
-      const int at = passed + cta_scan(u, &some, share);
-      if (first_unit >= passed + some) {
-        passed += some;
-        continue;
+    auto scan = [&](int v) {
+#pragma unroll
+      for (int o = 1; o < 32; o *= 2) {
+        const int n = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += n;
       }
-      __syncthreads();
-      if (first_unit >= at && first_unit < at + u) {
-        share[0] = s;
-        share[1] = at;
+      return v;
+    };
+    const int upto_units = scan(per * items), total = __shfl_sync(0xffffffffu, upto_units, 31);
+    if (total == 0) return;
+    ctas = min((int)gridDim.x, total);
+    each = total / ctas, extra = total - each * ctas;
+    // the shortest part that gives no more parts than CTAs: a candidate to a lane
+    const int longest = each + (extra > 0) + lane;
+    int count = 0;
+    for (int s = 0; s < k.b.n_seqs; ++s) {
+      const int p = __shfl_sync(0xffffffffu, per, s);
+      count += __shfl_sync(0xffffffffu, items, s) * ((p + longest - 1) / longest);
+    }
+    const unsigned fits = __ballot_sync(0xffffffffu, lane <= 3 && count <= (int)gridDim.x);
+    if (fits) {
+      const int most = each + (extra > 0) + __ffs(fits) - 1, pieces = (per + most - 1) / most;
+      const int upto = scan(items * pieces), before = upto - items * pieces;
+      const unsigned here = __ballot_sync(0xffffffffu, cta >= before && cta < upto);
+      if (!here) return;
+      seq = __ffs(here) - 1;
+      parts = __shfl_sync(0xffffffffu, pieces, seq);
+      const int of = __shfl_sync(0xffffffffu, per, seq), at = cta - __shfl_sync(0xffffffffu, before, seq);
+      const int item = at / parts;
+      part = at - item * parts;
+      seq_unit = __shfl_sync(0xffffffffu, upto_units - per * items, seq);
+      // even parts, the longer ones first
+      const int short_part = of / parts, longer = of - short_part * parts;
+      first_unit = seq_unit + item * of + short_part * part + min(part, longer);
+      end_unit = first_unit + short_part + (part < longer);
+    } else {
+      if (cta >= ctas) return;
+      first_unit = each * cta + min(cta, extra);
+      end_unit = first_unit + each + (cta < extra);
+      const unsigned here = __ballot_sync(0xffffffffu, first_unit < upto_units);
+      seq = __ffs(here) - 1;
+      seq_unit = __shfl_sync(0xffffffffu, upto_units - per * items, seq);
+    }
+  } else {
+    int mine = 0, total = 0;
+    for (int s = tid; s < k.b.n_seqs; s += kAttnThreads) mine += Kv4Units<WEIGHTS>(k, kv4_seq(k.b, s, k.status)).all();
+    const int before = cta_scan(mine, &total, share);
+    ctas = min((int)gridDim.x, total);
+    if (cta >= ctas) return;
+    each = total / ctas, extra = total - each * ctas;
+    first_unit = each * cta + min(cta, extra);
+    end_unit = first_unit + each + (cta < extra);
+    __syncthreads();
+    if (k.b.n_seqs <= kAttnThreads) {
+      if (first_unit >= before && first_unit < before + mine) {
+        share[0] = tid;
+        share[1] = before;
       }
       __syncthreads();
       seq = share[0];
       seq_unit = share[1];
-      break;
+    } else {
+      int passed = 0;
+      for (int base = 0; base < k.b.n_seqs; base += kAttnThreads) {
+        const int s = base + tid;
+        const int u = s < k.b.n_seqs ? Kv4Units<WEIGHTS>(k, kv4_seq(k.b, s, nullptr)).all() : 0;
+        int some;
+        const int at = passed + cta_scan(u, &some, share);
+        if (first_unit >= passed + some) {
+          passed += some;
+          continue;
+        }
+        __syncthreads();
+        if (first_unit >= at && first_unit < at + u) {
+          share[0] = s;
+          share[1] = at;
+        }
+        __syncthreads();
+        seq = share[0];
+        seq_unit = share[1];
+        break;
+      }
     }
   }
 
@@ -522,10 +585,12 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
+      T queries[kQuerySets<D, NT>][8];
+      load_queries<T, D, NT>(k, q, head, row0, rows, queries);  // on their way while the pages are looked up
       for (int i = 0; i < kStages; ++i) fetch();
 
       if (WEIGHTS) __syncthreads();  // the previous rows' fragments have been read
-      load_queries<T, D, NG, NT, QS>(k, q, head, row0, rows, smem);
+      place_queries<T, D, NG, NT, QS>(k, row0, rows, queries, smem);
       if (WEIGHTS && tid < R) {
         const int r = row0 + tid;
         float v = INFINITY;  // no weight for rows that are not there or see nothing
@@ -763,8 +828,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
 #pragma unroll
             for (int x = 4; x < 32; x *= 2) sum[nt][e] += __shfl_xor_sync(0xffffffffu, sum[nt][e], x);
         __syncthreads();
-        float *part = reinterpret_cast<float *>(smem);  // [warp][row][D], then [warp][2][row]
-        float *stat = part + kAttnWarps * R * D;
+        float *outs = reinterpret_cast<float *>(smem);  // [warp][row][D], then [warp][2][row]
+        float *stat = outs + kAttnWarps * R * D;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -772,7 +837,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
             const int n = nt * 8 + 2 * t + e;
 #pragma unroll
             for (int m = 0; m < D / 16; ++m)
-              *reinterpret_cast<float2 *>(part + (warp * R + n) * D + 16 * m + 2 * g) =
+              *reinterpret_cast<float2 *>(outs + (warp * R + n) * D + 16 * m + 2 * g) =
                   make_float2(o[nt][m][e], o[nt][m][e + 2]);
             if (g == 0) {
               stat[warp * 2 * R + n] = top[nt][e] == -INFINITY ? -INFINITY : base[nt][e];
@@ -807,7 +872,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
           for (int w = 0; w < kAttnWarps; ++w) {
             const float f = fast_exp2(stat[w * 2 * R + n] - to);
             l = fmaf(stat[w * 2 * R + R + n], f, l);
-            const float4 y = *reinterpret_cast<const float4 *>(part + (w * R + n) * D + d);
+            const float4 y = *reinterpret_cast<const float4 *>(outs + (w * R + n) * D + d);
             x.x = fmaf(y.x, f, x.x);
             x.y = fmaf(y.y, f, x.y);
             x.z = fmaf(y.z, f, x.z);
@@ -829,7 +894,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
             const int more = extra * (each + 1);
             return u < more ? u / (each + 1) : extra + (u - more) / each;
           };
-          const int c0 = cta_of(item_unit), c1 = cta_of(item_unit + units.per - 1);
+          const int c0 = parts ? cta - part : cta_of(item_unit);
+          const int count_parts = parts ? parts : cta_of(item_unit + units.per - 1) - c0 + 1;
           uint32_t *counters = static_cast<uint32_t *>(k.a.workspace);
           // whether this CTA is the last of `of` to arrive; all that the others wrote is then visible
           auto last_of = [&](uint32_t *counter, int of) {
@@ -849,8 +915,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
           constexpr int I = R * D / 4 / kAttnThreads;
           float4 x[I];
           float m[I], l[I];
-          const int parts = c1 - c0 + 1, group = (cta - c0) / kJoin, head_cta = c0 + group * kJoin;
-          const int in_group = min(kJoin, parts - group * kJoin), groups = (parts + kJoin - 1) / kJoin;
+          const int group = (cta - c0) / kJoin, head_cta = c0 + group * kJoin;
+          const int in_group = min(kJoin, count_parts - group * kJoin), groups = (count_parts + kJoin - 1) / kJoin;
           bool last = last_of(counters + (group ? 2 : 1) * kAttnCtas + head_cta, in_group);
           if (last) join_parts<D, R, I>(k, c0, head_cta, in_group, 1, x, m, l);
           if (last && groups > 1) {
