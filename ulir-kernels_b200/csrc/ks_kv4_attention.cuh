@@ -58,7 +58,7 @@ namespace ksb {
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
 constexpr int kTileBlocks = 2, kTileTokens = kTileBlocks * kKv4Block;
 constexpr int kUnitTokens = kAttnWarps * kTileTokens;
-constexpr int kJoin = 16;  // parts that are joined at once
+constexpr int kJoin = 8;  // parts that are joined at once
 // Words at the start of the workspace, 0 between calls: three per CTA, of the
 // item that begins in its stretch (finished groups of parts), of that item's
 // first group of parts and of a later group, which begins at this CTA.
@@ -316,7 +316,11 @@ __device__ __forceinline__ void tile_scores(const char *buf, const char *smem, f
   }
 }
 
-// Units of a sequence's work: those of one item, and how many items.
+// Units of a sequence's work: those of one item, and how many items.  In a
+// stretch over several items each begins with kItemUnits more, about the time
+// that it takes to finish one item and begin another.
+constexpr int kItemUnits = 3;
+
 template <bool WEIGHTS>
 struct Kv4Units {
   int per, items;
@@ -327,7 +331,7 @@ struct Kv4Units {
     per = (q.len + kUnitTokens - 1) / kUnitTokens;
     if (!WEIGHTS) per = max(per, 1);
   }
-  __device__ int all() const { return per * items; }
+  __device__ int all() const { return (kItemUnits + per) * items; }
 };
 
 // Sum over the CTA, and over its threads before this one.
@@ -358,7 +362,7 @@ __device__ __forceinline__ int cta_scan(int v, int *total, int *shared) {
 template <int D, int R, int I>
 __device__ __forceinline__ void join_parts(const Kv4AttnArgs &k, int c0, int first, int count, int step,
                                            float4 (&x)[I], float (&m)[I], float (&l)[I]) {
-  constexpr int B = 8 / I > 2 ? 8 / I : 2;  // parts in flight
+  constexpr int B = I <= 2 ? 8 : 4;  // parts in flight
 #pragma unroll
   for (int i = 0; i < I; ++i) {
     x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -436,20 +440,27 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       }
       return v;
     };
-    const int upto_units = scan(per * items), total = __shfl_sync(0xffffffffu, upto_units, 31);
+    const int upto_units = scan((kItemUnits + per) * items), total = __shfl_sync(0xffffffffu, upto_units, 31);
     if (total == 0) return;
+    int units = per * items;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) units += __shfl_xor_sync(0xffffffffu, units, o);
     ctas = min((int)gridDim.x, total);
     each = total / ctas, extra = total - each * ctas;
-    // the shortest part that gives no more parts than CTAs: a candidate to a lane
-    const int longest = each + (extra > 0) + lane;
+    // the shortest part that gives no more parts than CTAs: lane l counts those of candidate l % 4 in every eighth
+    // sequence
+    const int shortest = (units + (int)gridDim.x - 1) / (int)gridDim.x;
     int count = 0;
-    for (int s = 0; s < k.b.n_seqs; ++s) {
-      const int p = __shfl_sync(0xffffffffu, per, s);
-      count += __shfl_sync(0xffffffffu, items, s) * ((p + longest - 1) / longest);
+#pragma unroll
+    for (int s = 0; s < 32; s += 8) {
+      const int p = __shfl_sync(0xffffffffu, per, s + (lane >> 2)), n = __shfl_sync(0xffffffffu, items, s + (lane >> 2));
+      if (s < k.b.n_seqs) count += n * ((p + shortest + (lane & 3) - 1) / (shortest + (lane & 3)));
     }
-    const unsigned fits = __ballot_sync(0xffffffffu, lane <= 3 && count <= (int)gridDim.x);
+#pragma unroll
+    for (int o = 4; o < 32; o *= 2) count += __shfl_xor_sync(0xffffffffu, count, o);
+    const unsigned fits = __ballot_sync(0xffffffffu, lane < 4 && count <= (int)gridDim.x);
     if (fits) {
-      const int most = each + (extra > 0) + __ffs(fits) - 1, pieces = (per + most - 1) / most;
+      const int most = shortest + __ffs(fits) - 1, pieces = (per + most - 1) / most;
       const int upto = scan(items * pieces), before = upto - items * pieces;
       const unsigned here = __ballot_sync(0xffffffffu, cta >= before && cta < upto);
       if (!here) return;
@@ -458,10 +469,10 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       const int of = __shfl_sync(0xffffffffu, per, seq), at = cta - __shfl_sync(0xffffffffu, before, seq);
       const int item = at / parts;
       part = at - item * parts;
-      seq_unit = __shfl_sync(0xffffffffu, upto_units - per * items, seq);
+      seq_unit = __shfl_sync(0xffffffffu, upto_units - (kItemUnits + per) * items, seq);
       // even parts, the longer ones first
       const int short_part = of / parts, longer = of - short_part * parts;
-      first_unit = seq_unit + item * of + short_part * part + min(part, longer);
+      first_unit = seq_unit + item * (kItemUnits + of) + kItemUnits + short_part * part + min(part, longer);
       end_unit = first_unit + short_part + (part < longer);
     } else {
       if (cta >= ctas) return;
@@ -469,7 +480,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       end_unit = first_unit + each + (cta < extra);
       const unsigned here = __ballot_sync(0xffffffffu, first_unit < upto_units);
       seq = __ffs(here) - 1;
-      seq_unit = __shfl_sync(0xffffffffu, upto_units - per * items, seq);
+      seq_unit = __shfl_sync(0xffffffffu, upto_units - (kItemUnits + per) * items, seq);
     }
   } else {
     int mine = 0, total = 0;
@@ -525,10 +536,10 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
     const int rows = min(q.n_new, k.a.max_new) * k.group_heads;
     const int past = q.len - q.n_new + 1;  // tokens that the first new one sees
     // the part of one item that falls into the stretch
-    const int item = (unit - seq_unit) / units.per, from = (unit - seq_unit) - item * units.per;
-    const int upto = min(units.per, from + (end_unit - unit));
-    const int item_unit = unit - from;
-    unit += upto - from;
+    const int with = kItemUnits + units.per, item = (unit - seq_unit) / with, item_unit = seq_unit + item * with;
+    const int from = max(unit - item_unit - kItemUnits, 0), upto = min(end_unit - item_unit - kItemUnits, units.per);
+    unit = item_unit + kItemUnits + upto;
+    if (upto <= from) break;  // the item's work begins in the next stretch
     const int row_tiles = WEIGHTS ? 1 : units.items / k.c.kv_heads;
     const int head = item / row_tiles;
     const int first_tile = WEIGHTS ? 0 : item % row_tiles;
@@ -894,29 +905,30 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
             const int more = extra * (each + 1);
             return u < more ? u / (each + 1) : extra + (u - more) / each;
           };
-          const int c0 = parts ? cta - part : cta_of(item_unit);
-          const int count_parts = parts ? parts : cta_of(item_unit + units.per - 1) - c0 + 1;
+          const int c0 = parts ? cta - part : cta_of(item_unit + kItemUnits);
+          const int count_parts = parts ? parts : cta_of(item_unit + kItemUnits + units.per - 1) - c0 + 1;
           uint32_t *counters = static_cast<uint32_t *>(k.a.workspace);
           // whether this CTA is the last of `of` to arrive; all that the others wrote is then visible
           auto last_of = [&](uint32_t *counter, int of) {
-            __threadfence();
             __syncthreads();
             if (tid == 0) {
+              __threadfence();  // with the barrier before it, for the whole CTA
               const bool last = atomicAdd(counter, 1u) == (uint32_t)of - 1u;
               if (last) *counter = 0;
               share[0] = last;
+              __threadfence();
             }
             __syncthreads();
-            const bool last = share[0];
-            if (last) __threadfence();
-            return last;
+            return share[0] != 0;
           };
-          // up to kJoin parts at once, then the groups' results, which take the place of their first parts
+          // up to kJoin parts at once; more in groups (as many as each has parts), whose results take the place of
+          // their first parts, and then these
           constexpr int I = R * D / 4 / kAttnThreads;
           float4 x[I];
           float m[I], l[I];
-          const int group = (cta - c0) / kJoin, head_cta = c0 + group * kJoin;
-          const int in_group = min(kJoin, count_parts - group * kJoin), groups = (count_parts + kJoin - 1) / kJoin;
+          const int join = count_parts <= kJoin ? kJoin : (int)ceilf(sqrtf((float)count_parts));
+          const int group = (cta - c0) / join, head_cta = c0 + group * join;
+          const int in_group = min(join, count_parts - group * join), groups = (count_parts + join - 1) / join;
           bool last = last_of(counters + (group ? 2 : 1) * kAttnCtas + head_cta, in_group);
           if (last) join_parts<D, R, I>(k, c0, head_cta, in_group, 1, x, m, l);
           if (last && groups > 1) {
@@ -932,7 +944,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
               }
             }
             last = last_of(counters + c0, groups);
-            if (last) join_parts<D, R, I>(k, c0, c0, groups, kJoin, x, m, l);
+            if (last) join_parts<D, R, I>(k, c0, c0, groups, join, x, m, l);
           }
           if (last) {
 #pragma unroll
