@@ -413,30 +413,31 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 // Exclusive sums over the CTA (also of two counts below 2^16 each, packed).
 __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t *total, uint32_t *shared) {
+  constexpr int kWarps = kSelectThreads / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  uint32_t sum = v;
+  auto warp_scan = [&](uint32_t x) {
 #pragma unroll
-  for (int o = 1; o < 32; o *= 2) {
-    const uint32_t n = __shfl_up_sync(0xffffffffu, sum, o);
-    if (lane >= o) sum += n;
-  }
+    for (int o = 1; o < 32; o *= 2) {
+      const uint32_t n = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += n;
+    }
+    return x;
+  };
+  const uint32_t sum = warp_scan(v);
   __syncthreads();
   if (lane == 31) shared[warp] = sum;
   __syncthreads();
-  uint32_t before = 0, all = 0;
-#pragma unroll
-  for (int k = 0; k < kSelectThreads / 32; ++k) {
-    if (k < warp) before += shared[k];
-    all += shared[k];
-  }
-  *total = all;
-  return before + sum - v;
+  if (warp == 0) shared[lane] = warp_scan(lane < kWarps ? shared[lane] : 0u);
+  __syncthreads();
+  *total = shared[kWarps - 1];
+  return (warp ? shared[warp - 1] : 0u) + sum - v;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4View c, Kv4Batch b, Kv4Evict e, bool shared,
+template <bool SHARED>
+__global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4View c, Kv4Batch b, Kv4Evict e,
                                                                     uint32_t *status) {
   constexpr int kBins = 2048;
-  __shared__ uint32_t hist[kBins], scan[kSelectThreads / 32], found[2];
+  __shared__ uint32_t hist[kBins], scan[32], found[2];
   extern __shared__ uint32_t shared_keys[];
   const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
   int len = b.lens[seq];
@@ -447,7 +448,7 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4View c, K
   const EvictWorkspace ws =
       evict_workspace(e.workspace, (int64_t)b.n_seqs * c.kv_heads, b.max_len, e.budget);
   const int64_t row = (int64_t)seq * c.kv_heads + head;
-  uint32_t *keys = shared ? shared_keys : ws.keys + row * b.max_len;
+  uint32_t *keys = SHARED ? shared_keys : ws.keys + row * b.max_len;
   int32_t *list = ws.list + row * e.budget;
   const int count = min(len, e.budget);
   if (head == 0 && tid == 0) ws.count[seq] = count;
@@ -630,14 +631,16 @@ cudaError_t launch_kv4_evict(const Kv4View &c, const Kv4Batch &b, const Kv4Evict
   const uint64_t bit = (uint64_t)1 << (device & 63);
   if (!(ready.load(std::memory_order_relaxed) & bit)) {
     const cudaError_t err =
-        cudaFuncSetAttribute(kv4_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectShared);
+        cudaFuncSetAttribute(kv4_select_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectShared);
     if (err != cudaSuccess) return err;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
   const int64_t bytes = (int64_t)b.max_len * 4;
-  const bool shared = bytes <= kSelectShared;
-  kv4_select_kernel<<<dim3((unsigned)c.kv_heads, (unsigned)b.n_seqs), kSelectThreads, shared ? (size_t)bytes : 0,
-                      stream>>>(c, b, e, shared, status);
+  const dim3 rows((unsigned)c.kv_heads, (unsigned)b.n_seqs);
+  if (bytes <= kSelectShared)
+    kv4_select_kernel<true><<<rows, kSelectThreads, (size_t)bytes, stream>>>(c, b, e, status);
+  else
+    kv4_select_kernel<false><<<rows, kSelectThreads, 0, stream>>>(c, b, e, status);
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   const int most = e.budget < b.max_len ? e.budget : b.max_len;

@@ -58,7 +58,7 @@ namespace ksb {
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
 constexpr int kTileBlocks = 2, kTileTokens = kTileBlocks * kKv4Block;
 constexpr int kUnitTokens = kAttnWarps * kTileTokens;
-constexpr int kJoin = 8;  // parts that are joined at once
+constexpr int kJoin = 8;  // parts that are loaded together to be joined
 // Words at the start of the workspace, 0 between calls: three per CTA, of the
 // item that begins in its stretch (finished groups of parts), of that item's
 // first group of parts and of a later group, which begins at this CTA.
@@ -362,7 +362,7 @@ __device__ __forceinline__ int cta_scan(int v, int *total, int *shared) {
 template <int D, int R, int I>
 __device__ __forceinline__ void join_parts(const Kv4AttnArgs &k, int c0, int first, int count, int step,
                                            float4 (&x)[I], float (&m)[I], float (&l)[I]) {
-  constexpr int B = I <= 2 ? 8 : 4;  // parts in flight
+  constexpr int B = I <= 2 ? kJoin : kJoin / 2;  // parts in flight
 #pragma unroll
   for (int i = 0; i < I; ++i) {
     x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -921,12 +921,12 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
             __syncthreads();
             return share[0] != 0;
           };
-          // up to kJoin parts at once; more in groups (as many as each has parts), whose results take the place of
-          // their first parts, and then these
+          // few parts at once; more in groups (about as many as each has parts, these a multiple of what is loaded
+          // together), whose results take the place of their first parts, and then these
           constexpr int I = R * D / 4 / kAttnThreads;
           float4 x[I];
           float m[I], l[I];
-          const int join = count_parts <= kJoin ? kJoin : (int)ceilf(sqrtf((float)count_parts));
+          const int join = (int)ceilf(sqrtf((float)count_parts) / kJoin) * kJoin;
           const int group = (cta - c0) / join, head_cta = c0 + group * join;
           const int in_group = min(join, count_parts - group * join), groups = (count_parts + join - 1) / join;
           bool last = last_of(counters + (group ? 2 : 1) * kAttnCtas + head_cta, in_group);
