@@ -648,7 +648,7 @@ int ks_b200_kv4_read_async(const ks_b200_kv4_cache *cache,
  * before its first use (its first 8192 bytes are 0 again after each call, so
  * calls of any sizes may follow one another in it), not shared by calls that
  * may run at the same time (two graphs that replay at the same time need one
- * each).  After a call whose status reports a timeout, zero it again.
+ * each).
  */
 size_t ks_b200_kv4_attention_workspace(const ks_b200_kv4_cache *cache,
                                        size_t q_heads, size_t n_seqs,

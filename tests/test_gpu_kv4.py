@@ -286,6 +286,47 @@ def test_long_and_split(ks, cuda):
         _check(c, q, d**-0.5, out, lse, dtype)
 
 
+@pytest.mark.parametrize("n,heads,q_heads,dtype", [(33, 32, 32, "bf16"), (40, 1, 3, "f32"), (100, 2, 8, "f16"),
+                                                   (129, 1, 2, "f32"), (300, 3, 3, "bf16")])
+def test_many_sequences(ks, cuda, n, heads, q_heads, dtype):
+    """More sequences than a warp has lanes and a CTA threads, of unequal lengths, some without tokens."""
+    rng = np.random.default_rng(n)
+    lens = [int(x) for x in rng.integers(0, 90, n)]
+    lens[n // 2] = 1500
+    news = [min(int(x), 1) if s % 7 else min(int(x), 3) for s, x in enumerate(lens)]
+    news[1], lens[1] = 1, 0
+    c = Seqs(ks, cuda, lens, news, heads, 64, 64, 32, seed=n, weights=True)
+    before = c.w.double().cpu().numpy()
+    q = _query(c, q_heads, dtype)
+    out, lse = _attend(c, q, 0.125, accumulate=True)
+    c.ok()
+    _check(c, q, 0.125, out, lse, dtype, weights=c.w, before=before)
+
+
+def test_one_workspace_for_calls_of_all_sizes(ks, cuda):
+    """Calls of any sizes follow one another in one workspace, zeroed once."""
+    import torch
+
+    cases = []
+    for i, (lens, heads, q_heads, d, new) in enumerate([([5000], 1, 4, 128, 1), ([40, 900, 3], 2, 4, 64, 3),
+                                                        ([17] * 20, 4, 4, 128, 1), ([2500], 1, 1, 64, 1)]):
+        c = Seqs(ks, cuda, lens, [min(new, n) for n in lens], heads, d, 32, 64, seed=i)
+        cases.append((c, _query(c, q_heads, "f32"), max(lens), new))
+    need = max(ks.kv4_attention_workspace(c.cache, q.shape[1], len(c.lens), c.tokens, new, most)
+               for c, q, most, new in cases)
+    ws = torch.zeros(need, dtype=torch.uint8, device=cuda)
+    outs = []
+    for _ in range(2):
+        for c, q, most, new in cases:
+            out, lse = torch.zeros_like(q), torch.zeros(q.shape[:2], device=cuda)
+            ks.kv4_attention_async(c.cache, c.table, c.seq_lens, q, out, 0.1, ws, token_offsets=c.offsets, max_new=new,
+                                   max_len=most, lse=lse, status=c.status)
+            outs.append((c, q, out, lse))
+    for c, q, out, lse in outs:
+        c.ok()
+        _check(c, q, 0.1, out, lse, "f32")
+
+
 def test_empty_rows_and_rows_behind(ks, cuda):
     """Sequences without tokens, new tokens before position 0, rows before and behind the sequences, strided rows."""
     import torch
@@ -569,6 +610,21 @@ def test_evict(ks, cuda, d, group, page, lens, budget, recent):
             assert (got[keep[s]:] == 7).all()
 
 
+def test_evict_long(ks, cuda):
+    """More tokens than keys fit shared memory."""
+    import torch
+
+    n, budget, recent = 60001, 20011, 13
+    c = Seqs(ks, cuda, [n, 300], [0, 0], 1, 64, 64, 256, weights=True)
+    c.w.copy_(torch.floor(c.w * 4096) / 4096)  # with ties
+    _, _, w, _, _, to_lens, kept, keep = _evict(c, budget, recent)
+    c.ok()
+    assert to_lens.tolist() == keep == [budget, 300]
+    at = c.weights_of(0, c.w.cpu().numpy())[0]
+    assert (kept[0, 0].cpu().numpy() == _kept_of(at, n, budget, recent)).all()
+    assert kept[1, 0, :300].tolist() == list(range(300))
+
+
 def test_evict_in_place_lengths_and_no_list(ks, cuda):
     c = Seqs(ks, cuda, [90, 20, 64], [0] * 3, 3, 64, 32, 16, weights=True)
     _, _, _, _, _, to_lens, _, keep = _evict(c, 50, 10, kept=False, to_lens=c.seq_lens)
@@ -653,3 +709,47 @@ def test_generation(ks, cuda, dtype, d, group, q_heads):
     for _ in range(3):
         step([1, 1])
     step([3, 1])
+
+
+def test_with_the_w4a8_products(ks, cuda, oracle):
+    """A decode step around the cache, as the library's other calls make it: queries, keys and values are columns of one
+    W4A8 GEMM's output, read and appended in place, and the attention's result is quantised for the next GEMM."""
+    import torch
+
+    m, hidden, heads, kv_heads, d, group, page = 6, 512, 8, 2, 64, 32, 16
+    cols = (heads + 2 * kv_heads) * d
+    rng = np.random.default_rng(8)
+    x = rng.integers(-127, 128, (m, hidden), dtype=np.int8)
+    sx = rng.uniform(0.002, 0.004, m).astype(np.float32)
+    w = [rng.integers(0, 256, (n, k // 2), dtype=np.uint8) for n, k in ((cols, hidden), (hidden, heads * d))]
+    sw = [rng.uniform(2e-3, 4e-3, (n, k // 32)).astype(np.float16) for n, k in ((cols, hidden), (hidden, heads * d))]
+    dev = lambda a: torch.from_numpy(a.view(np.uint16) if a.dtype == np.float16 else a).to(cuda)  # noqa: E731
+    lens = [9, 40, 1, 17, 33, 64]
+    c = Seqs(ks, cuda, lens, [1] * m, kv_heads, d, group, page)
+    qkv = torch.zeros(m, cols, device=cuda)
+    ks.gemm_w4a8_async(dev(x), dev(sx), dev(w[0]), dev(sw[0]), qkv, m, cols, hidden, 32, status=c.status)
+    rows = qkv.view(m, heads + 2 * kv_heads, d)
+    q, k, v = rows[:, :heads], rows[:, heads:heads + kv_heads], rows[:, heads + kv_heads:]
+    ks.kv4_append_async(c.cache, c.table, c.seq_lens, k, v, status=c.status)
+    out, lse = _attend(c, q, d**-0.5, out=torch.zeros(m, heads, d, device=cuda), offsets=False)
+    a, sa = torch.zeros(m, heads * d, dtype=torch.int8, device=cuda), torch.zeros(m, device=cuda)
+    ks.quantize_per_token_async(out, heads * d, m, heads * d, a, heads * d, sa)
+    y = torch.zeros(m, hidden, device=cuda)
+    ks.gemm_w4a8_async(a, sa, dev(w[1]), dev(sw[1]), y, m, hidden, heads * d, 32, status=c.status)
+    c.ok()
+    # the definition, from the GEMM's own output on
+    for s, n in enumerate(lens):
+        p, slot = c.pages[s][(n - 1) // page], (n - 1) % page
+        c.k[p, :, slot] = O.kv4_value(*O.kv4_quantize(k[s].double().cpu().numpy(), group))
+        c.v[p, :, slot] = O.kv4_value(*O.kv4_quantize(v[s].double().cpu().numpy(), group))
+        c.scale_max = max(c.scale_max, O.kv4_quantize(k[s].double().cpu().numpy(), group)[1].astype(np.float64).max())
+    _check(c, q, d**-0.5, out, lse, "f32")
+    for s in range(m):
+        rc, want = oracle.matvec_w4a8_f16(x[s], w[0], hidden // 2, sw[0].view(np.uint16), hidden // 32, cols, hidden, 32,
+                                          float(sx[s]))
+        assert rc == 0 and O.w4a8_tolerance_ok(qkv[s].cpu().numpy(), want)[0]
+        rc, qs, scale = oracle.quantize_per_token(out[s].reshape(-1).cpu().numpy())
+        assert (a[s].cpu().numpy() == qs).all() and float(sa[s]) == np.float32(scale)
+        rc, want = oracle.matvec_w4a8_f16(qs, w[1], heads * d // 2, sw[1].view(np.uint16), heads * d // 32, hidden,
+                                          heads * d, 32, float(scale))
+        assert rc == 0 and O.w4a8_tolerance_ok(y[s].cpu().numpy(), want)[0]

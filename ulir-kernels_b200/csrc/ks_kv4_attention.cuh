@@ -10,7 +10,9 @@
 // units of work.  All units of the call stand in one line (sequence, head,
 // row tile, tokens) and every CTA of a grid that the GPU holds at once takes an
 // equal stretch of it, so that sequences of unequal lengths and few long ones
-// alike fill the GPU evenly.  Of an item (a row tile and all its tokens) that
+// alike fill the GPU evenly (an item's beginning counts as three units more,
+// about what it costs: 64 sequences of up to 8192 tokens, 8 heads, 72 us, 96
+// without; where few items give each CTA about one, it gets a part of one item).  Of an item (a row tile and all its tokens) that
 // a stretch ends within, each CTA leaves its part (maximum, sum, unnormalised
 // output, f32) in the workspace; the last of them to finish joins the parts in
 // their order, so results do not depend on which one that is.  Within a CTA
@@ -37,6 +39,16 @@
 // per group.  The maximum that the exponentials refer to, and that power of
 // two, are only raised when a tile exceeds them (the maximum by 2^4), which a
 // vote finds: most tiles need no reduction over lanes and no rescaling.
+//
+// What bounds it.  Making the operands: about 260 instructions of a warp for 16
+// tokens of a head (f16, bf16; 128 elements) and 390 (f32), issued in 0.55 of
+// the cycles, half of them on the integer pipe, while the tensor cores are busy a
+// fifth of the time (which is why these are the warp-wide products, whose A
+// operand is made in registers: a tensor-memory operand would have to be stored
+// there first, and the products are not what takes the time).  592 equal
+// items of 4096 tokens, group 128, bf16: 73 us, 4.4 TB/s of codes and scales,
+// where the same copies without the products take 58; f32 in 444 items, group
+// 32: 83 us, 3.2 TB/s.
 //
 // Precision.  Codes are exact in f16.  For f32 tensors queries (scaled by a
 // power of two per row) and weighted probabilities are split into two f16
@@ -80,8 +92,10 @@ struct Kv4AttnArgs {
   uint32_t *status;
 };
 
-// CTAs of a pass that an SM holds: bounded by registers (about 128 a thread
-// for one part of the queries, 168 for two; twice the accumulators with NT 2).
+// CTAs of a pass that an SM holds, bounded by registers: 128 a thread for one
+// part of the queries, 168 for two, 255 with NT 2.  (f16 and bf16 with 3 CTAs of
+// 168 registers: 88 us where 4 of 128 take 74, at 148 x 4096 tokens x 4 heads of
+// 128.)
 constexpr int kv4_ctas_per_sm(int nt, int qs) { return nt == 1 ? (qs == 1 ? 4 : 3) : 2; }
 
 // Partial results of CTA c: rows_tile x head_dim f32, then rows_tile maxima
@@ -449,7 +463,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
     each = total / ctas, extra = total - each * ctas;
     // the shortest part that gives no more parts than CTAs: lane l counts those of candidate l % 4 in every eighth
     // sequence
-    const int shortest = (units + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int shortest = max((units + (int)gridDim.x - 1) / (int)gridDim.x, 1);
     int count = 0;
 #pragma unroll
     for (int s = 0; s < 32; s += 8) {
@@ -615,10 +629,9 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       __syncthreads();
 
       // In powers of two: top, the maximum of rows 2t, 2t + 1 at its last rise (limit: the score, without the row's
-      // factor, at which it has to rise again), and
-      // base, what the exponentials refer to: top - lift, where 2^lift brings the largest value scale into
-      // [2^10, 2^11), so that products with probabilities up to 2^4 stay below f16's largest.  (lse in the weights'
-      // pass.)  Outputs and sums are both in units of 2^base.
+      // factor, at which it has to rise again), and base, what the exponentials refer to: top - lift, where 2^lift brings
+      // the largest value scale into [2^10, 2^11), so that products with probabilities up to 2^4 stay below f16's
+      // largest.  (lse in the weights' pass.)  Outputs and sums are both in units of 2^base.
       float factor[NT][2], base[NT][2], top[NT][2], limit[NT][2], sum[NT][2];
       int sees[NT][2];  // tokens that these rows see
 #pragma unroll

@@ -26,6 +26,7 @@ int cuda_fail(cudaError_t e, const char *what) {
 }
 
 constexpr size_t kMost = 0x7FFFFFFF;
+constexpr size_t kMaxLen = kMost - 16384;  // positions of 32 tiles ahead are 32-bit
 constexpr size_t kPlanSms = 148;  // a B200's; a constant, so that the workspace needs no device to be known
 
 bool misaligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) != 0; }
@@ -74,7 +75,7 @@ int batch_of(const Kv4View &v, const int32_t *page_table, size_t stride, const i
   const size_t holds = stride << v.page_shift;
   if (max_len > holds) return fail(KS_ERR_INVALID_ARG, "max_len is more than a row of the page table holds");
   if (max_len == 0) max_len = holds < kMost ? holds : kMost;
-  if (max_len > kMost - 1024) max_len = kMost - 1024;  // positions and tile ends are 32-bit
+  if (max_len > kMaxLen) max_len = kMaxLen;
   b->table = page_table;
   b->table_stride = (int64_t)stride;
   b->lens = seq_lens;
@@ -115,9 +116,9 @@ Kv4Plan plan_of(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_
 
 bool attention_sizes_ok(const Kv4View &v, size_t q_heads, size_t n_seqs, size_t max_new, size_t max_len) {
   return q_heads > 0 && q_heads % v.kv_heads == 0 && q_heads <= kMost && n_seqs > 0 && n_seqs <= 65535 && max_new > 0 &&
-         max_len > 0 && max_new <= max_len && max_len <= kMost - 1024 && max_new <= kMost / q_heads &&
+         max_len > 0 && max_new <= max_len && max_len <= kMaxLen && max_new <= kMost / q_heads &&
          // units of work, a row tile of at least 8 rows and 128 tokens each, are counted in 31 bits
-         n_seqs * v.kv_heads <= kMost / (max_new * (q_heads / v.kv_heads) / 8 + 1) / (max_len / kUnitTokens + 1);
+         n_seqs * v.kv_heads <= kMost / (max_new * (q_heads / v.kv_heads) / 8 + 1) / (max_len / kUnitTokens + 1 + kItemUnits);
 }
 
 // The counters, then two parts of every CTA: for any type (f16 and bf16 have the most CTAs).
