@@ -47,41 +47,61 @@ struct Kv4Runs {
   static __host__ __device__ constexpr int shift(int e) { return V ? (e / 4 % 4) * 8 + (e % 2) * 4 : (e % 8) * 4; }
 };
 
-template <typename T, int N>
-__device__ __forceinline__ void load_run(const T *p, bool vec, float *v) {
-  constexpr int kBytes = N * sizeof(T);
-  if (vec) {
-    T x[N];
-    if constexpr (kBytes == 8)
-      *reinterpret_cast<uint2 *>(x) = *reinterpret_cast<const uint2 *>(p);
-    else
+// One 32-bit word of a tensor's elements as f32, and back.
+__device__ __forceinline__ void unpack_word(uint32_t w, float *v, const float *) { v[0] = __uint_as_float(w); }
+__device__ __forceinline__ void unpack_word(uint32_t w, float *v, const __half *) {
+  const float2 f = unpack_f16(w);
+  v[0] = f.x, v[1] = f.y;
+}
+__device__ __forceinline__ void unpack_word(uint32_t w, float *v, const __nv_bfloat16 *) {
+  v[0] = __uint_as_float(w << 16), v[1] = __uint_as_float(w & 0xFFFF0000u);
+}
+__device__ __forceinline__ uint32_t pack_word(const float *v, const float *) { return __float_as_uint(v[0]); }
+__device__ __forceinline__ uint32_t pack_word(const float *v, const __half *) { return pack_f16(v[0], v[1]); }
+__device__ __forceinline__ uint32_t pack_word(const float *v, const __nv_bfloat16 *) {
+  const __nv_bfloat162 b = __floats2bfloat162_rn(v[0], v[1]);
+  return *reinterpret_cast<const uint32_t *>(&b);
+}
+
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void load_run(const T *p, float *v) {
+  constexpr int kWords = N * sizeof(T) / 4, kPer = 4 / sizeof(T);
+  if constexpr (VEC) {
+    uint32_t w[kWords];
+    if constexpr (kWords == 2) {
+      const uint2 x = *reinterpret_cast<const uint2 *>(p);
+      w[0] = x.x, w[1] = x.y;
+    } else {
 #pragma unroll
-      for (int k = 0; k < kBytes / 16; ++k)
-        reinterpret_cast<uint4 *>(x)[k] = reinterpret_cast<const uint4 *>(p)[k];
+      for (int k = 0; k < kWords; k += 4) {
+        const uint4 x = reinterpret_cast<const uint4 *>(p)[k / 4];
+        w[k] = x.x, w[k + 1] = x.y, w[k + 2] = x.z, w[k + 3] = x.w;
+      }
+    }
 #pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = kv4_load(&x[k]);
+    for (int k = 0; k < kWords; ++k) unpack_word(w[k], v + k * kPer, p);
   } else {
 #pragma unroll
     for (int k = 0; k < N; ++k) v[k] = kv4_load(p + k);
   }
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void store_run(T *p, bool vec, const float *v) {
-  constexpr int kBytes = N * sizeof(T);
-  T x[N];
+template <typename T, int N, bool VEC>
+__device__ __forceinline__ void store_run(T *p, const float *v) {
+  constexpr int kWords = N * sizeof(T) / 4, kPer = 4 / sizeof(T);
+  if constexpr (VEC) {
+    uint32_t w[kWords];
 #pragma unroll
-  for (int k = 0; k < N; ++k) kv4_store(&x[k], v[k]);
-  if (vec) {
-    if constexpr (kBytes == 8)
-      *reinterpret_cast<uint2 *>(p) = *reinterpret_cast<const uint2 *>(x);
+    for (int k = 0; k < kWords; ++k) w[k] = pack_word(v + k * kPer, p);
+    if constexpr (kWords == 2)
+      *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
     else
 #pragma unroll
-      for (int k = 0; k < kBytes / 16; ++k)
-        reinterpret_cast<uint4 *>(p)[k] = reinterpret_cast<const uint4 *>(x)[k];
+      for (int k = 0; k < kWords; k += 4)
+        reinterpret_cast<uint4 *>(p)[k / 4] = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
   } else {
 #pragma unroll
-    for (int k = 0; k < N; ++k) p[k] = x[k];
+    for (int k = 0; k < N; ++k) kv4_store(p + k, v[k]);
   }
 }
 
@@ -187,8 +207,13 @@ __device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *pl
     const T *src = x + (int64_t)(first_row + token) * token_stride + head * head_stride;
     const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
     float v[E];
+    if (vec) {
 #pragma unroll
-    for (int r = 0; r < R::kRuns; ++r) load_run<T, R::kLength>(src + R::first(t, r), vec, v + r * R::kLength);
+      for (int r = 0; r < R::kRuns; ++r) load_run<T, R::kLength, true>(src + R::first(t, r), v + r * R::kLength);
+    } else {
+#pragma unroll
+      for (int r = 0; r < R::kRuns; ++r) load_run<T, R::kLength, false>(src + R::first(t, r), v + r * R::kLength);
+    }
     const Kv4Place p = places[token];
     if (p.page < 0) continue;
     // extremes of the thread's 8 elements of every 32 (e / 8 for both orders; NaN is passed over)
@@ -225,9 +250,11 @@ __device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *pl
     }
     const __half mine = kv4_scale(l, h);
     const float scale = __half2float(mine), inverse = __fdiv_rn(1.0f, scale);
-    // Codes are q = rne(v * (1 / s)), at most one beside rne(v / s) and that only next to a tie: then the remainder
-    // v - q * s (exact) is at least half of s.  Held scales (v / s may leave [-8.5, 7.5]) and values that are not
-    // finite go through the quotient.  A word is q + 8 in base 16, exact in f32 four codes at a time.
+    // Codes are q = rne(v * (1 / s)) with 1 / s in two parts: the f32 nearest to a quotient that is off by no more than
+    // 2^-45, so a quotient on a tie gives the tie.  One beside a tie gives it too only if that is within 2^-24, which is
+    // ruled out where v has 11 bits (s has, so they differ by 2^-16 at least); for f32 the remainder v - q * s (exact)
+    // then decides.  Held scales (v / s may leave [-8.5, 7.5]) and values that are not finite go through the quotient.
+    // A word is q + 8 in base 16, exact in f32 four codes at a time.
     const bool plain = zero == 0.0f;
     odd |= !plain;
     float sums[D / 32][2];
@@ -235,20 +262,22 @@ __device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *pl
     for (int w = 0; w < D / 32; ++w) sums[w][0] = sums[w][1] = 8388608.0f + 34952.0f;  // 2^23 + 0x8888
 #pragma unroll
     for (int g = 0; g < G32; ++g) {
-      const float s = __shfl_sync(lanes, scale, g, 4), inv = __shfl_sync(lanes, inverse, g, 4), half = 0.5f * s;
-      float q[8], off = -1.0f;
+      const float s = __shfl_sync(lanes, scale, g, 4), inv = __shfl_sync(lanes, inverse, g, 4);
+      const float rest = __fmaf_rn(-s, inv, 1.0f) * inv;
+      float q[8], off = 0.0f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        q[e] = __fsub_rn(__fadd_rn(v[8 * g + e] * inv, kMagic), kMagic);
-        off = fmaxf(off, fabsf(__fmaf_rn(-q[e], s, v[8 * g + e])) - half);
+        const float y = __fmaf_rn(v[8 * g + e], inv, v[8 * g + e] * rest);
+        q[e] = __fsub_rn(__fadd_rn(y, kMagic), kMagic);
+        if (sizeof(T) == 4) off = fmaxf(off, fabsf(y - q[e]));
       }
       if (!plain || s >= 65504.0f || s < 0x1p-14f) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) q[e] = kv4_code(isnan(v[8 * g + e]) ? 0.0f : v[8 * g + e], s);
-      } else if (off >= 0.0f) {
+      } else if (sizeof(T) == 4 && off >= 0.5f - 0x1p-20f) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float r = __fmaf_rn(-q[e], s, v[8 * g + e]);
+          const float r = __fmaf_rn(-q[e], s, v[8 * g + e]), half = 0.5f * s;
           const bool is_odd = __float_as_uint(q[e] + kMagic) & 1u;
           if (fabsf(r) > half || (fabsf(r) == half && is_odd)) q[e] += copysignf(1.0f, r);
         }
@@ -319,15 +348,15 @@ __device__ __forceinline__ void read_rows(const Kv4View &c, const Kv4Place *plac
 #pragma unroll
       for (int w = 0; w < D / 32; ++w) word_codes(words[n][w], f[w]);
       const bool vec = (reinterpret_cast<uintptr_t>(dst[n]) & 15) == 0;
+      float v[D / 4];
 #pragma unroll
-      for (int r = 0; r < R::kRuns; ++r) {
-        float v[R::kLength];
+      for (int e = 0; e < D / 4; ++e) v[e] = f[R::word(e)][R::shift(e) / 4] * s[n][e / 8];  // exact in f32
+      if (vec) {
 #pragma unroll
-        for (int k = 0; k < R::kLength; ++k) {
-          const int e = r * R::kLength + k;
-          v[k] = f[R::word(e)][R::shift(e) / 4] * s[n][e / 8];  // exact in f32
-        }
-        store_run<T, R::kLength>(dst[n] + R::first(t, r), vec, v);
+        for (int r = 0; r < R::kRuns; ++r) store_run<T, R::kLength, true>(dst[n] + R::first(t, r), v + r * R::kLength);
+      } else {
+#pragma unroll
+        for (int r = 0; r < R::kRuns; ++r) store_run<T, R::kLength, false>(dst[n] + R::first(t, r), v + r * R::kLength);
       }
     }
   }
