@@ -164,11 +164,11 @@ __device__ __forceinline__ void find_places(const Kv4View &c, const Kv4Batch &b,
 
 // Of x[0 .. 2N), the lane keeps the extremes of its own and its partner's (lane ^ o) upper or lower N, in x[0 .. N).
 template <int N, bool MAX, int SIZE>
-__device__ __forceinline__ void hand_over(float (&x)[SIZE], int o, bool upper, unsigned lanes) {
+__device__ __forceinline__ void hand_over(float (&x)[SIZE], int o, bool upper) {
 #pragma unroll
   for (int g = 0; g < N; ++g) {
     const float give = upper ? x[g] : x[g + N], keep = upper ? x[g + N] : x[g];
-    const float got = __shfl_xor_sync(lanes, give, o);
+    const float got = __shfl_xor_sync(0xffffffffu, give, o);
     x[g] = MAX ? fmaxf(keep, got) : fminf(keep, got);
   }
 }
@@ -200,22 +200,23 @@ __device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *pl
   constexpr float kMagic = 12582912.0f;   // 1.5 * 2^23: adding it rounds to an integer, ties to even
   constexpr int group = D / NG;
   const int t = threadIdx.x & 3;
-  const unsigned lanes = 15u << (threadIdx.x & 28);
   bool odd = false;
-  for (RowWalk at(threadIdx.x >> 2, c.kv_heads); at.token < tokens; at.next()) {
+  // whole warps go on while one of their rows is there
+  for (RowWalk at(threadIdx.x >> 2, c.kv_heads); __any_sync(0xffffffffu, at.token < tokens); at.next()) {
     const int token = at.token, head = at.head;
+    const Kv4Place p = token < tokens ? places[token] : Kv4Place{-1, 0};
     const T *src = x + (int64_t)(first_row + token) * token_stride + head * head_stride;
-    const bool vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
     float v[E];
-    if (vec) {
+    if (p.page < 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = 0.0f;
+    } else if ((reinterpret_cast<uintptr_t>(src) & 15) == 0) {
 #pragma unroll
       for (int r = 0; r < R::kRuns; ++r) load_run<T, R::kLength, true>(src + R::first(t, r), v + r * R::kLength);
     } else {
 #pragma unroll
       for (int r = 0; r < R::kRuns; ++r) load_run<T, R::kLength, false>(src + R::first(t, r), v + r * R::kLength);
     }
-    const Kv4Place p = places[token];
-    if (p.page < 0) continue;
     // extremes of the thread's 8 elements of every 32 (e / 8 for both orders; NaN is passed over)
     float lo[G32], hi[G32], zero = 0.0f;
 #pragma unroll
@@ -231,22 +232,22 @@ __device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *pl
     // over the four threads: each step hands the other half of the groups to the partner, thread t ends with group of
     // 32 t (t % 2 where there are two), makes the scale of its group and all take it from there
     if constexpr (G32 == 4) {
-      hand_over<2, false>(lo, 2, t & 2, lanes);
-      hand_over<2, true>(hi, 2, t & 2, lanes);
+      hand_over<2, false>(lo, 2, t & 2);
+      hand_over<2, true>(hi, 2, t & 2);
     } else {
 #pragma unroll
       for (int g = 0; g < 2; ++g) {
-        lo[g] = fminf(lo[g], __shfl_xor_sync(lanes, lo[g], 2));
-        hi[g] = fmaxf(hi[g], __shfl_xor_sync(lanes, hi[g], 2));
+        lo[g] = fminf(lo[g], __shfl_xor_sync(0xffffffffu, lo[g], 2));
+        hi[g] = fmaxf(hi[g], __shfl_xor_sync(0xffffffffu, hi[g], 2));
       }
     }
-    hand_over<1, false>(lo, 1, t & 1, lanes);
-    hand_over<1, true>(hi, 1, t & 1, lanes);
+    hand_over<1, false>(lo, 1, t & 1);
+    hand_over<1, true>(hi, 1, t & 1);
     float l = lo[0], h = hi[0];
 #pragma unroll
     for (int o = 1; 32 * o < group; o *= 2) {
-      l = fminf(l, __shfl_xor_sync(lanes, l, o));
-      h = fmaxf(h, __shfl_xor_sync(lanes, h, o));
+      l = fminf(l, __shfl_xor_sync(0xffffffffu, l, o));
+      h = fmaxf(h, __shfl_xor_sync(0xffffffffu, h, o));
     }
     const __half mine = kv4_scale(l, h);
     const float scale = __half2float(mine), inverse = __fdiv_rn(1.0f, scale);
@@ -262,7 +263,7 @@ __device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *pl
     for (int w = 0; w < D / 32; ++w) sums[w][0] = sums[w][1] = 8388608.0f + 34952.0f;  // 2^23 + 0x8888
 #pragma unroll
     for (int g = 0; g < G32; ++g) {
-      const float s = __shfl_sync(lanes, scale, g, 4), inv = __shfl_sync(lanes, inverse, g, 4);
+      const float s = __shfl_sync(0xffffffffu, scale, g, 4), inv = __shfl_sync(0xffffffffu, inverse, g, 4);
       const float rest = __fmaf_rn(-s, inv, 1.0f) * inv;
       float q[8], off = 0.0f;
 #pragma unroll
@@ -294,6 +295,7 @@ __device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *pl
 #pragma unroll
     for (int w = 0; w < D / 32; ++w)
       words[w] = prmt(__float_as_uint(sums[w][0]), __float_as_uint(sums[w][1]), 0x5410) ^ 0x88888888u;
+    if (p.page < 0) continue;
     uint8_t *half = kv4_block(c, p.page, head, p.slot) + (V ? c.block_bytes / 2 : 0);
     copy_words<D / 8>(half + (p.slot & 15) * (D / 2) + t * (D / 8), words);
     constexpr int each = group / 32;
