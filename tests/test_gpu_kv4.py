@@ -303,6 +303,18 @@ def test_many_sequences(ks, cuda, n, heads, q_heads, dtype):
     _check(c, q, 0.125, out, lse, dtype, weights=c.w, before=before)
 
 
+def test_weights_beside_sequences_without_tokens(ks, cuda):
+    """Every other sequence has a new token but no cached one: the others' tokens all get their weights."""
+    for n in (20, 40, 150):
+        lens = [0 if s % 2 else 40 + s for s in range(n)]
+        c = Seqs(ks, cuda, lens, [1] * n, 8, 64, 64, 32, seed=n, weights=True)
+        before = c.w.double().cpu().numpy()
+        q = _query(c, 16, "bf16")
+        out, lse = _attend(c, q, 0.125, accumulate=True)
+        c.ok()
+        _check(c, q, 0.125, out, lse, "bf16", weights=c.w, before=before)
+
+
 def test_one_workspace_for_calls_of_all_sizes(ks, cuda):
     """Calls of any sizes follow one another in one workspace, zeroed once."""
     import torch

@@ -552,8 +552,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
     // the part of one item that falls into the stretch
     const int with = kItemUnits + units.per, item = (unit - seq_unit) / with, item_unit = seq_unit + item * with;
     const int from = max(unit - item_unit - kItemUnits, 0), upto = min(end_unit - item_unit - kItemUnits, units.per);
-    unit = item_unit + kItemUnits + upto;
-    if (upto <= from) break;  // the item's work begins in the next stretch
+    unit = upto > from ? item_unit + kItemUnits + upto : item_unit + with;
+    if (upto <= from) continue;  // its work begins in the next stretch, or (weights of no tokens) it has none
     const int row_tiles = WEIGHTS ? 1 : units.items / k.c.kv_heads;
     const int head = item / row_tiles;
     const int first_tile = WEIGHTS ? 0 : item % row_tiles;
