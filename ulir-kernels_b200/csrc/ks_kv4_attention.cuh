@@ -6,20 +6,20 @@
 // in one pass over the cache, with the running maximum and sum of the softmax.
 //
 // Work.  The rows of one key/value head (its query heads times the new
-// tokens) are cut into tiles of 8 NT; a tile's tokens, 128 at a time, are the
-// units of work.  All units of the call stand in one line (sequence, head,
-// row tile, tokens) and every CTA of a grid that the GPU holds at once takes an
-// equal stretch of it, so that sequences of unequal lengths and few long ones
-// alike fill the GPU evenly (an item's beginning counts as three units more,
-// about what it costs: 64 sequences of up to 8192 tokens, 8 heads, 72 us, 96
-// without; where few items give each CTA about one, it gets a part of one item).  Of an item (a row tile and all its tokens) that
+// tokens) are cut into tiles of 8 NT; a row tile's tokens, 128 or 256 at a
+// time, are the units of work.  All units of the call stand in one line
+// (sequence, head, row tile, tokens) and every CTA of a grid that the GPU holds
+// at once takes an equal stretch of it, so that sequences of unequal lengths and
+// few long ones alike fill the GPU evenly.  An item's beginning counts as three units more,
+// about what it costs: 64 sequences of up to 8192 tokens, 8 heads, take 70 us,
+// 98 without.  (Where few items give each CTA about one, it gets a part of one
+// item.)  Of an item (a row tile and all its tokens) that
 // a stretch ends within, each CTA leaves its part (maximum, sum, unnormalised
 // output, f32) in the workspace; the last of them to finish joins the parts in
 // their order, so results do not depend on which one that is.  Within a CTA
-// four warps take turns at tiles of 32 tokens, each through a ring of its own
-// in shared memory that its lanes fill by asynchronous 16-byte copies (a bulk
-// copy for each tile, issued by one lane, held its warp up for some 400 cycles
-// of about 3000 that it spends on a tile, ten of these copies for about 60).
+// four warps take turns at tiles of 32 or 64 tokens, each through a ring of its
+// own in shared memory that its lanes fill by asynchronous 16-byte copies (one
+// bulk copy for each tile, issued by a lane, took the same time).
 //
 // Products.  Both run on the tensor cores with the tokens' codes as the A
 // operand, made in registers, and the query rows as the 8-wide N side, so that
@@ -45,10 +45,13 @@
 // the cycles, half of them on the integer pipe, while the tensor cores are busy a
 // fifth of the time (which is why these are the warp-wide products, whose A
 // operand is made in registers: a tensor-memory operand would have to be stored
-// there first, and the products are not what takes the time).  592 equal
-// items of 4096 tokens, group 128, bf16: 73 us, 4.4 TB/s of codes and scales,
-// where the same copies without the products take 58; f32 in 444 items, group
-// 32: 83 us, 3.2 TB/s.
+// there first, and the products are not what takes the time).  444 equal
+// items of 4096 tokens, 128 elements, bf16: 54 us, 4.4 TB/s of codes and
+// scales with groups of 128, 61 us, 4.3 TB/s with groups of 32; f32 68 and 80 us,
+// 3.5 and 3.3 TB/s.  The copies without the products take 0.8 of the time.
+// A call's beginning (the lengths, the queries) and end (the four warps' sums,
+// the join of an item's parts) take 9 us together, which is what short calls
+// take.
 //
 // Precision.  Codes are exact in f16.  For f32 tensors queries (scaled by a
 // power of two per row) and weighted probabilities are split into two f16
@@ -68,8 +71,15 @@
 namespace ksb {
 
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
-constexpr int kTileBlocks = 2, kTileTokens = kTileBlocks * kKv4Block;
-constexpr int kUnitTokens = kAttnWarps * kTileTokens;
+// Blocks of a warp's tile: four where two such tiles of every warp fit shared
+// memory and their scores the registers, for fewer waits and votes (64 sequences
+// of up to 8192 tokens, bf16, groups of 128: 70 us, 72 with two blocks and four
+// CTAs; a sequence of 131072: 40, 42; 8 of 2048 in pages of 32, f16: 21, 19.5).
+__host__ __device__ constexpr int kv4_tile_blocks(int nt, int groups) { return nt == 1 && groups <= 2 ? 4 : 2; }
+// Tokens of a unit of work.
+__host__ __device__ constexpr int kv4_unit_tokens(int nt, int groups) {
+  return kAttnWarps * kv4_tile_blocks(nt, groups) * kKv4Block;
+}
 constexpr int kJoin = 8;  // parts that are loaded together to be joined
 // Words at the start of the workspace, 0 between calls: three per CTA, of the
 // item that begins in its stretch (finished groups of parts), of that item's
@@ -80,6 +90,7 @@ constexpr int kAttnCtas = 680, kAttnCounters = 2048;
 struct Kv4Plan {
   int rows_tile;  // 8 NT
   int row_tiles;  // tiles of a (sequence, key/value head), at most
+  int unit;       // tokens of a unit of work
   int ctas;
 };
 
@@ -92,11 +103,10 @@ struct Kv4AttnArgs {
   uint32_t *status;
 };
 
-// CTAs of a pass that an SM holds, bounded by registers: 128 a thread for one
-// part of the queries, 168 for two, 255 with NT 2.  (f16 and bf16 with 3 CTAs of
-// 168 registers: 88 us where 4 of 128 take 74, at 148 x 4096 tokens x 4 heads of
-// 128.)
-constexpr int kv4_ctas_per_sm(int nt, int qs) { return nt == 1 ? (qs == 1 ? 4 : 3) : 2; }
+// CTAs of a pass that an SM holds, bounded by registers: 168 a thread, 255 with
+// NT 2.  (Four CTAs of 128 registers, tiles of two blocks, f16 and bf16: the same
+// time per item over 148 sequences of 4096 tokens, 4 heads.)
+constexpr int kv4_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
 // Partial results of CTA c: rows_tile x head_dim f32, then rows_tile maxima
 // and sums; slot 0 of an item that an earlier CTA began, slot 1 of one that a
@@ -150,8 +160,9 @@ __device__ __forceinline__ int kv4_token(int g) { return g ^ ((g >> 1) & 1); }
 template <int D, int NG, int NT, int QS>
 struct Kv4Smem {
   static constexpr int kBlock = kv4_block_bytes(D, NG);
+  static constexpr int kTileBlocks = kv4_tile_blocks(NT, NG);
   static constexpr int kStage = kTileBlocks * kBlock;
-  static constexpr int kStages = kv4_ctas_per_sm(NT, QS) == 4 ? 2 : 3;
+  static constexpr int kStages = kTileBlocks == 4 ? 2 : 3;
   static constexpr int kRing = kAttnWarps * kStages * kStage;
   static constexpr int kMerge = kAttnWarps * 8 * NT * (D + 2) * 4;  // over the ring, once it is drained
   static constexpr int kQ = kRing > kMerge ? kRing : kMerge;        // NT x D/32 x QS fragments of 512 bytes
@@ -267,18 +278,18 @@ __device__ __forceinline__ void key_pairs(uint32_t x, uint32_t (&a)[4]) {
   a[3] = and_xor(x8, H, FH);
 }
 
-// The scores of a tile's tokens, without the rows' factors: s[b][nt][0..3] of
+// The scores of two blocks' tokens, without the rows' factors: s[b][nt][0..3] of
 // (token g, row 2t), (g, 2t + 1), (g + 8, 2t), (g + 8, 2t + 1) of block b,
 // tokens as kv4_token has them.
 template <int D, int NG, int NT, int QS>
-__device__ __forceinline__ void tile_scores(const char *buf, const char *smem, float (&s)[kTileBlocks][NT][4]) {
+__device__ __forceinline__ void block_scores(const char *buf, const char *smem, float (*s)[NT][4]) {
   using S = Kv4Smem<D, NG, NT, QS>;
   constexpr int W = D / 32 / NG;
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, tok = kv4_token(g);
-  uint32_t x[kTileBlocks][2][D / 32];
-  float sc[kTileBlocks][2][NG];
+  uint32_t x[2][2][D / 32];
+  float sc[2][2][NG];
 #pragma unroll
-  for (int b = 0; b < kTileBlocks; ++b)
+  for (int b = 0; b < 2; ++b)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       lds<D / 8>(buf + b * S::kBlock + (tok + 8 * e) * (D / 2) + t * (D / 8), x[b][e]);
@@ -286,7 +297,7 @@ __device__ __forceinline__ void tile_scores(const char *buf, const char *smem, f
     }
 #pragma unroll
   for (int gr = 0; gr < NG; ++gr) {
-    float acc[kTileBlocks][NT][QS][4];
+    float acc[2][NT][QS][4];
     float4 start[NT][QS];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -302,7 +313,7 @@ __device__ __forceinline__ void tile_scores(const char *buf, const char *smem, f
         for (int p = 0; p < QS; ++p)
           lds<16>(smem + S::kQ + ((nt * (D / 32) + w) * QS + p) * 512 + lane * 16, q[nt][p]);
 #pragma unroll
-      for (int b = 0; b < kTileBlocks; ++b) {
+      for (int b = 0; b < 2; ++b) {
         uint32_t u[4], v[4];
         key_pairs(x[b][0][w], u);
         key_pairs(x[b][1][w], v);
@@ -319,7 +330,7 @@ __device__ __forceinline__ void tile_scores(const char *buf, const char *smem, f
       }
     }
 #pragma unroll
-    for (int b = 0; b < kTileBlocks; ++b)
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -342,7 +353,7 @@ struct Kv4Units {
     const int rows = min(q.n_new, k.a.max_new) * k.group_heads;
     // the weights' pass takes all row tiles of a stretch of tokens together; without tokens it has nothing to do
     items = rows == 0 ? 0 : k.c.kv_heads * (WEIGHTS ? 1 : (rows + k.p.rows_tile - 1) / k.p.rows_tile);
-    per = (q.len + kUnitTokens - 1) / kUnitTokens;
+    per = (q.len + k.p.unit - 1) / k.p.unit;
     if (!WEIGHTS) per = max(per, 1);
   }
   __device__ int all() const { return (kItemUnits + per) * items; }
@@ -426,10 +437,11 @@ __device__ __forceinline__ void join_parts(const Kv4AttnArgs &k, int c0, int fir
 
 // WEIGHTS: adds the attention weights of every token to the cache's, given the rows' lse.
 template <typename T, int D, int NG, int NT, int QS, int PS, bool WEIGHTS>
-__global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_attention_kernel(const Kv4AttnArgs k) {
+__global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attention_kernel(const Kv4AttnArgs k) {
   using S = Kv4Smem<D, NG, NT, QS>;
   constexpr bool kWide = QS == 2;  // sums over tokens in f32 registers
-  constexpr int R = 8 * NT, kStages = S::kStages;
+  constexpr int R = 8 * NT, kStages = S::kStages, kTileBlocks = S::kTileBlocks, kTileTokens = kTileBlocks * kKv4Block;
+  constexpr int kUnitTokens = kv4_unit_tokens(NT, NG);
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   int *share = reinterpret_cast<int *>(smem + S::kShare);
@@ -568,25 +580,32 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
       // A lane knows where one of the next 32 of this warp's tiles stands; where that tile is whole and within a page,
       // the same copies fetch it each time.
       constexpr int N = WEIGHTS ? S::kBlock / 2 : S::kBlock;  // of a block: its keys alone, or all
-      int fetched = 0, page0 = 0, page1 = 0;
+      constexpr int kShift = kTileBlocks == 4 ? 6 : 5;        // a page of 2^kShift tokens holds whole tiles
+      int fetched = 0, pages[kTileBlocks];
       char *to = ring + lane * 16;
       const uint8_t *mine_at = nullptr;
       auto fetch = [&]() {
         if (fetched < count) {
-          const int at = begin + (warp + fetched * kAttnWarps) * kTileTokens;
+          const int at = begin + (warp + fetched * kAttnWarps) * kTileTokens, mask = (1 << k.c.page_shift) - 1;
           if (!(fetched & 31)) {
             const int lane_at = at + lane * kAttnWarps * kTileTokens;
-            if (lane_at < end) {
-              page0 = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, lane_at, k.status), 0);
-              mine_at = kv4_block(k.c, page0, head, lane_at & ((1 << k.c.page_shift) - 1));
+            pages[0] = 0;
+            if (lane_at < end) pages[0] = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, lane_at, k.status), 0);
+            mine_at = kv4_block(k.c, pages[0], head, lane_at & mask);
+            if (k.c.page_shift < kShift) {
+#pragma unroll
+              for (int b = 1; b < kTileBlocks; ++b) {
+                pages[b] = 0;
+                if (lane_at + b * kKv4Block < end)
+                  pages[b] =
+                      max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, lane_at + b * kKv4Block, k.status), 0);
+              }
             }
-            if (k.c.page_shift == 4 && lane_at + kKv4Block < end)
-              page1 = max(kv4_page(k.c, k.b.table, k.b.table_stride, seq, lane_at + kKv4Block, k.status), 0);
           }
           const uint8_t *src = reinterpret_cast<const uint8_t *>(
                                    __shfl_sync(0xffffffffu, reinterpret_cast<uintptr_t>(mine_at), fetched & 31)) +
                                lane * 16;
-          if (k.c.page_shift > 4 && at + kTileTokens <= end) {
+          if (k.c.page_shift >= kShift && at + kTileTokens <= end) {
             constexpr int kPieces = WEIGHTS ? kTileBlocks : 1, kBytes = WEIGHTS ? N : S::kStage;
 #pragma unroll
             for (int b = 0; b < kPieces; ++b)
@@ -595,14 +614,17 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
                 if (c + 512 <= kBytes || c + lane * 16 < kBytes)
                   copy16_async(to + b * S::kBlock + c, src + b * S::kBlock + c);
           } else {
-#pragma unroll 1
-            for (int b = 0; b < kTileBlocks && at + b * kKv4Block < end; ++b) {
-              if (b > 0)
-                src = k.c.page_shift > 4
-                          ? src + S::kBlock
-                          : kv4_block(k.c, __shfl_sync(0xffffffffu, page1, fetched & 31), head, 0) + lane * 16;
-#pragma unroll 1
-              for (int c = 0; c + lane * 16 < N; c += 512) copy16_async(to + b * S::kBlock + c, src + c);
+#pragma unroll
+            for (int b = 0; b < kTileBlocks; ++b) {
+              if (at + b * kKv4Block >= end) break;
+              const uint8_t *from = src + b * S::kBlock;
+              if (k.c.page_shift < kShift)
+                from = kv4_block(k.c, __shfl_sync(0xffffffffu, pages[b], fetched & 31), head,
+                                 (at + b * kKv4Block) & mask) +
+                       lane * 16;
+#pragma unroll
+              for (int c = 0; c < N; c += 512)
+                if (c + 512 <= N || c + lane * 16 < N) copy16_async(to + b * S::kBlock + c, from + c);
             }
           }
           to = to + S::kStage == ring + lane * 16 + kStages * S::kStage ? ring + lane * 16 : to + S::kStage;
@@ -663,7 +685,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
         __syncwarp();  // every lane's copies are there
         float p[kTileBlocks][NT][4];
-        tile_scores<D, NG, NT, QS>(buf, smem, p);
+#pragma unroll
+        for (int b = 0; b < kTileBlocks; b += 2) block_scores<D, NG, NT, QS>(buf + b * S::kBlock, smem, p + b);
         const bool whole = at + kTileTokens <= all_see;
         if (!whole) {
 #pragma unroll
@@ -711,10 +734,11 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT, QS)) kv4_att
               rise |= m[nt][e] > limit[nt][e];
             }
           if (!whole) {  // what stands behind the last token is not a scale
-            if (lane < kTileTokens && at + lane >= end)
-              for (int gr = 0; gr < NG; ++gr)
-                reinterpret_cast<__half *>(buf + (lane >> 4) * S::kBlock + S::kBlock / 2 + 8 * D)[(lane & 15) * NG + gr] =
-                    __ushort_as_half(0);
+            for (int x = lane; x < kTileTokens; x += 32)
+              if (at + x >= end)
+                for (int gr = 0; gr < NG; ++gr)
+                  reinterpret_cast<__half *>(buf + (x >> 4) * S::kBlock + S::kBlock / 2 + 8 * D)[(x & 15) * NG + gr] =
+                      __ushort_as_half(0);
             __syncwarp();
           }
           __half2 h[kTileBlocks][2][(NG + 1) / 2], big = __floats2half2_rn(0.0f, 0.0f);

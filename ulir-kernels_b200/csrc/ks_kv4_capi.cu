@@ -102,14 +102,16 @@ int rows_ok(const void *p, size_t tokens, size_t token_stride, size_t heads, siz
 // How the attention is cut.  Row tiles of 8 while the rows of a key/value head
 // fit, else 16; as many CTAs as the GPU holds at once, but no more than there
 // can be units of work.
-Kv4Plan plan_of(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_new, size_t max_len, int dtype) {
+Kv4Plan plan_of(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_new, size_t max_len) {
   Kv4Plan p;
   const size_t rows = max_new * group_heads;
-  p.rows_tile = rows <= 8 ? 8 : 16;
+  const int nt = rows <= 8 ? 1 : 2;
+  p.rows_tile = 8 * nt;
   p.row_tiles = (int)((rows + p.rows_tile - 1) / p.rows_tile);
-  const size_t units = n_seqs * v.kv_heads * p.row_tiles * ((max_len + kUnitTokens - 1) / kUnitTokens);
-  const size_t ctas = kPlanSms * kv4_ctas_per_sm(p.rows_tile / 8, dtype == KS_B200_DTYPE_F32 ? 2 : 1);
-  static_assert(kPlanSms * 4 <= kAttnCtas && 3 * kAttnCtas <= kAttnCounters, "three counters to a CTA");
+  p.unit = kv4_unit_tokens(nt, v.groups);
+  const size_t units = n_seqs * v.kv_heads * p.row_tiles * ((max_len + p.unit - 1) / p.unit);
+  const size_t ctas = kPlanSms * kv4_ctas_per_sm(nt);
+  static_assert(kPlanSms * kv4_ctas_per_sm(1) <= kAttnCtas && 3 * kAttnCtas <= kAttnCounters, "three counters to a CTA");
   p.ctas = (int)(units < ctas ? units : ctas);
   return p;
 }
@@ -118,12 +120,13 @@ bool attention_sizes_ok(const Kv4View &v, size_t q_heads, size_t n_seqs, size_t 
   return q_heads > 0 && q_heads % v.kv_heads == 0 && q_heads <= kMost && n_seqs > 0 && n_seqs <= 65535 && max_new > 0 &&
          max_len > 0 && max_new <= max_len && max_len <= kMaxLen && max_new <= kMost / q_heads &&
          // units of work, a row tile of at least 8 rows and 128 tokens each, are counted in 31 bits
-         n_seqs * v.kv_heads <= kMost / (max_new * (q_heads / v.kv_heads) / 8 + 1) / (max_len / kUnitTokens + 1 + kItemUnits);
+         n_seqs * v.kv_heads <=
+             kMost / (max_new * (q_heads / v.kv_heads) / 8 + 1) / (max_len / kv4_unit_tokens(2, 1) + 1 + kItemUnits);
 }
 
-// The counters, then two parts of every CTA: for any type (f16 and bf16 have the most CTAs).
+// The counters, then two parts of every CTA.
 size_t attention_bytes(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_new, size_t max_len) {
-  const Kv4Plan p = plan_of(v, group_heads, n_seqs, max_new, max_len, KS_B200_DTYPE_F16);
+  const Kv4Plan p = plan_of(v, group_heads, n_seqs, max_new, max_len);
   return 4 * (kAttnCounters + 2 * (size_t)p.ctas * p.rows_tile * (v.head_dim + 2));
 }
 
@@ -218,7 +221,7 @@ extern "C" int ks_b200_kv4_attention_async(const ks_b200_kv4_cache *cache, const
   if (!attention_sizes_ok(k.c, q_heads, n_seqs, max_new, (size_t)k.b.max_len))
     return fail(KS_ERR_UNSUPPORTED, "too many rows or tokens for one call");
   k.group_heads = (int)(q_heads / k.c.kv_heads);
-  k.p = plan_of(k.c, k.group_heads, n_seqs, max_new, (size_t)k.b.max_len, dtype);
+  k.p = plan_of(k.c, k.group_heads, n_seqs, max_new, (size_t)k.b.max_len);
   const size_t need = attention_bytes(k.c, k.group_heads, n_seqs, max_new, (size_t)k.b.max_len);
   if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
     return fail(KS_ERR_WORKSPACE, "workspace smaller than ks_b200_kv4_attention_workspace, or not 16-byte aligned");
