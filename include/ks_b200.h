@@ -639,8 +639,8 @@ int ks_b200_kv4_read_async(const ks_b200_kv4_cache *cache,
  * [n_tokens][q_heads], or NULL.  accumulate != 0 adds to cache->weights of
  * every cached token the attention weight it received, summed over the
  * sequence's new tokens and the query heads of its key/value head, in a fixed
- * order; then lse may not be NULL, and no page may belong to two sequences of
- * the call (without it, sequences may share pages).
+ * order; then lse may not be NULL, and no page may occur twice among the
+ * sequences of the call (without it, sequences may share pages).
  * max_new and max_len bound the new and the cached tokens of any sequence
  * (max_new <= max_len <= page_table_stride * page_size): they size the launch.
  * out may not overlap q.  workspace: device memory, 16-byte aligned,
@@ -679,7 +679,9 @@ int ks_b200_kv4_attention_async(const ks_b200_kv4_cache *cache,
  * free for other use afterwards.  kept: int32 [n_seqs][kv_heads][budget], or
  * NULL: the old position of each kept token; entries past a sequence's kept
  * tokens are left as they are.  max_len bounds the sequences' lengths.
- * workspace as for the attention.
+ * workspace: device memory, 16-byte aligned, ks_b200_kv4_evict_workspace(...)
+ * bytes, not shared by calls that may run at the same time.  Its first 8192
+ * bytes are left as they are, so that the attention's may serve, in turn.
  */
 size_t ks_b200_kv4_evict_workspace(const ks_b200_kv4_cache *cache, size_t n_seqs,
                                    size_t max_len, size_t budget);

@@ -765,3 +765,33 @@ def test_with_the_w4a8_products(ks, cuda, oracle):
         rc, want = oracle.matvec_w4a8_f16(qs, w[1], heads * d // 2, sw[1].view(np.uint16), heads * d // 32, hidden,
                                           heads * d, 32, float(scale))
         assert rc == 0 and O.w4a8_tolerance_ok(y[s].cpu().numpy(), want)[0]
+
+
+def test_one_workspace_for_attention_and_eviction_in_turn(ks, cuda):
+    """The eviction leaves the words alone that the attention wants to be 0, whatever they hold."""
+    import torch
+
+    c = Seqs(ks, cuda, [3000, 700], [1, 1], 2, 128, 32, 64, weights=True, seed=4)
+    q = _query(c, 8, "f32")
+    to_pool_pages = 2 * 32
+    n = c.n_pages + to_pool_pages
+    pool, w = torch.zeros((n, *c.pool.shape[1:]), dtype=torch.uint8, device=cuda), torch.zeros((n, 2, 64), device=cuda)
+    pool[: c.n_pages], w[: c.n_pages] = c.pool, c.w
+    cache = ks.Kv4Cache(pool, n, 64, 2, 128, 32, weights=w)
+    to_table = torch.arange(c.n_pages, n, dtype=torch.int32, device=cuda).reshape(2, 32)
+    to_lens = torch.zeros(2, dtype=torch.int32, device=cuda)
+    need = max(ks.kv4_attention_workspace(cache, 8, 2, 2, 1, 3000), ks.kv4_evict_workspace(cache, 2, 3000, 2000))
+    ws = torch.zeros(need, dtype=torch.uint8, device=cuda)
+    outs = []
+    for _ in range(2):
+        out, lse = torch.zeros_like(q), torch.zeros(2, 8, device=cuda)
+        ks.kv4_attention_async(cache, c.table, c.seq_lens, q, out, 0.1, ws, max_len=3000, lse=lse, status=c.status)
+        outs.append((out, lse))
+        ks.kv4_evict_async(cache, c.table, c.seq_lens, to_table, to_lens, 3000, 2000, 100, ws, status=c.status)
+        assert not ws[:8192].any()
+    ws[:8192] = 3
+    ks.kv4_evict_async(cache, c.table, c.seq_lens, to_table, to_lens, 3000, 2000, 100, ws, status=c.status)
+    c.ok()
+    assert (ws[:8192] == 3).all() and to_lens.tolist() == [2000, 700]
+    for out, lse in outs:
+        _check(c, q, 0.1, out, lse, "f32")

@@ -431,6 +431,7 @@ cudaError_t launch_rows(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, u
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectShared = 200 * 1024;  // keys that fit stay in shared memory
 
+// Behind the words that the attention wants to be 0, so that one workspace serves both in turn.
 struct EvictWorkspace {
   uint32_t *keys;  // [seq][head][max_len]
   int32_t *list;   // [seq][head][budget]
@@ -439,7 +440,7 @@ struct EvictWorkspace {
 
 __host__ __device__ inline EvictWorkspace evict_workspace(void *w, int64_t rows, int64_t max_len, int64_t budget) {
   EvictWorkspace e;
-  e.keys = static_cast<uint32_t *>(w);
+  e.keys = static_cast<uint32_t *>(w) + kKv4Counters;
   e.list = reinterpret_cast<int32_t *>(e.keys + rows * max_len);
   e.count = e.list + rows * budget;
   return e;
@@ -663,7 +664,7 @@ cudaError_t launch_kv4_read(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &
 
 size_t kv4_evict_workspace(const Kv4View &c, int n_seqs, int max_len, int budget) {
   const size_t rows = (size_t)n_seqs * c.kv_heads;
-  return (rows * ((size_t)max_len + budget) + n_seqs) * 4;
+  return (kKv4Counters + rows * ((size_t)max_len + budget) + n_seqs) * 4;
 }
 
 cudaError_t launch_kv4_evict(const Kv4View &c, const Kv4Batch &b, const Kv4Evict &e, uint32_t *status,

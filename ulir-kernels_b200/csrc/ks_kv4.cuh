@@ -30,6 +30,8 @@
 namespace ksb {
 
 constexpr int kKv4Block = 16;  // tokens
+// Words at the start of a workspace that are 0 between calls of the attention.
+constexpr int kKv4Counters = 2048;
 
 __host__ __device__ constexpr int kv4_half_block_bytes(int d, int groups) { return kKv4Block * (d / 2 + 2 * groups); }
 __host__ __device__ constexpr int kv4_block_bytes(int d, int groups) { return 2 * kv4_half_block_bytes(d, groups); }

@@ -81,10 +81,10 @@ __host__ __device__ constexpr int kv4_unit_tokens(int nt, int groups) {
   return kAttnWarps * kv4_tile_blocks(nt, groups) * kKv4Block;
 }
 constexpr int kJoin = 8;  // parts that are loaded together to be joined
-// Words at the start of the workspace, 0 between calls: three per CTA, of the
+// Of kKv4Counters at the start of the workspace a CTA has three, of the
 // item that begins in its stretch (finished groups of parts), of that item's
 // first group of parts and of a later group, which begins at this CTA.
-constexpr int kAttnCtas = 680, kAttnCounters = 2048;
+constexpr int kAttnCtas = 680;
 
 // How a call is cut: the same on the host, for the workspace, and in the kernel.
 struct Kv4Plan {
@@ -112,7 +112,7 @@ constexpr int kv4_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 // and sums; slot 0 of an item that an earlier CTA began, slot 1 of one that a
 // later CTA ends.
 __device__ __forceinline__ float *kv4_partial(const Kv4AttnArgs &k, int cta, int slot) {
-  return static_cast<float *>(k.a.workspace) + kAttnCounters +
+  return static_cast<float *>(k.a.workspace) + kKv4Counters +
          ((int64_t)cta * 2 + slot) * (k.p.rows_tile * (k.c.head_dim + 2));
 }
 

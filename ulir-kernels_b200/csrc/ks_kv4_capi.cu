@@ -111,7 +111,7 @@ Kv4Plan plan_of(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_
   p.unit = kv4_unit_tokens(nt, v.groups);
   const size_t units = n_seqs * v.kv_heads * p.row_tiles * ((max_len + p.unit - 1) / p.unit);
   const size_t ctas = kPlanSms * kv4_ctas_per_sm(nt);
-  static_assert(kPlanSms * kv4_ctas_per_sm(1) <= kAttnCtas && 3 * kAttnCtas <= kAttnCounters, "three counters to a CTA");
+  static_assert(kPlanSms * kv4_ctas_per_sm(1) <= kAttnCtas && 3 * kAttnCtas <= kKv4Counters, "three counters to a CTA");
   p.ctas = (int)(units < ctas ? units : ctas);
   return p;
 }
@@ -127,7 +127,7 @@ bool attention_sizes_ok(const Kv4View &v, size_t q_heads, size_t n_seqs, size_t 
 // The counters, then two parts of every CTA.
 size_t attention_bytes(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_new, size_t max_len) {
   const Kv4Plan p = plan_of(v, group_heads, n_seqs, max_new, max_len);
-  return 4 * (kAttnCounters + 2 * (size_t)p.ctas * p.rows_tile * (v.head_dim + 2));
+  return 4 * (kKv4Counters + 2 * (size_t)p.ctas * p.rows_tile * (v.head_dim + 2));
 }
 
 }  // namespace
