@@ -143,3 +143,32 @@ def test_oracle_quantize():
     assert s.tolist() == [[1.0, 65504.0]] and q[0, 0] == 7 and q[0, 1] == 2 and q[0, 40] == -8
     q, s = O.kv4_quantize(np.full((1, 32), 1e-30), 32)
     assert s[0, 0] == np.float16(2.0**-24) and (q == 0).all()
+
+
+def test_evict_workspace_lies_behind_the_attentions_counters(ks):
+    """One workspace may serve both in turn: the first 8192 bytes are not the eviction's."""
+    c = ks.Kv4Cache(1 << 12, 10, 64, 8, 128, 32)
+    assert ks.kv4_evict_workspace(c, 3, 1000, 100) >= 8192 + 3 * 8 * 1100 * 4
+
+
+def test_python_index_checks(ks):
+    """Tables, lengths and offsets that the library would read wrongly or past their ends."""
+    torch = pytest.importorskip("torch")
+    c = ks.Kv4Cache(16, 4, 16, 2, 64, 32, weights=4)
+    table, lens = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    k, ws = torch.zeros(2, 2, 64), torch.zeros(16, dtype=torch.uint8)
+    off = torch.arange(3, dtype=torch.int32)
+    kept = torch.zeros(2, 2, 8, dtype=torch.int64)
+    for bad in ((table.long(), lens, off), (table, lens.long(), off), (table, lens, off.long()), (table, lens, off[:2]),
+                (table[:1], lens, off), (table.t().contiguous().t(), lens, off),
+                (table, torch.zeros(4).int()[::2], off), (table.float(), lens, off)):
+        for call in (ks.kv4_append_async, ks.kv4_read_async):
+            with pytest.raises(ValueError):
+                call(c, bad[0], bad[1], k, k, token_offsets=bad[2])
+        with pytest.raises(ValueError):
+            ks.kv4_attention_async(c, bad[0], bad[1], k, k.clone(), 1.0, ws, token_offsets=bad[2])
+    with pytest.raises(ValueError):
+        ks.kv4_attention_async(c, table, lens, k, k.clone(), 1.0, ws, lse=torch.zeros(2, 2, dtype=torch.float64))
+    for bad in ((table.long(), lens, None), (table, lens.long(), None), (table, lens[:1], None), (table, lens, kept)):
+        with pytest.raises(ValueError):
+            ks.kv4_evict_async(c, table, lens, bad[0], bad[1], 64, 8, 4, ws, kept=bad[2])

@@ -406,9 +406,38 @@ class _Dtypes(dict):
 _DTYPES = _Dtypes()
 
 
+class _IsDtype(dict):
+    """Whether a torch dtype is the one of this name, looked up by name once."""
+
+    def __init__(self, name):
+        super().__init__()
+        self._name = name
+
+    def __missing__(self, dtype):
+        return self.setdefault(dtype, str(dtype) == self._name)
+
+
+_INT32, _FLOAT32 = _IsDtype("torch.int32"), _IsDtype("torch.float32")
+
+
 # The kv4 calls stand in a decode loop, so they take what they need from their tensors once and directly.
 def _at(t):
     return None if t is None else t.data_ptr()
+
+
+def _sequences(page_table, seq_lens, token_offsets=None):
+    """The table's row stride and the number of sequences, which table, lengths and offsets have to be for."""
+    n_seqs = seq_lens.numel()
+    stride, one = page_table.stride()
+    rows, columns = page_table.shape
+    if not _INT32[page_table.dtype] or rows < n_seqs or (one != 1 and columns > 1):
+        raise ValueError("a page table must be int32 [n_seqs, pages], its rows contiguous")
+    if not _INT32[seq_lens.dtype] or not seq_lens.is_contiguous():
+        raise ValueError("seq_lens must be contiguous int32 [n_seqs]")
+    if token_offsets is not None and (not _INT32[token_offsets.dtype] or token_offsets.numel() <= n_seqs or
+                                      not token_offsets.is_contiguous()):
+        raise ValueError("token_offsets must be contiguous int32 [n_seqs + 1]")
+    return stride, n_seqs
 
 
 class Kv4Cache(ctypes.Structure):
@@ -436,8 +465,9 @@ def _kv4_rows(call, cache, page_table, seq_lens, k, v, token_offsets, status, st
     shape = k.shape
     if k.dtype != v.dtype or shape != v.shape or shape[1:] != cache._row or k1 != 1 or v1 != 1:
         raise ValueError("k and v must be [n_tokens, kv_heads, head_dim] of one type, the last dimension contiguous")
-    rc = call(cache._address, page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(), _at(token_offsets),
-              seq_lens.numel(), shape[0], k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DTYPES[k.dtype], _at(status),
+    stride, n_seqs = _sequences(page_table, seq_lens, token_offsets)
+    rc = call(cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), n_seqs,
+              shape[0], k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DTYPES[k.dtype], _at(status),
               stream_handle(stream))
     if rc:
         check(rc)
@@ -467,12 +497,12 @@ def kv4_attention_async(cache, page_table, seq_lens, q, out, scale, workspace, t
     n_tokens, q_heads, head_dim = shape = q.shape
     if q.dtype != out.dtype or shape != out.shape or head_dim != cache._row[1] or q1 != 1 or o1 != 1:
         raise ValueError("q and out must be [n_tokens, q_heads, head_dim] of one type, the last dimension contiguous")
-    if lse is not None and (lse.shape != shape[:2] or not lse.is_contiguous()):
+    if lse is not None and (lse.shape != shape[:2] or not _FLOAT32[lse.dtype] or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous f32 [n_tokens, q_heads]")
-    stride = page_table.stride(0)
+    stride, n_seqs = _sequences(page_table, seq_lens, token_offsets)
     rc = lib().ks_b200_kv4_attention_async(
-        cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), seq_lens.numel(),
-        n_tokens, max_new, stride * cache.page_size if max_len is None else max_len, q.data_ptr(), qt, qh, q_heads,
+        cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), n_seqs, n_tokens,
+        max_new, stride * cache.page_size if max_len is None else max_len, q.data_ptr(), qt, qh, q_heads,
         scale, out.data_ptr(), ot, oh, _DTYPES[q.dtype], _at(lse), 1 if accumulate else 0, workspace.data_ptr(),
         workspace.numel(), _at(status), stream_handle(stream))
     if rc:
@@ -486,13 +516,18 @@ def kv4_evict_workspace(cache, n_seqs, max_len, budget) -> int:
 def kv4_evict_async(cache, page_table, seq_lens, to_table, to_lens, max_len, budget, recent, workspace, kept=None,
                     status=None, stream=None) -> None:
     """Keep the newest `recent` tokens of each sequence and head and the heaviest others, `budget` in all, in the
-    pages of to_table; kept: None or int32 [n_seqs, kv_heads, budget] for their old positions."""
-    n_seqs = seq_lens.numel()
-    if kept is not None and (kept.shape != (n_seqs, cache._row[0], budget) or not kept.is_contiguous()):
+    pages of to_table; kept: None or int32 [n_seqs, kv_heads, budget] for their old positions; workspace: a device
+    byte tensor, which may be the attention's."""
+    stride, n_seqs = _sequences(page_table, seq_lens)
+    to_stride, to_seqs = _sequences(to_table, to_lens)
+    if to_seqs != n_seqs:
+        raise ValueError("seq_lens and to_lens must be of one length")
+    if kept is not None and (kept.shape != (n_seqs, cache._row[0], budget) or not _INT32[kept.dtype] or
+                             not kept.is_contiguous()):
         raise ValueError("kept must be a contiguous int32 [n_seqs, kv_heads, budget]")
     rc = lib().ks_b200_kv4_evict_async(
-        cache._address, page_table.data_ptr(), page_table.stride(0), seq_lens.data_ptr(), n_seqs, max_len,
-        to_table.data_ptr(), to_table.stride(0), to_lens.data_ptr(), budget, recent, _at(kept), workspace.data_ptr(),
+        cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), n_seqs, max_len,
+        to_table.data_ptr(), to_stride, to_lens.data_ptr(), budget, recent, _at(kept), workspace.data_ptr(),
         workspace.numel(), _at(status), stream_handle(stream))
     if rc:
         check(rc)
