@@ -90,7 +90,6 @@ constexpr int kAttnCtas = 680;
 struct Kv4Plan {
   int rows_tile;  // 8 NT
   int row_tiles;  // tiles of a (sequence, key/value head), at most
-  int unit;       // tokens of a unit of work
   int ctas;
 };
 
@@ -346,14 +345,16 @@ __device__ __forceinline__ void block_scores(const char *buf, const char *smem, 
 // that it takes to finish one item and begin another.
 constexpr int kItemUnits = 3;
 
-template <bool WEIGHTS>
+// (R rows to a row tile, UNIT tokens to a unit: powers of two.)
+template <bool WEIGHTS, int R, int UNIT>
 struct Kv4Units {
-  int per, items;
+  int per, row_tiles, items;
   __device__ Kv4Units(const Kv4AttnArgs &k, const Kv4Seq &q) {
     const int rows = min(q.n_new, k.a.max_new) * k.group_heads;
     // the weights' pass takes all row tiles of a stretch of tokens together; without tokens it has nothing to do
-    items = rows == 0 ? 0 : k.c.kv_heads * (WEIGHTS ? 1 : (rows + k.p.rows_tile - 1) / k.p.rows_tile);
-    per = (q.len + k.p.unit - 1) / k.p.unit;
+    row_tiles = rows == 0 ? 0 : WEIGHTS ? 1 : (int)((unsigned)(rows + R - 1) / R);
+    items = k.c.kv_heads * row_tiles;
+    per = (int)((unsigned)(q.len + UNIT - 1) / UNIT);
     if (!WEIGHTS) per = max(per, 1);
   }
   __device__ int all() const { return (kItemUnits + per) * items; }
@@ -442,6 +443,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
   constexpr bool kWide = QS == 2;  // sums over tokens in f32 registers
   constexpr int R = 8 * NT, kStages = S::kStages, kTileBlocks = S::kTileBlocks, kTileTokens = kTileBlocks * kKv4Block;
   constexpr int kUnitTokens = kv4_unit_tokens(NT, NG);
+  using Units = Kv4Units<WEIGHTS, R, kUnitTokens>;
   extern __shared__ __align__(128) char smem[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   int *share = reinterpret_cast<int *>(smem + S::kShare);
@@ -455,7 +457,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
   if (k.b.n_seqs <= 32) {  // every warp by itself, a sequence to a lane
     int per = 1, items = 0;
     if (lane < k.b.n_seqs) {
-      const Kv4Units<WEIGHTS> u(k, kv4_seq(k.b, lane, k.status));
+      const Units u(k, kv4_seq(k.b, lane, k.status));
       per = u.per, items = u.items;
     }
     auto scan = [&](int v) {
@@ -510,7 +512,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
     }
   } else {
     int mine = 0, total = 0;
-    for (int s = tid; s < k.b.n_seqs; s += kAttnThreads) mine += Kv4Units<WEIGHTS>(k, kv4_seq(k.b, s, k.status)).all();
+    for (int s = tid; s < k.b.n_seqs; s += kAttnThreads) mine += Units(k, kv4_seq(k.b, s, k.status)).all();
     const int before = cta_scan(mine, &total, share);
     ctas = min((int)gridDim.x, total);
     if (cta >= ctas) return;
@@ -530,7 +532,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
       int passed = 0;
       for (int base = 0; base < k.b.n_seqs; base += kAttnThreads) {
         const int s = base + tid;
-        const int u = s < k.b.n_seqs ? Kv4Units<WEIGHTS>(k, kv4_seq(k.b, s, nullptr)).all() : 0;
+        const int u = s < k.b.n_seqs ? Units(k, kv4_seq(k.b, s, nullptr)).all() : 0;
         int some;
         const int at = passed + cta_scan(u, &some, share);
         if (first_unit >= passed + some) {
@@ -552,7 +554,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
 
   for (int unit = first_unit; unit < end_unit && seq < k.b.n_seqs;) {
     const Kv4Seq q = kv4_seq(k.b, seq, nullptr);
-    const Kv4Units<WEIGHTS> units(k, q);
+    const Units units(k, q);
     if (unit >= seq_unit + units.all()) {
       seq_unit += units.all();
       ++seq;
@@ -566,9 +568,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
     const int from = max(unit - item_unit - kItemUnits, 0), upto = min(end_unit - item_unit - kItemUnits, units.per);
     unit = upto > from ? item_unit + kItemUnits + upto : item_unit + with;
     if (upto <= from) continue;  // its work begins in the next stretch, or (weights of no tokens) it has none
-    const int row_tiles = WEIGHTS ? 1 : units.items / k.c.kv_heads;
-    const int head = item / row_tiles;
-    const int first_tile = WEIGHTS ? 0 : item % row_tiles;
+    const int head = units.row_tiles == 1 ? item : item / units.row_tiles;
+    const int first_tile = item - head * units.row_tiles;
     const int last_tile = WEIGHTS ? (rows - 1) / R : first_tile;
 
     for (int tile = first_tile; tile <= last_tile; ++tile) {
@@ -949,11 +950,11 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
           auto last_of = [&](uint32_t *counter, int of) {
             __syncthreads();
             if (tid == 0) {
-              __threadfence();  // with the barrier before it, for the whole CTA
-              const bool last = atomicAdd(counter, 1u) == (uint32_t)of - 1u;
+              uint32_t before;  // with the barriers around it, for the whole CTA
+              asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+              const bool last = before == (uint32_t)of - 1u;
               if (last) *counter = 0;
               share[0] = last;
-              __threadfence();
             }
             __syncthreads();
             return share[0] != 0;

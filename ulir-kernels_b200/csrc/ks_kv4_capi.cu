@@ -108,8 +108,8 @@ Kv4Plan plan_of(const Kv4View &v, size_t group_heads, size_t n_seqs, size_t max_
   const int nt = rows <= 8 ? 1 : 2;
   p.rows_tile = 8 * nt;
   p.row_tiles = (int)((rows + p.rows_tile - 1) / p.rows_tile);
-  p.unit = kv4_unit_tokens(nt, v.groups);
-  const size_t units = n_seqs * v.kv_heads * p.row_tiles * ((max_len + p.unit - 1) / p.unit);
+  const size_t unit = kv4_unit_tokens(nt, v.groups);
+  const size_t units = n_seqs * v.kv_heads * p.row_tiles * ((max_len + unit - 1) / unit);
   const size_t ctas = kPlanSms * kv4_ctas_per_sm(nt);
   static_assert(kPlanSms * kv4_ctas_per_sm(1) <= kAttnCtas && 3 * kAttnCtas <= kKv4Counters, "three counters to a CTA");
   p.ctas = (int)(units < ctas ? units : ctas);
