@@ -795,3 +795,76 @@ def test_one_workspace_for_attention_and_eviction_in_turn(ks, cuda):
     assert (ws[:8192] == 3).all() and to_lens.tolist() == [2000, 700]
     for out, lse in outs:
         _check(c, q, 0.1, out, lse, "f32")
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_overlapping_launches_give_the_same(ks, cuda, dtype):
+    """Steps that feed one another directly (append of what the attention gave, attention on its own result, eviction,
+    read), on the default stream, where no launch overlaps another, on a stream of their own and as a graph there: the
+    same bits."""
+    import torch
+
+    heads, q_heads, d, page, steps, n_seqs = 2, 8, 128, 64, 6, 3
+    start = [700, 1, 130]
+    pages = 16
+    results = []
+    side = torch.cuda.Stream()
+    for mode in ("default", "side", "graph"):
+        rng = torch.Generator(device=cuda).manual_seed(3)
+        pool = torch.zeros(2 * n_seqs * pages, ks.kv4_page_bytes(page, heads, d, 32), dtype=torch.uint8, device=cuda)
+        w = torch.zeros(2 * n_seqs * pages, heads, page, device=cuda)
+        cache = ks.Kv4Cache(pool, len(pool), page, heads, d, 32, weights=w)
+        table = torch.arange(n_seqs * pages, dtype=torch.int32, device=cuda).reshape(n_seqs, pages)
+        to_table = table + n_seqs * pages
+        status = torch.zeros(2, dtype=torch.int32, device=cuda)
+        first = np.concatenate([[0], np.cumsum(start)])
+        kv = torch.randn(2, first[-1], heads, d, generator=rng, device=cuda).to(_type(dtype))
+        offsets = torch.tensor(first, dtype=torch.int32, device=cuda)
+        lens = [torch.tensor([n + i for n in start], dtype=torch.int32, device=cuda) for i in range(steps + 1)]
+        x = torch.randn(n_seqs, q_heads, d, generator=rng, device=cuda).to(_type(dtype))
+        outs = [x] + [torch.zeros_like(x) for _ in range(steps)]
+        lse = torch.zeros(n_seqs, q_heads, device=cuda)
+        ws = torch.zeros(max(ks.kv4_attention_workspace(cache, q_heads, n_seqs, n_seqs, 1, 1024),
+                             ks.kv4_evict_workspace(cache, n_seqs, 1024, 100)), dtype=torch.uint8, device=cuda)
+        to_lens = torch.zeros(n_seqs, dtype=torch.int32, device=cuda)
+        back = torch.zeros(2, n_seqs * 100, heads, d, device=cuda, dtype=_type(dtype))
+        kept = [min(n + steps, 100) for n in start]
+        back_offsets = torch.tensor(np.concatenate([[0], np.cumsum(kept)]), dtype=torch.int32, device=cuda)
+
+        def chain(stream):
+            pool.zero_()
+            w.zero_()
+            ks.kv4_append_async(cache, table, lens[0], kv[0], kv[1], token_offsets=offsets, status=status,
+                                stream=stream)
+            for i in range(steps):
+                ks.kv4_append_async(cache, table, lens[i + 1], outs[i][:, ::4], outs[i][:, 1::4], status=status,
+                                    stream=stream)
+                ks.kv4_attention_async(cache, table, lens[i + 1], outs[i], outs[i + 1], 0.3, ws, max_len=1024, lse=lse,
+                                       accumulate=True, status=status, stream=stream)
+            ks.kv4_evict_async(cache, table, lens[steps], to_table, to_lens, 1024, 100, 10, ws, status=status,
+                               stream=stream)
+            ks.kv4_read_async(cache, to_table, to_lens, back[0], back[1], token_offsets=back_offsets, status=status,
+                              stream=stream)
+
+        torch.cuda.synchronize()
+        if mode == "default":
+            chain(None)
+        else:
+            with torch.cuda.stream(side):
+                chain(side)
+            side.synchronize()
+            if mode == "graph":
+                g = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(g, stream=side):
+                    chain(torch.cuda.current_stream())
+                for t in outs[1:] + [back, lse]:
+                    t.zero_()
+                for _ in range(3):
+                    g.replay()
+        torch.cuda.synchronize()
+        assert status.tolist() == [0, 0] and to_lens.tolist() == kept
+        results.append([t.clone() for t in outs[1:] + [back, lse, w, pool]])
+    assert results[0][-4].float().abs().sum() > 0 and results[0][-2].sum() > 0
+    for other in results[1:]:
+        for a, b in zip(results[0], other):
+            assert torch.equal(a, b)

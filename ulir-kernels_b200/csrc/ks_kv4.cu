@@ -376,6 +376,7 @@ __global__ void __launch_bounds__(kRowThreads, READ ? 4 : 3) kv4_rows_kernel(Kv4
                                                                               int cta_tokens, uint32_t *status) {
   __shared__ Kv4Place places[kRowTokens];
   const int first = blockIdx.x * cta_tokens, tokens = min(cta_tokens, b.n_tokens - first);
+  kv4_begin();
   find_places(c, b, first, tokens, places, status);
   if constexpr (READ) {
     if (blockIdx.y == 0)
@@ -398,13 +399,10 @@ cudaError_t launch_rows(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, u
   tokens = tokens < 1 ? 1 : tokens > kRowTokens ? kRowTokens : tokens;
   while (tokens > 1 && (b.n_tokens + tokens - 1) / tokens < 148) tokens /= 2;
   const dim3 grid((unsigned)((b.n_tokens + tokens - 1) / tokens), 2);
-  if (r.dtype == kF32)
-    kv4_rows_kernel<float, D, NG, READ><<<grid, kRowThreads, 0, stream>>>(c, b, r, tokens, status);
-  else if (r.dtype == kF16)
-    kv4_rows_kernel<__half, D, NG, READ><<<grid, kRowThreads, 0, stream>>>(c, b, r, tokens, status);
-  else
-    kv4_rows_kernel<__nv_bfloat16, D, NG, READ><<<grid, kRowThreads, 0, stream>>>(c, b, r, tokens, status);
-  return cudaGetLastError();
+  auto *kernel = r.dtype == kF32   ? kv4_rows_kernel<float, D, NG, READ>
+                 : r.dtype == kF16 ? kv4_rows_kernel<__half, D, NG, READ>
+                                   : kv4_rows_kernel<__nv_bfloat16, D, NG, READ>;
+  return kv4_launch(kernel, grid, kRowThreads, 0, stream, c, b, r, tokens, status);
 }
 
 template <bool READ>
@@ -482,6 +480,7 @@ __global__ void __launch_bounds__(kSelectThreads) kv4_select_kernel(Kv4View c, K
   __shared__ uint32_t hist[kBins], scan[32], found[2];
   extern __shared__ uint32_t shared_keys[];
   const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x;
+  kv4_begin();
   int len = b.lens[seq];
   if (len < 0 || len > b.max_len) {
     if (tid == 0) set_status(status, kStatusBadScale);
@@ -587,6 +586,7 @@ __global__ void __launch_bounds__(kMoveThreads) kv4_move_kernel(Kv4View c, Kv4Ba
   const int head = blockIdx.y, seq = blockIdx.z, tid = threadIdx.x, base = blockIdx.x * kMoveTokens;
   const EvictWorkspace ws =
       evict_workspace(e.workspace, (int64_t)b.n_seqs * c.kv_heads, b.max_len, e.budget);
+  kv4_begin();
   const int count = ws.count[seq];
   if (blockIdx.x == 0 && head == 0 && tid == 0) e.to_lens[seq] = count;
   if (base >= count) return;
@@ -679,19 +679,14 @@ cudaError_t launch_kv4_evict(const Kv4View &c, const Kv4Batch &b, const Kv4Evict
   }
   const int64_t bytes = (int64_t)b.max_len * 4;
   const dim3 rows((unsigned)c.kv_heads, (unsigned)b.n_seqs);
-  if (bytes <= kSelectShared)
-    kv4_select_kernel<true><<<rows, kSelectThreads, (size_t)bytes, stream>>>(c, b, e, status);
-  else
-    kv4_select_kernel<false><<<rows, kSelectThreads, 0, stream>>>(c, b, e, status);
-  cudaError_t err = cudaGetLastError();
+  const bool shared = bytes <= kSelectShared;
+  cudaError_t err = kv4_launch(shared ? kv4_select_kernel<true> : kv4_select_kernel<false>, rows, kSelectThreads,
+                               shared ? (size_t)bytes : 0, stream, c, b, e, status);
   if (err != cudaSuccess) return err;
   const int most = e.budget < b.max_len ? e.budget : b.max_len;
   const dim3 grid((unsigned)((most + kMoveTokens - 1) / kMoveTokens), (unsigned)c.kv_heads, (unsigned)b.n_seqs);
-  if (c.head_dim == 128)
-    kv4_move_kernel<128><<<grid, kMoveThreads, 0, stream>>>(c, b, e, status);
-  else
-    kv4_move_kernel<64><<<grid, kMoveThreads, 0, stream>>>(c, b, e, status);
-  return cudaGetLastError();
+  return kv4_launch(c.head_dim == 128 ? kv4_move_kernel<128> : kv4_move_kernel<64>, grid, kMoveThreads, 0, stream, c, b,
+                    e, status);
 }
 
 }  // namespace ksb

@@ -36,6 +36,33 @@ constexpr int kKv4Counters = 2048;
 __host__ __device__ constexpr int kv4_half_block_bytes(int d, int groups) { return kKv4Block * (d / 2 + 2 * groups); }
 __host__ __device__ constexpr int kv4_block_bytes(int d, int groups) { return 2 * kv4_half_block_bytes(d, groups); }
 
+// On streams where launches may overlap, every kernel of the cache waits for
+// the kernels before it before it touches memory, and lets the next one be set
+// up after that.
+__device__ __forceinline__ void kv4_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void kv4_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void kv4_begin() {
+  kv4_wait();
+  kv4_next();
+}
+
+template <typename... A, typename... B>
+cudaError_t kv4_launch(void (*kernel)(A...), dim3 grid, int threads, size_t shared, cudaStream_t stream, B... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  if (pdl_enabled(stream)) {
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, A(args)...);
+}
+
 // A sequence's part of the call: its cached tokens (the new ones among them),
 // its first row among the packed new tokens and how many it has.  A
 // descriptor that does not fit the call's buffers is reported in status word

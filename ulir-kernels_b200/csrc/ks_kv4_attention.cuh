@@ -454,6 +454,12 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
   // some three units' time between them.
   int ctas, first_unit, end_unit, each = 0, extra = 0, seq = k.b.n_seqs, seq_unit = 0, parts = 0, part = 0;
   const int cta = blockIdx.x;
+  // The weights' pass reads no more than the first pass did (which waited for what came before it) until it needs lse;
+  // every CTA waits once.
+  if (!WEIGHTS) kv4_wait();
+  auto end = [] {
+    if (WEIGHTS) kv4_wait();
+  };
   if (k.b.n_seqs <= 32) {  // every warp by itself, a sequence to a lane
     int per = 1, items = 0;
     if (lane < k.b.n_seqs) {
@@ -469,7 +475,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
       return v;
     };
     const int upto_units = scan((kItemUnits + per) * items), total = __shfl_sync(0xffffffffu, upto_units, 31);
-    if (total == 0) return;
+    if (total == 0) return end();
     int units = per * items;
 #pragma unroll
     for (int o = 1; o < 32; o *= 2) units += __shfl_xor_sync(0xffffffffu, units, o);
@@ -491,7 +497,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
       const int most = shortest + __ffs(fits) - 1, pieces = (per + most - 1) / most;
       const int upto = scan(items * pieces), before = upto - items * pieces;
       const unsigned here = __ballot_sync(0xffffffffu, cta >= before && cta < upto);
-      if (!here) return;
+      if (!here) return end();
       seq = __ffs(here) - 1;
       parts = __shfl_sync(0xffffffffu, pieces, seq);
       const int of = __shfl_sync(0xffffffffu, per, seq), at = cta - __shfl_sync(0xffffffffu, before, seq);
@@ -503,7 +509,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
       first_unit = seq_unit + item * (kItemUnits + of) + kItemUnits + short_part * part + min(part, longer);
       end_unit = first_unit + short_part + (part < longer);
     } else {
-      if (cta >= ctas) return;
+      if (cta >= ctas) return end();
       first_unit = each * cta + min(cta, extra);
       end_unit = first_unit + each + (cta < extra);
       const unsigned here = __ballot_sync(0xffffffffu, first_unit < upto_units);
@@ -515,7 +521,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
     for (int s = tid; s < k.b.n_seqs; s += kAttnThreads) mine += Units(k, kv4_seq(k.b, s, k.status)).all();
     const int before = cta_scan(mine, &total, share);
     ctas = min((int)gridDim.x, total);
-    if (cta >= ctas) return;
+    if (cta >= ctas) return end();
     each = total / ctas, extra = total - each * ctas;
     first_unit = each * cta + min(cta, extra);
     end_unit = first_unit + each + (cta < extra);
@@ -637,7 +643,10 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
       load_queries<T, D, NT>(k, q, head, row0, rows, queries);  // on their way while the pages are looked up
       for (int i = 0; i < kStages; ++i) fetch();
 
-      if (WEIGHTS) __syncthreads();  // the previous rows' fragments have been read
+      if (WEIGHTS) {
+        kv4_wait();
+        __syncthreads();  // the previous rows' fragments have been read
+      }
       place_queries<T, D, NG, NT, QS>(k, row0, rows, queries, smem);
       if (WEIGHTS && tid < R) {
         const int r = row0 + tid;
@@ -869,6 +878,9 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
         fetch();
       }
       if constexpr (!WEIGHTS) {
+        // The next kernel may be set up: not before, or its CTAs would take the places that the first CTAs to end leave,
+        // some SMs more of them than others.
+        if (unit >= end_unit) kv4_next();
         // join the warps: the ring is drained, each writes its part over it
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -996,6 +1008,7 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
       }
     }
   }
+  end();
 }
 
 template <typename T, int D, int NG, int NT, int QS, int PS, bool WEIGHTS>
@@ -1009,8 +1022,7 @@ cudaError_t launch_kv4_attention_pass(const Kv4AttnArgs &k, cudaStream_t stream,
     if (e != cudaSuccess) return e;
     ready.fetch_or(bit, std::memory_order_relaxed);
   }
-  f<<<(unsigned)k.p.ctas, kAttnThreads, bytes, stream>>>(k);
-  return cudaGetLastError();
+  return kv4_launch(f, dim3((unsigned)k.p.ctas), kAttnThreads, bytes, stream, k);
 }
 
 template <typename T, int D, int NG, int NT, int QS, int PS>
