@@ -11,8 +11,9 @@
 // (sequence, head, row tile, tokens) and every CTA of a grid that the GPU holds
 // at once takes an equal stretch of it, so that sequences of unequal lengths and
 // few long ones alike fill the GPU evenly.  An item's beginning counts as three units more,
-// about what it costs: 64 sequences of up to 8192 tokens, 8 heads, take 70 us,
-// 98 without.  (Where few items give each CTA about one, it gets a part of one
+// about what it costs: 64 sequences of up to 8192 tokens, 8 heads, take 67 us
+// (70 before joins were made shorter, and then 98 without).  (Where few items
+// give each CTA about one, it gets a part of one
 // item.)  Of an item (a row tile and all its tokens) that
 // a stretch ends within, each CTA leaves its part (maximum, sum, unnormalised
 // output, f32) in the workspace; the last of them to finish joins the parts in
@@ -46,11 +47,11 @@
 // fifth of the time (which is why these are the warp-wide products, whose A
 // operand is made in registers: a tensor-memory operand would have to be stored
 // there first, and the products are not what takes the time).  444 equal
-// items of 4096 tokens, 128 elements, bf16: 54 us, 4.4 TB/s of codes and
+// items of 4096 tokens, 128 elements, bf16: 54 us, 4.5 TB/s of codes and
 // scales with groups of 128, 61 us, 4.3 TB/s with groups of 32; f32 68 and 80 us,
 // 3.5 and 3.3 TB/s.  The copies without the products take 0.8 of the time.
 // A call's beginning (the lengths, the queries) and end (the four warps' sums,
-// the join of an item's parts) take 9 us together, which is what short calls
+// the join of an item's parts) take 8 us together, which is what short calls
 // take.
 //
 // Precision.  Codes are exact in f16.  For f32 tensors queries (scaled by a
@@ -73,8 +74,9 @@ namespace ksb {
 constexpr int kAttnWarps = 4, kAttnThreads = 32 * kAttnWarps;
 // Blocks of a warp's tile: four where two such tiles of every warp fit shared
 // memory and their scores the registers, for fewer waits and votes (64 sequences
-// of up to 8192 tokens, bf16, groups of 128: 70 us, 72 with two blocks and four
-// CTAs; a sequence of 131072: 40, 42; 8 of 2048 in pages of 32, f16: 21, 19.5).
+// of up to 8192 tokens, bf16, groups of 64: 70 us, 72 with two blocks and four
+// CTAs; a sequence of 131071: 40, 42; 8 of 2047 in pages of 32, f16: 21, 19.5, all
+// before the joins were made shorter).
 __host__ __device__ constexpr int kv4_tile_blocks(int nt, int groups) { return nt == 1 && groups <= 2 ? 4 : 2; }
 // Tokens of a unit of work.
 __host__ __device__ constexpr int kv4_unit_tokens(int nt, int groups) {
