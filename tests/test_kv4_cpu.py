@@ -172,3 +172,24 @@ def test_python_index_checks(ks):
     for bad in ((table.long(), lens, None), (table, lens.long(), None), (table, lens[:1], None), (table, lens, kept)):
         with pytest.raises(ValueError):
             ks.kv4_evict_async(c, table, lens, bad[0], bad[1], 64, 8, 4, ws, kept=bad[2])
+
+
+def test_python_cache_checks(ks):
+    """A pool or weights smaller than the pages they are said to be."""
+    torch = pytest.importorskip("torch")
+    need = 4 * ks.kv4_page_bytes(16, 2, 64, 32)
+    pool, w = torch.zeros(need, dtype=torch.uint8), torch.zeros(4, 2, 16)
+    ks.Kv4Cache(pool, 4, 16, 2, 64, 32, weights=w)
+    for bad in ((pool[1:], w), (torch.zeros(2 * need, dtype=torch.uint8)[::2], w), (pool, w[:3]), (pool, w.half())):
+        with pytest.raises(ValueError):
+            ks.Kv4Cache(bad[0], 4, 16, 2, 64, 32, weights=bad[1])
+
+
+def test_evict_sizes_beyond_64_bits(ks):
+    most = 2**31 - 1
+    c = ks.Kv4Cache(16, 1, 16, 65535, 64, 32, weights=4)
+    assert ks.kv4_evict_workspace(c, 65535, most, most) == 0
+    assert ks.kv4_evict_workspace(c, 1, most, most) > 65535 * 2 * most * 4
+    rc = ks.lib().ks_b200_kv4_evict_async(c._address, 16, most, 16, 65535, most, 16, most, 16, most, 0, None, 16,
+                                          2**64 - 1, None, None)
+    assert rc == ks.KS_ERR_UNSUPPORTED

@@ -248,13 +248,19 @@ extern "C" int ks_b200_kv4_attention_async(const ks_b200_kv4_cache *cache, const
   return e == cudaSuccess ? KS_OK : cuda_fail(e, "kernel launch");
 }
 
+// 0: more lists and weights than any memory holds, or than 64 bits count.
+static size_t evict_bytes(const Kv4View &v, size_t n_seqs, size_t max_len, size_t budget) {
+  if (n_seqs * v.kv_heads > ((size_t)1 << 58) / (max_len + budget)) return 0;
+  return kv4_evict_workspace(v, (int)n_seqs, (int)max_len, (int)budget);
+}
+
 extern "C" size_t ks_b200_kv4_evict_workspace(const ks_b200_kv4_cache *cache, size_t n_seqs, size_t max_len,
                                               size_t budget) {
   Kv4View v{};
   if (view_of(cache, &v) != KS_OK || n_seqs == 0 || n_seqs > 65535 || max_len == 0 || max_len > kMost || budget == 0 ||
       budget > kMost)
     return 0;
-  return kv4_evict_workspace(v, (int)n_seqs, (int)max_len, (int)budget);
+  return evict_bytes(v, n_seqs, max_len, budget);
 }
 
 extern "C" int ks_b200_kv4_evict_async(const ks_b200_kv4_cache *cache, const int32_t *page_table,
@@ -278,7 +284,8 @@ extern "C" int ks_b200_kv4_evict_async(const ks_b200_kv4_cache *cache, const int
   const size_t most = budget < (size_t)b.max_len ? budget : (size_t)b.max_len;
   if ((to_table_stride << v.page_shift) < most)
     return fail(KS_ERR_INVALID_ARG, "a row of to_table holds fewer tokens than may be kept");
-  const size_t need = kv4_evict_workspace(v, b.n_seqs, b.max_len, (int)budget);
+  const size_t need = evict_bytes(v, n_seqs, (size_t)b.max_len, budget);
+  if (need == 0) return fail(KS_ERR_UNSUPPORTED, "too many heads, tokens or kept tokens for one call");
   if (!workspace || misaligned(workspace, 16) || workspace_bytes < need)
     return fail(KS_ERR_WORKSPACE, "workspace smaller than ks_b200_kv4_evict_workspace, or not 16-byte aligned");
   const Kv4Evict e{to_table, (int64_t)to_table_stride, to_lens, kept, (int)budget, (int)recent, workspace};

@@ -426,7 +426,7 @@ def _at(t):
 
 
 def _sequences(page_table, seq_lens, token_offsets=None):
-    """The table's row stride and the number of sequences, which table, lengths and offsets have to be for."""
+    """The table's row stride and columns and the number of sequences, which table, lengths and offsets are for."""
     n_seqs = seq_lens.numel()
     stride, one = page_table.stride()
     rows, columns = page_table.shape
@@ -437,7 +437,7 @@ def _sequences(page_table, seq_lens, token_offsets=None):
     if token_offsets is not None and (not _INT32[token_offsets.dtype] or token_offsets.numel() <= n_seqs or
                                       not token_offsets.is_contiguous()):
         raise ValueError("token_offsets must be contiguous int32 [n_seqs + 1]")
-    return stride, n_seqs
+    return stride, n_seqs, columns
 
 
 class Kv4Cache(ctypes.Structure):
@@ -450,6 +450,12 @@ class Kv4Cache(ctypes.Structure):
 
     def __init__(self, pool, n_pages, page_size, kv_heads, head_dim, group_size, weights=None):
         super().__init__(addr(pool), addr(weights), n_pages, page_size, kv_heads, head_dim, group_size)
+        need = n_pages * kv4_page_bytes(page_size, kv_heads, head_dim, group_size)
+        if hasattr(pool, "numel") and (pool.numel() * pool.element_size() < need or not pool.is_contiguous()):
+            raise ValueError(f"a pool of {n_pages} such pages is {need} contiguous bytes")
+        if hasattr(weights, "numel") and (weights.numel() < n_pages * kv_heads * page_size or
+                                          not _FLOAT32[weights.dtype] or not weights.is_contiguous()):
+            raise ValueError("weights must be contiguous f32 [n_pages, kv_heads, page_size]")
         self._tensors = (pool, weights)
         self._row = (kv_heads, head_dim)
         self._address = ctypes.addressof(self)
@@ -465,7 +471,7 @@ def _kv4_rows(call, cache, page_table, seq_lens, k, v, token_offsets, status, st
     shape = k.shape
     if k.dtype != v.dtype or shape != v.shape or shape[1:] != cache._row or k1 != 1 or v1 != 1:
         raise ValueError("k and v must be [n_tokens, kv_heads, head_dim] of one type, the last dimension contiguous")
-    stride, n_seqs = _sequences(page_table, seq_lens, token_offsets)
+    stride, n_seqs, _ = _sequences(page_table, seq_lens, token_offsets)
     rc = call(cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), n_seqs,
               shape[0], k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DTYPES[k.dtype], _at(status),
               stream_handle(stream))
@@ -499,10 +505,10 @@ def kv4_attention_async(cache, page_table, seq_lens, q, out, scale, workspace, t
         raise ValueError("q and out must be [n_tokens, q_heads, head_dim] of one type, the last dimension contiguous")
     if lse is not None and (lse.shape != shape[:2] or not _FLOAT32[lse.dtype] or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous f32 [n_tokens, q_heads]")
-    stride, n_seqs = _sequences(page_table, seq_lens, token_offsets)
+    stride, n_seqs, columns = _sequences(page_table, seq_lens, token_offsets)
     rc = lib().ks_b200_kv4_attention_async(
         cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), n_seqs, n_tokens,
-        max_new, stride * cache.page_size if max_len is None else max_len, q.data_ptr(), qt, qh, q_heads,
+        max_new, columns * cache.page_size if max_len is None else max_len, q.data_ptr(), qt, qh, q_heads,
         scale, out.data_ptr(), ot, oh, _DTYPES[q.dtype], _at(lse), 1 if accumulate else 0, workspace.data_ptr(),
         workspace.numel(), _at(status), stream_handle(stream))
     if rc:
@@ -518,8 +524,8 @@ def kv4_evict_async(cache, page_table, seq_lens, to_table, to_lens, max_len, bud
     """Keep the newest `recent` tokens of each sequence and head and the heaviest others, `budget` in all, in the
     pages of to_table; kept: None or int32 [n_seqs, kv_heads, budget] for their old positions; workspace: a device
     byte tensor, which may be the attention's."""
-    stride, n_seqs = _sequences(page_table, seq_lens)
-    to_stride, to_seqs = _sequences(to_table, to_lens)
+    stride, n_seqs, _ = _sequences(page_table, seq_lens)
+    to_stride, to_seqs, _ = _sequences(to_table, to_lens)
     if to_seqs != n_seqs:
         raise ValueError("seq_lens and to_lens must be of one length")
     if kept is not None and (kept.shape != (n_seqs, cache._row[0], budget) or not _INT32[kept.dtype] or
