@@ -134,7 +134,7 @@ __device__ __forceinline__ float kv4_code(float v, float s) {
   return fminf(fmaxf(q, -8.0f), 7.0f);
 }
 
-constexpr int kRowThreads = 256, kRowTokens = 32;  // tokens of a CTA, at most
+constexpr int kRowThreads = 256, kRowTokens = 256;  // tokens of a CTA, at most
 
 struct Kv4Place {
   int page, slot;  // page -1: the row is left out
@@ -367,9 +367,10 @@ __device__ __forceinline__ void read_rows(const Kv4View &c, const Kv4Place *plac
 // One pass over what is read and written, with nothing shared between tokens:
 // four threads to a token's row, so that a warp's 16-byte pieces fill whole
 // sectors on both sides, keys and values in CTAs of their own.  19880 tokens,
-// 8 heads of 128, bf16, groups of 64: append 31 us (3.4 TB/s; the quantisation's
+// 8 heads of 128, bf16, groups of 64: append 30 us (3.4 TB/s; the quantisation's
 // instructions bound it: quotients by a reciprocal, with one branch on
-// alignment to a row, took 8 us off), read 23 us (4.4 TB/s); 65536 tokens, f16: read 61 us, 5.6 TB/s.
+// alignment to a row, took 8 us off), read 21 us (4.9 TB/s); 58000 tokens, f16:
+// read 57 us, 5.3 TB/s.
 // 64 tokens take 4 us, the latency of the lookup and of one row.
 template <typename T, int D, int NG, bool READ>
 __global__ void __launch_bounds__(kRowThreads, READ ? 4 : 3) kv4_rows_kernel(Kv4View c, Kv4Batch b, Kv4Rows r,
@@ -391,12 +392,19 @@ __global__ void __launch_bounds__(kRowThreads, READ ? 4 : 3) kv4_rows_kernel(Kv4
   }
 }
 
-// Tokens of a CTA: enough for its threads (four to a head) four times over,
-// fewer where that would leave SMs without a CTA.
+// Tokens of a CTA: what gives all that the GPU holds at once the same number, so
+// that the lookup is done once (19880 tokens: append 29.7 us, read 20.7; with
+// CTAs of 32 tokens, one after the other, 30.2 and 22.9; 58000 tokens: read 57
+// and 61), in whole turns of its threads (four to a head); fewer where that
+// would leave SMs without a CTA.
 template <bool READ, int D, int NG>
 cudaError_t launch_rows(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, uint32_t *status, cudaStream_t stream) {
-  int tokens = 4 * kRowThreads / 4 / c.kv_heads;
-  tokens = tokens < 1 ? 1 : tokens > kRowTokens ? kRowTokens : tokens;
+  constexpr int kSlots = 148 * (READ ? 4 : 3) / 2;  // of keys, and of values
+  const int turn = c.kv_heads < kRowThreads / 4 ? kRowThreads / 4 / c.kv_heads : 1;
+  const int waves = (b.n_tokens - 1) / (kSlots * kRowTokens) + 1;
+  int tokens = (b.n_tokens - 1) / (kSlots * waves) + 1;
+  tokens = (tokens + turn - 1) / turn * turn;
+  tokens = tokens > kRowTokens ? kRowTokens : tokens;
   while (tokens > 1 && (b.n_tokens + tokens - 1) / tokens < 148) tokens /= 2;
   const dim3 grid((unsigned)((b.n_tokens + tokens - 1) / tokens), 2);
   auto *kernel = r.dtype == kF32   ? kv4_rows_kernel<float, D, NG, READ>
@@ -425,7 +433,7 @@ cudaError_t launch_rows(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, u
 // writes only the workspace, so to_lens may be the sequences' own lengths.
 // 32 sequences of up to 8192 tokens to 2048, 8 heads of 128, groups of 64: 45
 // us, 17 of them the search (each CTA's passes follow one another: latency) and
-// 28 the move (147 MB, 5.2 TB/s).  One sequence of 1100: 10 us, latency.
+// 28 the move (130 MB, 4.7 TB/s).  One sequence of 1100: 10 us, latency.
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectShared = 200 * 1024;  // keys that fit stay in shared memory
 
