@@ -868,3 +868,27 @@ def test_overlapping_launches_give_the_same(ks, cuda, dtype):
     for other in results[1:]:
         for a, b in zip(results[0], other):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("tokens,heads", [(80000, 1), (60001, 2), (9473, 3)])
+def test_append_and_read_more_tokens_than_the_gpu_holds_at_once(ks, cuda, tokens, heads):
+    """CTAs of many tokens, in one wave or several, the last one short."""
+    import torch
+
+    d, group, page = 64, 32, 256
+    pages = -(-tokens // page)
+    pool = torch.zeros(pages, ks.kv4_page_bytes(page, heads, d, group), dtype=torch.uint8, device=cuda)
+    cache = ks.Kv4Cache(pool, pages, page, heads, d, group)
+    table = torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=cuda)[None]
+    lens = torch.tensor([tokens], dtype=torch.int32, device=cuda)
+    offsets = torch.tensor([0, tokens], dtype=torch.int32, device=cuda)
+    kv = torch.randn(2, tokens, heads, d, generator=torch.Generator(device=cuda).manual_seed(5), device=cuda)
+    back = torch.full_like(kv, float("nan"))
+    status = torch.zeros(2, dtype=torch.int32, device=cuda)
+    ks.kv4_append_async(cache, table, lens, kv[0], kv[1], token_offsets=offsets, status=status)
+    ks.kv4_read_async(cache, table, lens, back[0], back[1], token_offsets=offsets, status=status)
+    torch.cuda.synchronize()
+    assert status.tolist() == [0, 0]
+    q, s = O.kv4_quantize(kv.double().cpu().numpy().reshape(-1, d), group)
+    want = q.reshape(-1, d // group, group) * s.reshape(-1, d // group, 1).astype(np.float64)
+    assert (back.double().cpu().numpy().reshape(want.shape) == want).all()
