@@ -892,3 +892,54 @@ def test_append_and_read_more_tokens_than_the_gpu_holds_at_once(ks, cuda, tokens
     q, s = O.kv4_quantize(kv.double().cpu().numpy().reshape(-1, d), group)
     want = q.reshape(-1, d // group, group) * s.reshape(-1, d // group, 1).astype(np.float64)
     assert (back.double().cpu().numpy().reshape(want.shape) == want).all()
+
+
+def test_captured_over_two_streams(ks, cuda):
+    """Calls after a join of streams, and after copies and fills, in a graph: launches that may overlap what is before
+    them in one stream still come after all of it."""
+    import torch
+
+    c = Seqs(ks, cuda, [900, 333], [1, 1], 2, 128, 32, 64, weights=True, seed=8)
+    q = _query(c, 8, "f32")
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    k, v = torch.randn(2, 2, 2, 128, device=cuda)
+    want_cache, want_w = c.pool.clone(), c.w.clone()
+    ws = [torch.zeros(ks.kv4_attention_workspace(c.cache, 8, 2, 2, 1, 1024), dtype=torch.uint8, device=cuda)
+          for _ in range(2)]
+    out = [torch.zeros_like(q) for _ in range(2)]
+    lse = [torch.zeros(2, 8, device=cuda) for _ in range(2)]
+    back = torch.zeros(2, 2, 2, 128, device=cuda)
+    qa, ka = torch.zeros_like(q), torch.zeros_like(k)
+
+    def both(first, second):
+        qa.copy_(q)
+        ka.copy_(k)
+        ks.kv4_append_async(c.cache, c.table, c.seq_lens, ka, v, status=c.status, stream=first)
+        second.wait_stream(first)
+        with torch.cuda.stream(second):
+            ks.kv4_attention_async(c.cache, c.table, c.seq_lens, qa, out[1], 0.2, ws[1], max_len=1024, lse=lse[1],
+                                   status=c.status, stream=second)
+        ks.kv4_read_async(c.cache, c.table, c.seq_lens, back[0], back[1], status=c.status, stream=first)
+        first.wait_stream(second)
+        ks.kv4_attention_async(c.cache, c.table, c.seq_lens, out[1], out[0], 0.2, ws[0], max_len=1024, lse=lse[0],
+                               accumulate=True, status=c.status, stream=first)
+        qa.zero_()
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(a):
+        both(a, b)
+    torch.cuda.synchronize()
+    wants = [t.clone() for t in (*out, *lse, back, c.pool, c.w)]
+    assert wants[0].abs().sum() > 0 and not torch.equal(wants[6], want_w)
+    g = torch.cuda.CUDAGraph()
+    c.pool.copy_(want_cache)
+    with torch.cuda.graph(g, stream=a):
+        c.w.copy_(want_w)
+        both(torch.cuda.current_stream(), b)
+    for t in (*out, *lse, back):
+        t.zero_()
+    for _ in range(4):
+        g.replay()
+    c.ok()
+    for got, want in zip((*out, *lse, back, c.pool, c.w), wants):
+        assert torch.equal(got, want)
