@@ -943,3 +943,47 @@ def test_captured_over_two_streams(ks, cuda):
     c.ok()
     for got, want in zip((*out, *lse, back, c.pool, c.w), wants):
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype,d,q_heads,n", [("f16", 64, 1, 524288), ("f16", 128, 12, 262144), ("bf16", 64, 4, 262144)])
+def test_long_items_whole_in_a_cta(ks, cuda, dtype, d, q_heads, n):
+    """As many sequences as there are CTAs (more than there are with 16 rows), on the same pages, each of them long, with
+    values of one sign and a late rise of the scores: sums over many tiles of one CTA.
+
+    Bound.  Truncating steps of the accumulators, each up to 2^-23 of the sum, go on for 128 products:
+    2^-16.  The f32 sums over a warp's (at most 128) such stretches and 4 warps: 2^-17.  Exponentials and the two parts of
+    the weights (2^-18), their sum and the division (2^-20): 2^-15 in all, 2^-11 more in one f16 part (bf16).  The scores
+    (at most about 2^5, over 2^4 products of 2^-23 or less) move all the weights of a row by 2^-16 at most.  Values are
+    positive, so all of this is relative to the result, which is then rounded once."""
+    import torch
+
+    T, page, seqs = _type(dtype), 256, 444
+    pages = n // page
+    pool = torch.zeros(pages, ks.kv4_page_bytes(page, 1, d, 64), dtype=torch.uint8, device=cuda)
+    cache = ks.Kv4Cache(pool, pages, page, 1, d, 64)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda).repeat(seqs, 1)
+    lens = torch.full((seqs,), n, dtype=torch.int32, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    q = torch.randn(1, q_heads, d, generator=gen, device=cuda)
+    k = torch.randn(n, 1, d, generator=gen, device=cuda) * 0.1
+    k[n // 2:] += 6.0 / 0.125 * q.mean(1) / (q.mean(1) ** 2).sum()  # the mean query's scores by 6
+    v = torch.rand(n, 1, d, generator=gen, device=cuda) + 1.0
+    q = q.to(T)
+    offsets = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+    status = torch.zeros(2, dtype=torch.int32, device=cuda)
+    ks.kv4_append_async(cache, table[:1], lens[:1], k, v, token_offsets=offsets, status=status)
+    ks.kv4_read_async(cache, table[:1], lens[:1], k, v, token_offsets=offsets, status=status)
+    out = torch.zeros(seqs, q_heads, d, dtype=T, device=cuda)
+    lse = torch.zeros(seqs, q_heads, device=cuda)
+    ws = torch.zeros(ks.kv4_attention_workspace(cache, q_heads, seqs, seqs, 1, n), dtype=torch.uint8, device=cuda)
+    ks.kv4_attention_async(cache, table, lens, q.expand(seqs, q_heads, d), out, 0.125, ws, max_len=n, lse=lse,
+                           status=status)
+    torch.cuda.synchronize()
+    assert status.tolist() == [0, 0]
+    x = q[0].double() @ k[:, 0].double().T * 0.125
+    want, z = torch.softmax(x, -1) @ v[:, 0].double(), torch.logsumexp(x, -1)
+    assert x.abs().max() < 40
+    rel = torch.finfo(T).eps / 2 + 2.0**-15 + 2.0**-16 + (2.0**-11 if dtype == "bf16" else 0)
+    worst = max(float(((o.double() - want) / want).abs().max()) for o in out)
+    assert worst <= rel, worst
+    assert ((lse.double() - z).abs() <= 2.0**-16 + 2.0**-22 * z.abs()).all()

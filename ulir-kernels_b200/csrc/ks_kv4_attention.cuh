@@ -60,9 +60,13 @@
 // few steps would cost two bits: so the queries' first parts are integers up to
 // 2^11, whose sums of up to 128 products stay below 2^24 and are exact, the
 // second parts have accumulators of their own, and sums over tokens leave the
-// accumulators after 32 tokens and go on in f32 registers.  f16 and bf16
-// queries fit one part, and for bf16 results one part of the probabilities (11
-// bits) is well below the result's own rounding.
+// accumulators after a tile and go on in f32 registers.  f16 and bf16 queries
+// fit one part, and for bf16 results one part of the probabilities (11 bits) is
+// an eighth of the result's own rounding.  Their sums over tokens stay in the
+// accumulators for 128 products, a loss of at most 2^-16, and are then added up
+// in f32 (kept for a whole item of 524288 tokens, they lost 7e-4, more than half
+// a step of f16; adding up after every tile, as for f32, takes 6 % more time at
+// 64 sequences of up to 8192, this 1 %).
 #pragma once
 
 #include <atomic>
@@ -82,6 +86,8 @@ __host__ __device__ constexpr int kv4_tile_blocks(int nt, int groups) { return n
 __host__ __device__ constexpr int kv4_unit_tokens(int nt, int groups) {
   return kAttnWarps * kv4_tile_blocks(nt, groups) * kKv4Block;
 }
+// Products after which sums over tokens leave the accumulators (f16 and bf16; each may cost 2^-23 of the sum).
+constexpr int kFoldProducts = 128;
 constexpr int kJoin = 8;  // parts that are loaded together to be joined
 // Of kKv4Counters at the start of the workspace a CTA has three, of the
 // item that begins in its stretch (finished groups of parts), of that item's
@@ -444,6 +450,8 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
   using S = Kv4Smem<D, NG, NT, QS>;
   constexpr bool kWide = QS == 2;  // sums over tokens in f32 registers
   constexpr int R = 8 * NT, kStages = S::kStages, kTileBlocks = S::kTileBlocks, kTileTokens = kTileBlocks * kKv4Block;
+  constexpr bool kFold = !kWide && !WEIGHTS;  // or there after every kFoldTiles tiles
+  constexpr int kFoldTiles = kFoldProducts / (kTileBlocks * PS);
   constexpr int kUnitTokens = kv4_unit_tokens(NT, NG);
   using Units = Kv4Units<WEIGHTS, R, kUnitTokens>;
   extern __shared__ __align__(128) char smem[];
@@ -691,7 +699,34 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
       float lift = 0.0f;
       __half2 scale_limit = __floats2half2_rn(0.0f, 0.0f);  // value scales up to this one fit
 
-      for (int i = 0, stage_out = 0; i < count; ++i, stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1) {
+      // A turn's sums (f16, bf16), added to those of the turns before it, which are in units of 2^folded_base (volatile: in
+      // local memory, the registers are taken); unfold brings them to units of 2^base, which has only risen.
+      [[maybe_unused]] volatile float folded[kFold ? NT : 1][kFold ? D / 16 : 1][4], folded_base[kFold ? NT : 1][2];
+      [[maybe_unused]] auto unfold = [&](int nt, int e) { return fast_exp2(folded_base[nt][e] - base[nt][e]); };
+      auto fold = [&](int i) {
+        if constexpr (kFold) {
+          if (i == count) return;
+          const bool first = i == kFoldTiles;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float f = first ? 0.0f : unfold(nt, e);
+              folded_base[nt][e] = top[nt][e] == -INFINITY ? -INFINITY : base[nt][e];
+#pragma unroll
+              for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+                for (int h = e; h < 4; h += 2) {
+                  folded[nt][m][h] = first ? o[nt][m][h] : fmaf(folded[nt][m][h], f, o[nt][m][h]);
+                  o[nt][m][h] = 0.0f;
+                }
+            }
+        }
+      };
+
+      for (int i = 0, stage_out = 0; i < count; fold(i))  // turns, and tiles of a turn
+      for (const int turn = kFold ? min(i + kFoldTiles, count) : count; i < turn;
+           ++i, stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1) {
         const int at = begin + (warp + i * kAttnWarps) * kTileTokens;
         char *buf = ring + stage_out * S::kStage;
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
@@ -883,6 +918,19 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
         // The next kernel may be set up: not before, or its CTAs would take the places that the first CTAs to end leave,
         // some SMs more of them than others.
         if (unit >= end_unit) kv4_next();
+        if constexpr (kFold) {
+          if (count > kFoldTiles)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float f = unfold(nt, e);
+#pragma unroll
+                for (int m = 0; m < D / 16; ++m)
+#pragma unroll
+                  for (int h = e; h < 4; h += 2) o[nt][m][h] = fmaf(folded[nt][m][h], f, o[nt][m][h]);
+              }
+        }
         // join the warps: the ring is drained, each writes its part over it
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
