@@ -572,9 +572,12 @@ int ks_b200_import_ggml_q4_0_async(const void *blocks, size_t block_row_stride,
  * of the packed [n_tokens] tensors of keys, values, queries and outputs, in
  * order (token_offsets NULL: one row each, row s).  page_table, seq_lens and
  * token_offsets are int32 device memory, read when the call runs, so a
- * captured graph follows them.  Table entries past a sequence's tokens are not
- * read.  Rows below token_offsets[0] or from token_offsets[n_seqs] on are left
- * as they are.  Tensors are [n_tokens][heads][head_dim] with strides in
+ * captured graph follows them.  A row of the table holds page_table_stride
+ * entries (where it is part of a wider one, max_len, and of to_table the
+ * smaller of max_len and budget, bounds what is read of it).
+ * Table entries past a sequence's tokens are not read.  Rows below
+ * token_offsets[0] or from token_offsets[n_seqs] on are left as they are.
+ * Tensors are [n_tokens][heads][head_dim] with strides in
  * elements, the last dimension contiguous, of type KS_B200_DTYPE_*.
  *
  * Device pointers, queued on `stream`, no allocation, capturable.  status
@@ -627,6 +630,28 @@ int ks_b200_kv4_read_async(const ks_b200_kv4_cache *cache,
                            size_t k_token_stride, size_t k_head_stride, void *v,
                            size_t v_token_stride, size_t v_head_stride,
                            int dtype, uint32_t *status, void *stream);
+
+/*
+ * As ks_b200_kv4_append_async and ks_b200_kv4_read_async, with max_len, a bound
+ * of the sequences' cached tokens (0 < max_len <= page_table_stride *
+ * page_size; a longer sequence is reported): for a table whose rows are part of
+ * wider ones, so that the entries behind a row's part are never read.
+ */
+int ks_b200_kv4_append_bounded_async(const ks_b200_kv4_cache *cache,
+                                     const int32_t *page_table, size_t page_table_stride,
+                                     const int32_t *seq_lens, const int32_t *token_offsets,
+                                     size_t n_seqs, size_t n_tokens, size_t max_len,
+                                     const void *k, size_t k_token_stride,
+                                     size_t k_head_stride, const void *v,
+                                     size_t v_token_stride, size_t v_head_stride,
+                                     int dtype, uint32_t *status, void *stream);
+int ks_b200_kv4_read_bounded_async(const ks_b200_kv4_cache *cache,
+                                   const int32_t *page_table, size_t page_table_stride,
+                                   const int32_t *seq_lens, const int32_t *token_offsets,
+                                   size_t n_seqs, size_t n_tokens, size_t max_len,
+                                   void *k, size_t k_token_stride, size_t k_head_stride,
+                                   void *v, size_t v_token_stride, size_t v_head_stride,
+                                   int dtype, uint32_t *status, void *stream);
 
 /*
  * Attention of the newest tokens over the cache, causal among them: with n

@@ -987,3 +987,65 @@ def test_long_items_whole_in_a_cta(ks, cuda, dtype, d, q_heads, n):
     worst = max(float(((o.double() - want) / want).abs().max()) for o in out)
     assert worst <= rel, worst
     assert ((lse.double() - z).abs() <= 2.0**-16 + 2.0**-22 * z.abs()).all()
+
+
+@pytest.mark.parametrize("part", ["first", "last", "middle"])
+def test_tables_that_are_columns_of_wider_ones(ks, cuda, part):
+    """The same as with tables of their own; a sequence longer than the columns hold is reported, and the pages that the
+    columns beside them name are neither read nor written."""
+    import torch
+
+    c = Seqs(ks, cuda, [100, 40], [1, 1], 2, 64, 32, 16, weights=True, spare=30)
+    columns, to_columns, budget = c.table.shape[1], 2, 32
+    at = {"first": 0, "last": 12, "middle": 5}[part]
+    others = np.setdiff1d(np.arange(c.n_pages), np.concatenate(c.pages))
+    to_pages = others[:4].reshape(2, 2)
+    beside = torch.from_numpy(others[4:24].astype(np.int32)).to(cuda)
+
+    def wide(table):  # columns of a wider one, which for the last rows ends the storage
+        n = table.shape[1]
+        big = beside.repeat(2)[: 2 * 20].reshape(2, 20).clone()[:, : at + n if part == "last" else 20].contiguous()
+        big[:, at:at + n] = table
+        return big[:, at:at + n]
+
+    own = c.table.clone()
+    to_own = torch.from_numpy(to_pages.astype(np.int32)).to(cuda)
+    q = _query(c, 4, "f32")
+    x = torch.randn(2, 2, 2, 64, device=cuda)
+    start, wstart = c.pool.clone(), c.w.clone()
+    results = []
+    for table, to_table in ((own, to_own), (wide(own), wide(to_own))):
+        c.pool.copy_(start)
+        c.w.copy_(wstart)
+        c.table = table
+        ks.kv4_append_async(c.cache, table, c.seq_lens, x[0], x[1], status=c.status)
+        back = torch.zeros_like(x)
+        ks.kv4_read_async(c.cache, table, c.seq_lens, back[0], back[1], status=c.status)
+        out, lse = _attend(c, q, 0.1, accumulate=True, max_len=16 * columns)
+        to_lens = torch.zeros(2, dtype=torch.int32, device=cuda)
+        ws = torch.zeros(ks.kv4_evict_workspace(c.cache, 2, 100, budget), dtype=torch.uint8, device=cuda)
+        ks.kv4_evict_async(c.cache, table, c.seq_lens, to_table, to_lens, 100, budget, 8, ws, status=c.status)
+        c.ok()
+        results.append((back, out, lse, to_lens, c.pool.clone(), c.w.clone()))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    # the last row's sequence one page longer than its columns
+    before, wbefore = c.pool.clone(), c.w.clone()
+    long = torch.tensor([100, 16 * columns + 5], dtype=torch.int32, device=cuda)
+    ks.kv4_append_async(c.cache, c.table, long, x[0], x[1], status=c.status)
+    torch.cuda.synchronize()
+    assert c.status.tolist() == [1, 0]
+    changed = (c.pool != before).flatten(1).any(1) | (c.w != wbefore).flatten(1).any(1)
+    assert set(changed.nonzero().flatten().tolist()) <= set(c.pages[0].tolist())
+    c.status.zero_()
+    back = torch.full_like(x, 7)
+    ks.kv4_read_async(c.cache, c.table, long, back[0], back[1], status=c.status)
+    torch.cuda.synchronize()
+    assert c.status.tolist() == [1, 0] and (back[:, 1] == 7).all() and not (back[:, 0] == 7).any()
+    # one sequence, whose table of one row has no distance to a next one
+    column = torch.from_numpy(c.pages[0].astype(np.int32)).to(cuda)[:, None]
+    c.status.zero_()
+    back = torch.zeros(2, 1, 2, 64, device=cuda)
+    ks.kv4_read_async(c.cache, column.t(), c.seq_lens[:1], back[0], back[1], status=c.status)
+    c.ok()
+    assert torch.equal(back[:, 0], results[0][0][:, 0])

@@ -193,3 +193,46 @@ def test_evict_sizes_beyond_64_bits(ks):
     rc = ks.lib().ks_b200_kv4_evict_async(c._address, 16, most, 16, 65535, most, 16, most, 16, most, 0, None, 16,
                                           2**64 - 1, None, None)
     assert rc == ks.KS_ERR_UNSUPPORTED
+
+
+def test_python_tables_that_are_columns_of_wider_ones(ks):
+    """What a row of a table holds are its columns, not the distance to the next row."""
+    torch = pytest.importorskip("torch")
+    c = ks.Kv4Cache(1 << 12, 40, 16, 2, 64, 32, weights=1 << 12)
+    big, lens = torch.zeros(2, 10, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    x, ws = torch.zeros(2, 2, 64), torch.zeros(1 << 16, dtype=torch.uint8)
+
+    def refused(call, *args, **kwargs):
+        with pytest.raises(ks.KernelSmithError) as e:
+            call(*args, **kwargs)
+        assert e.value.rc == ks.KS_ERR_INVALID_ARG, e.value
+
+    for table in (big[:, :2], big[:, 8:], big[:, 4:6]):
+        refused(ks.kv4_attention_async, c, table, lens, x, x.clone(), 1.0, ws, max_len=33)
+        refused(ks.kv4_evict_async, c, table, lens, big, lens, 33, 40, 8, ws)
+        refused(ks.kv4_evict_async, c, big, lens, table, lens, 100, 40, 8, ws)  # 40 tokens are three pages
+        refused(ks.kv4_evict_async, c, big, lens, table, lens, 33, 40, 8, ws)
+    # rows that lie over each other, and a table without columns
+    over = torch.zeros(20, dtype=torch.int32).as_strided((2, 10), (4, 1))
+    for call in (ks.kv4_append_async, ks.kv4_read_async):
+        with pytest.raises(ValueError):
+            call(c, over, lens, x, x.clone())
+        refused(call, c, big[:, :0], lens, x, x.clone())
+    with pytest.raises(ValueError):
+        ks.kv4_attention_async(c, over, lens, x, x.clone(), 1.0, ws)
+
+
+@pytest.mark.parametrize("name", ["append", "read"])
+def test_bounded_refusals(ks, call, name):
+    """max_len of the bounded forms; all else as in the forms without."""
+    s = ks.Kv4Cache(call.base, 4, 32, 2, 64, 32)
+    f = getattr(ks.lib(), f"ks_b200_kv4_{name}_bounded_async")
+
+    def run(max_len, n_tokens=3, k=call.base):
+        return f(s._address, call.base, 4, call.base, call.base, 2, n_tokens, max_len, k, 128, 64, call.base, 128, 64,
+                 ks.DTYPE_F32, None, None)
+
+    for bad in (0, 129, 2**64 - 1):
+        assert run(bad) == ks.KS_ERR_INVALID_ARG and ks.last_error()
+    assert run(128, k=None) == ks.KS_ERR_INVALID_ARG
+    assert run(128, n_tokens=0) == ks.KS_OK

@@ -61,7 +61,9 @@ int view_of(const ks_b200_kv4_cache *c, Kv4View *v) {
   return KS_OK;
 }
 
-// max_len 0: what a row of the table holds.
+// max_len kTableHolds: what a row of the table holds.
+constexpr size_t kTableHolds = ~(size_t)0;
+
 int batch_of(const Kv4View &v, const int32_t *page_table, size_t stride, const int32_t *seq_lens,
              const int32_t *offsets, size_t n_seqs, size_t n_tokens, size_t max_len, Kv4Batch *b) {
   if (!page_table || !seq_lens) return fail(KS_ERR_INVALID_ARG, "NULL pointer");
@@ -73,8 +75,8 @@ int batch_of(const Kv4View &v, const int32_t *page_table, size_t stride, const i
   if (n_seqs > 65535 || n_tokens > kMost || stride > kMost)
     return fail(KS_ERR_UNSUPPORTED, "at most 65535 sequences, 2^31 - 1 tokens and table entries");
   const size_t holds = stride << v.page_shift;
+  if (max_len == kTableHolds) max_len = holds;
   if (max_len > holds) return fail(KS_ERR_INVALID_ARG, "max_len is more than a row of the page table holds");
-  if (max_len == 0) max_len = holds < kMost ? holds : kMost;
   if (max_len > kMaxLen) max_len = kMaxLen;
   b->table = page_table;
   b->table_stride = (int64_t)stride;
@@ -140,16 +142,18 @@ extern "C" size_t ks_b200_kv4_page_bytes(size_t page_size, size_t kv_heads, size
 namespace {
 
 int rows_call(bool append, const ks_b200_kv4_cache *cache, const int32_t *page_table, size_t page_table_stride,
-              const int32_t *seq_lens, const int32_t *token_offsets, size_t n_seqs, size_t n_tokens, void *k,
-              size_t k_token_stride, size_t k_head_stride, void *v, size_t v_token_stride, size_t v_head_stride,
-              int dtype, uint32_t *status, void *stream) {
+              const int32_t *seq_lens, const int32_t *token_offsets, size_t n_seqs, size_t n_tokens, size_t max_len,
+              void *k, size_t k_token_stride, size_t k_head_stride, void *v, size_t v_token_stride,
+              size_t v_head_stride, int dtype, uint32_t *status, void *stream) {
   Kv4View view{};
   Kv4Batch b;
   int rc;
   if ((rc = view_of(cache, &view)) != KS_OK) return rc;
-  if ((rc = batch_of(view, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, 0, &b)) != KS_OK)
+  if ((rc = batch_of(view, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, max_len, &b)) !=
+      KS_OK)
     return rc;
   if (n_tokens == 0) return KS_OK;
+  if (max_len == 0) return fail(KS_ERR_INVALID_ARG, "max_len must be > 0");
   if ((rc = rows_ok(k, n_tokens, k_token_stride, cache->kv_heads, k_head_stride, cache->head_dim, dtype, !append)) !=
           KS_OK ||
       (rc = rows_ok(v, n_tokens, v_token_stride, cache->kv_heads, v_head_stride, cache->head_dim, dtype, !append)) !=
@@ -170,7 +174,19 @@ extern "C" int ks_b200_kv4_append_async(const ks_b200_kv4_cache *cache, const in
                                         size_t k_token_stride, size_t k_head_stride, const void *v,
                                         size_t v_token_stride, size_t v_head_stride, int dtype, uint32_t *status,
                                         void *stream) {
-  return rows_call(true, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens,
+  return rows_call(true, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, kTableHolds,
+                   const_cast<void *>(k), k_token_stride, k_head_stride, const_cast<void *>(v), v_token_stride,
+                   v_head_stride, dtype, status, stream);
+}
+
+extern "C" int ks_b200_kv4_append_bounded_async(const ks_b200_kv4_cache *cache, const int32_t *page_table,
+                                                size_t page_table_stride, const int32_t *seq_lens,
+                                                const int32_t *token_offsets, size_t n_seqs, size_t n_tokens,
+                                                size_t max_len, const void *k, size_t k_token_stride,
+                                                size_t k_head_stride, const void *v, size_t v_token_stride,
+                                                size_t v_head_stride, int dtype, uint32_t *status, void *stream) {
+  if (max_len == kTableHolds) return fail(KS_ERR_INVALID_ARG, "max_len is more than a row of the page table holds");
+  return rows_call(true, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, max_len,
                    const_cast<void *>(k), k_token_stride, k_head_stride, const_cast<void *>(v), v_token_stride,
                    v_head_stride, dtype, status, stream);
 }
@@ -180,7 +196,18 @@ extern "C" int ks_b200_kv4_read_async(const ks_b200_kv4_cache *cache, const int3
                                       const int32_t *token_offsets, size_t n_seqs, size_t n_tokens, void *k,
                                       size_t k_token_stride, size_t k_head_stride, void *v, size_t v_token_stride,
                                       size_t v_head_stride, int dtype, uint32_t *status, void *stream) {
-  return rows_call(false, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, k,
+  return rows_call(false, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, kTableHolds,
+                   k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype, status, stream);
+}
+
+extern "C" int ks_b200_kv4_read_bounded_async(const ks_b200_kv4_cache *cache, const int32_t *page_table,
+                                              size_t page_table_stride, const int32_t *seq_lens,
+                                              const int32_t *token_offsets, size_t n_seqs, size_t n_tokens,
+                                              size_t max_len, void *k, size_t k_token_stride, size_t k_head_stride,
+                                              void *v, size_t v_token_stride, size_t v_head_stride, int dtype,
+                                              uint32_t *status, void *stream) {
+  if (max_len == kTableHolds) return fail(KS_ERR_INVALID_ARG, "max_len is more than a row of the page table holds");
+  return rows_call(false, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, max_len, k,
                    k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype, status, stream);
 }
 

@@ -152,6 +152,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _sz, c_int, _vp, _vp],
     ),
+    "ks_b200_kv4_append_bounded_async": (
+        c_int,
+        [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _sz, c_int, _vp, _vp],
+    ),
+    "ks_b200_kv4_read_bounded_async": (
+        c_int,
+        [_vp, _vp, _sz, _vp, _vp, _sz, _sz, _sz, _vp, _sz, _sz, _vp, _sz, _sz, c_int, _vp, _vp],
+    ),
     "ks_b200_kv4_attention_workspace": (_sz, [_vp, _sz, _sz, _sz, _sz, _sz]),
     "ks_b200_kv4_attention_async": (
         c_int,
@@ -426,18 +434,32 @@ def _at(t):
 
 
 def _sequences(page_table, seq_lens, token_offsets=None):
-    """The table's row stride and columns and the number of sequences, which table, lengths and offsets are for."""
+    """The table's row stride and columns and the number of sequences, which table, lengths and offsets are for.  The
+    columns are what a row holds: of a table that is part of a wider one the stride is more."""
     n_seqs = seq_lens.numel()
     stride, one = page_table.stride()
     rows, columns = page_table.shape
     if not _INT32[page_table.dtype] or rows < n_seqs or (one != 1 and columns > 1):
         raise ValueError("a page table must be int32 [n_seqs, pages], its rows contiguous")
+    if stride < columns:
+        if n_seqs > 1:
+            raise ValueError("the rows of a page table may not lie over each other")
+        stride = columns  # of a single row
     if not _INT32[seq_lens.dtype] or not seq_lens.is_contiguous():
         raise ValueError("seq_lens must be contiguous int32 [n_seqs]")
     if token_offsets is not None and (not _INT32[token_offsets.dtype] or token_offsets.numel() <= n_seqs or
                                       not token_offsets.is_contiguous()):
         raise ValueError("token_offsets must be contiguous int32 [n_seqs + 1]")
     return stride, n_seqs, columns
+
+
+def _bound(max_len, holds):
+    """max_len, or what a row of the page table holds and it may not exceed."""
+    if max_len is None:
+        return holds
+    if max_len > holds:
+        raise KernelSmithError(KS_ERR_INVALID_ARG, "max_len is more than a row of the page table holds")
+    return max_len
 
 
 class Kv4Cache(ctypes.Structure):
@@ -471,22 +493,22 @@ def _kv4_rows(call, cache, page_table, seq_lens, k, v, token_offsets, status, st
     shape = k.shape
     if k.dtype != v.dtype or shape != v.shape or shape[1:] != cache._row or k1 != 1 or v1 != 1:
         raise ValueError("k and v must be [n_tokens, kv_heads, head_dim] of one type, the last dimension contiguous")
-    stride, n_seqs, _ = _sequences(page_table, seq_lens, token_offsets)
+    stride, n_seqs, columns = _sequences(page_table, seq_lens, token_offsets)
     rc = call(cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), n_seqs,
-              shape[0], k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DTYPES[k.dtype], _at(status),
-              stream_handle(stream))
+              shape[0], columns * cache.page_size, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DTYPES[k.dtype],
+              _at(status), stream_handle(stream))
     if rc:
         check(rc)
 
 
 def kv4_append_async(cache, page_table, seq_lens, k, v, token_offsets=None, status=None, stream=None) -> None:
     """Quantise the newest tokens of each sequence, k and v [n_tokens, kv_heads, head_dim], into the cache."""
-    _kv4_rows(lib().ks_b200_kv4_append_async, cache, page_table, seq_lens, k, v, token_offsets, status, stream)
+    _kv4_rows(lib().ks_b200_kv4_append_bounded_async, cache, page_table, seq_lens, k, v, token_offsets, status, stream)
 
 
 def kv4_read_async(cache, page_table, seq_lens, k, v, token_offsets=None, status=None, stream=None) -> None:
     """Dequantise the newest tokens of each sequence into k and v [n_tokens, kv_heads, head_dim]."""
-    _kv4_rows(lib().ks_b200_kv4_read_async, cache, page_table, seq_lens, k, v, token_offsets, status, stream)
+    _kv4_rows(lib().ks_b200_kv4_read_bounded_async, cache, page_table, seq_lens, k, v, token_offsets, status, stream)
 
 
 def kv4_attention_workspace(cache, q_heads, n_seqs, n_tokens, max_new, max_len) -> int:
@@ -506,11 +528,11 @@ def kv4_attention_async(cache, page_table, seq_lens, q, out, scale, workspace, t
     if lse is not None and (lse.shape != shape[:2] or not _FLOAT32[lse.dtype] or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous f32 [n_tokens, q_heads]")
     stride, n_seqs, columns = _sequences(page_table, seq_lens, token_offsets)
+    max_len = _bound(max_len, columns * cache.page_size)
     rc = lib().ks_b200_kv4_attention_async(
         cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), n_seqs, n_tokens,
-        max_new, columns * cache.page_size if max_len is None else max_len, q.data_ptr(), qt, qh, q_heads,
-        scale, out.data_ptr(), ot, oh, _DTYPES[q.dtype], _at(lse), 1 if accumulate else 0, workspace.data_ptr(),
-        workspace.numel(), _at(status), stream_handle(stream))
+        max_new, max_len, q.data_ptr(), qt, qh, q_heads, scale, out.data_ptr(), ot, oh, _DTYPES[q.dtype], _at(lse),
+        1 if accumulate else 0, workspace.data_ptr(), workspace.numel(), _at(status), stream_handle(stream))
     if rc:
         check(rc)
 
@@ -524,10 +546,13 @@ def kv4_evict_async(cache, page_table, seq_lens, to_table, to_lens, max_len, bud
     """Keep the newest `recent` tokens of each sequence and head and the heaviest others, `budget` in all, in the
     pages of to_table; kept: None or int32 [n_seqs, kv_heads, budget] for their old positions; workspace: a device
     byte tensor, which may be the attention's."""
-    stride, n_seqs, _ = _sequences(page_table, seq_lens)
-    to_stride, to_seqs, _ = _sequences(to_table, to_lens)
+    stride, n_seqs, columns = _sequences(page_table, seq_lens)
+    to_stride, to_seqs, to_columns = _sequences(to_table, to_lens)
     if to_seqs != n_seqs:
         raise ValueError("seq_lens and to_lens must be of one length")
+    max_len = _bound(max_len, columns * cache.page_size)
+    if to_columns * cache.page_size < min(budget, max_len):
+        raise KernelSmithError(KS_ERR_INVALID_ARG, "a row of to_table holds fewer tokens than may be kept")
     if kept is not None and (kept.shape != (n_seqs, cache._row[0], budget) or not _INT32[kept.dtype] or
                              not kept.is_contiguous()):
         raise ValueError("kept must be a contiguous int32 [n_seqs, kv_heads, budget]")
