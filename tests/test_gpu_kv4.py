@@ -1049,3 +1049,39 @@ def test_tables_that_are_columns_of_wider_ones(ks, cuda, part):
     ks.kv4_read_async(c.cache, column.t(), c.seq_lens[:1], back[0], back[1], status=c.status)
     c.ok()
     assert torch.equal(back[:, 0], results[0][0][:, 0])
+
+
+@pytest.mark.parametrize("name", ["append", "read"])
+@pytest.mark.parametrize("n", [3, 600])
+def test_bad_descriptors_of_sequences_without_rows(ks, cuda, name, n):
+    """Offsets beyond the rows and offsets that fall are reported though no row of the call is theirs, a bad length though
+    the sequence has no new token."""
+    import torch
+
+    d, heads, page = 64, 2, 16
+    pool = torch.zeros(2 * n, ks.kv4_page_bytes(page, heads, d, 32), dtype=torch.uint8, device=cuda)
+    cache = ks.Kv4Cache(pool, 2 * n, page, heads, d, 32)
+    table = torch.arange(2 * n, dtype=torch.int32, device=cuda).reshape(n, 2)
+    call = ks.kv4_append_async if name == "append" else ks.kv4_read_async
+
+    def status_of(news, tokens, change=None, at=0, value=0):
+        offsets = torch.tensor(np.concatenate([[0], np.cumsum(news)]), dtype=torch.int32, device=cuda)
+        lens = torch.full((n,), 20, dtype=torch.int32, device=cuda)
+        if change == "offset":
+            offsets[at] = value
+        if change == "length":
+            lens[at] = value
+        x = torch.ones(2, tokens, heads, d, device=cuda)
+        status = torch.zeros(2, dtype=torch.int32, device=cuda)
+        call(cache, table, lens, x[0], x[1], token_offsets=offsets, status=status)
+        torch.cuda.synchronize()
+        return status.tolist()
+
+    idle = [4] + [0] * (n - 1)
+    assert status_of(idle, 4) == [0, 0] and status_of([4] * n, 4 * n) == [0, 0]
+    assert status_of(idle[:-1] + [5], 4) == [1, 0]  # the last sequence's rows are all beyond the tensors'
+    for at in (1, n - 1):
+        for length in (-1, 33, 1 << 30):
+            assert status_of(idle, 4, "length", at, length) == [1, 0]
+    for value in (2, -5, 5):  # fall at the sequence before or behind, or go beyond the rows
+        assert status_of(idle, 4, "offset", n - 1, value) == [1, 0]

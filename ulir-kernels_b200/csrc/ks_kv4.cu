@@ -159,6 +159,10 @@ __device__ __forceinline__ void find_places(const Kv4View &c, const Kv4Batch &b,
     }
     places[threadIdx.x] = p;
   }
+  // One CTA looks at every sequence, so that those without a row are reported too: from the last thread down, as the
+  // first ones have the lookups of short calls.
+  if (blockIdx.x == 0 && blockIdx.y == 0)
+    for (int s = kRowThreads - 1 - (int)threadIdx.x; s < b.n_seqs; s += kRowThreads) kv4_seq(b, s, status);
   __syncthreads();
 }
 
