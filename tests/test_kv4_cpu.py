@@ -236,3 +236,18 @@ def test_bounded_refusals(ks, call, name):
         assert run(bad) == ks.KS_ERR_INVALID_ARG and ks.last_error()
     assert run(128, k=None) == ks.KS_ERR_INVALID_ARG
     assert run(128, n_tokens=0) == ks.KS_OK
+
+
+def test_python_offsets_need_max_new(ks):
+    """Without it, rows behind the first of a sequence were left unwritten and, without status, nothing said so."""
+    torch = pytest.importorskip("torch")
+    c = ks.Kv4Cache(16, 4, 16, 2, 64, 32)
+    table, lens = torch.zeros(2, 4, dtype=torch.int32), torch.zeros(2, dtype=torch.int32)
+    q, ws, offsets = torch.zeros(5, 2, 64), torch.zeros(16, dtype=torch.uint8), torch.tensor([0, 2, 5]).int()
+    with pytest.raises(ValueError, match="max_new"):
+        ks.kv4_attention_async(c, table, lens, q, q.clone(), 1.0, ws, token_offsets=offsets)
+    # with it, and without offsets, the library looks at what follows (too small a workspace)
+    for rows, kwargs in ((5, dict(token_offsets=offsets, max_new=3)), (2, {})):
+        with pytest.raises(ks.KernelSmithError) as e:
+            ks.kv4_attention_async(c, table, lens, q[:rows], q[:rows].clone(), 1.0, ws, **kwargs)
+        assert e.value.rc == ks.KS_ERR_WORKSPACE

@@ -515,11 +515,11 @@ def kv4_attention_workspace(cache, q_heads, n_seqs, n_tokens, max_new, max_len) 
     return lib().ks_b200_kv4_attention_workspace(cache._address, q_heads, n_seqs, n_tokens, max_new, max_len)
 
 
-def kv4_attention_async(cache, page_table, seq_lens, q, out, scale, workspace, token_offsets=None, max_new=1,
+def kv4_attention_async(cache, page_table, seq_lens, q, out, scale, workspace, token_offsets=None, max_new=None,
                         max_len=None, lse=None, accumulate=False, status=None, stream=None) -> None:
-    """Attention of the newest tokens, q and out [n_tokens, q_heads, head_dim], over the cache.  max_len: no
-    sequence is longer (default: what a row of the page table holds); workspace: a device byte tensor, zero-filled
-    before its first use."""
+    """Attention of the newest tokens, q and out [n_tokens, q_heads, head_dim], over the cache.  max_new: no sequence
+    has more new tokens (needed with token_offsets, else 1); max_len: no sequence is longer (default: what a row of the
+    page table holds); workspace: a device byte tensor, zero-filled before its first use."""
     qt, qh, q1 = q.stride()
     ot, oh, o1 = out.stride()
     n_tokens, q_heads, head_dim = shape = q.shape
@@ -528,6 +528,10 @@ def kv4_attention_async(cache, page_table, seq_lens, q, out, scale, workspace, t
     if lse is not None and (lse.shape != shape[:2] or not _FLOAT32[lse.dtype] or not lse.is_contiguous()):
         raise ValueError("lse must be a contiguous f32 [n_tokens, q_heads]")
     stride, n_seqs, columns = _sequences(page_table, seq_lens, token_offsets)
+    if max_new is None:
+        if token_offsets is not None:
+            raise ValueError("token_offsets needs max_new, the most new tokens of a sequence")
+        max_new = 1
     max_len = _bound(max_len, columns * cache.page_size)
     rc = lib().ks_b200_kv4_attention_async(
         cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), n_seqs, n_tokens,
