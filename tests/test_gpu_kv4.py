@@ -1085,3 +1085,47 @@ def test_bad_descriptors_of_sequences_without_rows(ks, cuda, name, n):
             assert status_of(idle, 4, "length", at, length) == [1, 0]
     for value in (2, -5, 5):  # fall at the sequence before or behind, or go beyond the rows
         assert status_of(idle, 4, "offset", n - 1, value) == [1, 0]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,group,heads,q_heads,lens,news", [
+    (128, 32, 2, 8, [3000, 700, 33, 1], [1, 1, 1, 1]),
+    (64, 64, 3, 3, [1500, 90, 400], [1, 1, 1]),
+    (128, 128, 1, 6, [800, 64], [9, 5]),
+    (64, 32, 2, 2, [900, 5], [30, 5]),
+])
+def test_lse_and_weights_by_their_norms(ks, cuda, dtype, d, group, heads, q_heads, lens, news):
+    """lse and the added weights of all rows together, where roundings do not add up to their worst case.
+
+    A score's error, per row: its roundings to f32 (as for the outputs' norm) 2^-22 |z|, sums, exponentials and the
+    logarithm 2^-20.  f16 and bf16 queries: the products run in accumulators that truncate, half of 2^-23 of the partial
+    sum in the mean over d / 16 steps, and that partial sum is about 8 |sum q| of a group (from which it starts) and
+    8 sqrt(sum q^2) (codes + 8, of random signs) times the key scale.  f32 queries: what is left of two parts, 2^-23 of
+    the row's largest element over d elements of random sign, times the keys' root mean square.  A weight's relative
+    error is that of the score and of lse, an exponential (2^-21) and the sums (2^-23)."""
+    c = Seqs(ks, cuda, lens, news, heads, d, group, 16, seed=d + group, weights=True)
+    before = c.w.double().cpu().numpy()
+    q, scale = _query(c, q_heads, dtype), d**-0.5
+    out, lse = _attend(c, q, scale, accumulate=True)
+    c.ok()
+    qn, lse = q.double().cpu().numpy(), lse.double().cpu().numpy()
+    after = c.w.double().cpu().numpy()
+    sums = np.abs(qn.reshape(*qn.shape[:2], -1, group).sum(-1)).max(-1)
+    if dtype == "f32":
+        product = 2.0**-23 * np.abs(qn).max(-1) * d**0.5 * (c.k**2).mean() ** 0.5
+    else:
+        product = 2.0**-24 * d / 16 * 8 * c.scale_max * (sums + np.sqrt((qn**2).sum(-1)))
+    err = most = werr = wmost = 0.0
+    for s in range(len(lens)):
+        a, n = c.first[s], news[s]
+        _, z, w, _, _ = O.kv4_attention(qn[a:a + n], c.cached(s, "k"), c.cached(s, "v"), scale, n)
+        seen = np.isfinite(z)
+        bound = np.where(seen, 2.0**-20 + 2.0**-22 * np.abs(np.where(seen, z, 0)), 0) \
+            + scale * product[a:a + n]
+        err, most = err + ((lse[a:a + n] - z)[seen] ** 2).sum(), most + (bound[seen] ** 2).sum()
+        old, got = c.weights_of(s, before), c.weights_of(s, after)
+        rel = 2 * bound.max() + 2.0**-21
+        werr = werr + ((got - old - w) ** 2).sum()
+        wmost = wmost + ((rel * w + 2.0**-23 * (old + w)) ** 2).sum()
+    assert err**0.5 <= most**0.5, (err**0.5, most**0.5)
+    assert werr**0.5 <= wmost**0.5, (werr**0.5, wmost**0.5)
