@@ -1129,3 +1129,93 @@ def test_lse_and_weights_by_their_norms(ks, cuda, dtype, d, group, heads, q_head
         wmost = wmost + ((rel * w + 2.0**-23 * (old + w)) ** 2).sum()
     assert err**0.5 <= most**0.5, (err**0.5, most**0.5)
     assert werr**0.5 <= wmost**0.5, (werr**0.5, wmost**0.5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,group,q_heads", [(128, 32, 4), (64, 64, 1), (128, 64, 12), (128, 128, 2), (64, 32, 9)])
+@pytest.mark.parametrize("order", ["last", "first", "groups", "shared"])
+def test_values_of_unlike_sizes(ks, cuda, dtype, d, group, q_heads, order):
+    """A result far below the values that have next to no weight in it keeps its bits.
+
+    last, first: one token has all the weight, its values are 2^-k of the others', which come before or after it.
+    groups: the first groups' values are 2^k of the others', in every token.  shared: the large values have weights of
+    about 2^-k, so that both are in the result.  Errors by group and head, against the group's norm: scores of up to 64
+    are rounded to f32 (2^-21 of |lse|), exponentials, sums and the two parts are within 2^-17, one part of bf16 2^-12,
+    and the result is rounded once."""
+    import torch
+
+    T, n, page = _type(dtype), 300, 32
+    half = torch.finfo(T).eps / 2
+    for k in (12, 18, 24, 30, 38):
+        c = Seqs(ks, cuda, [n], [1], 1, d, group, page, seed=k, garbage=True)
+        gen = torch.Generator(device=cuda).manual_seed(k)
+        # the largest scale is 2^12, the least 2^(12 - k) about
+        big, small = 2.0**12 * 7, 2.0**12 * 7 * 2.0**-min(k, 34)
+        keys = torch.zeros(n, 1, d, device=cuda)
+        values = torch.randn(n, 1, d, generator=gen, device=cuda).clamp(-1, 1) * 0.83  # scales of many bits
+        one = {"first": 7, "last": 290}.get(order, 150)
+        gap = min(k, 34) * 0.693 if order == "shared" else 64.0
+        if order == "groups":
+            values *= torch.where(torch.arange(d, device=cuda) < max(group, d // 2), big, small)
+            if group == d:
+                continue
+        else:
+            keys[one] = gap / d
+            values *= big
+            values[one] *= small / big
+        offsets = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+        ks.kv4_append_async(c.cache, c.table, c.seq_lens, keys, values, token_offsets=offsets, status=c.status)
+        ks.kv4_read_async(c.cache, c.table, c.seq_lens, keys, values, token_offsets=offsets, status=c.status)
+        q = torch.ones(1, q_heads, d, device=cuda).to(T)
+        out, lse = _attend(c, q, 1.0)
+        c.ok()
+        want, z, _, _, _ = O.kv4_attention(q.double().cpu().numpy(), keys.double().cpu().numpy(),
+                                           values.double().cpu().numpy(), 1.0, 1)
+        got = out.double().cpu().numpy()
+        tiny = float(torch.finfo(T).smallest_normal) * half  # of results below the type's normal numbers
+        most = half + 2.0**-17 + 2.0**-21 * np.abs(z).max() + (2.0**-12 if dtype == "bf16" else 0)
+        err = np.sqrt(((got - want).reshape(q_heads, -1, group) ** 2).sum(-1))
+        norm = np.sqrt((want.reshape(q_heads, -1, group) ** 2).sum(-1))
+        assert (err <= most * norm + 2 * tiny * group**0.5).all(), (k, (err / norm).max(), most)
+
+
+@pytest.mark.parametrize("dtype,d,q_heads", [("f16", 128, 2), ("bf16", 64, 9), ("f32", 128, 1)])
+def test_values_of_unlike_sizes_in_long_items(ks, cuda, dtype, d, q_heads):
+    """The same where each CTA goes over a long item: its first three quarters have the large values and together a weight
+    of 2^-24, the rest values 2^-30 of theirs and, but for the last token, lower scores still."""
+    import torch
+
+    T, n, page, seqs, group = _type(dtype), 40000, 64, 444, 64
+    pages = -(-n // page)
+    pool = torch.zeros(pages, ks.kv4_page_bytes(page, 1, d, group), dtype=torch.uint8, device=cuda)
+    cache = ks.Kv4Cache(pool, pages, page, 1, d, group)
+    table = torch.arange(pages, dtype=torch.int32, device=cuda).repeat(seqs, 1)
+    lens = torch.full((seqs,), n, dtype=torch.int32, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    score = torch.rand(n, 1, 1, generator=gen, device=cuda) * 8  # e^8 = 2^11.5
+    score[3 * n // 4:] -= 8
+    score[-1] = 33  # 2^47.6 against the sum of 30000 of up to 2^11.5
+    k = (score / d).expand(n, 1, d).contiguous()
+    v = torch.randn(n, 1, d, generator=gen, device=cuda) * 2.0**12
+    v[3 * n // 4:] *= 2.0**-30
+    offsets = torch.tensor([0, n], dtype=torch.int32, device=cuda)
+    status = torch.zeros(2, dtype=torch.int32, device=cuda)
+    ks.kv4_append_async(cache, table[:1], lens[:1], k, v, token_offsets=offsets, status=status)
+    ks.kv4_read_async(cache, table[:1], lens[:1], k, v, token_offsets=offsets, status=status)
+    q = torch.ones(seqs, q_heads, d, dtype=T, device=cuda)
+    out, lse = torch.zeros_like(q), torch.zeros(seqs, q_heads, device=cuda)
+    ws = torch.zeros(ks.kv4_attention_workspace(cache, q_heads, seqs, seqs, 1, n), dtype=torch.uint8, device=cuda)
+    ks.kv4_attention_async(cache, table, lens, q, out, 1.0, ws, max_len=n, lse=lse, status=status)
+    torch.cuda.synchronize()
+    assert status.tolist() == [0, 0]
+    x = q[0].double() @ k[:, 0].double().T
+    p = torch.softmax(x, -1)
+    want, z = p @ v[:, 0].double(), torch.logsumexp(x, -1)
+    # both parts are in the result, within 2^6 of one another
+    parts = [(p[:, a] @ v[a, 0].double()).norm() for a in (slice(0, 3 * n // 4), slice(3 * n // 4, n))]
+    assert 2.0**-6 < parts[0] / parts[1] < 2.0**6
+    most = torch.finfo(T).eps / 2 + 2.0**-17 + 2.0**-16 + 2.0**-21 * z.max() + (2.0**-12 if dtype == "bf16" else 0)
+    tiny = torch.finfo(T).smallest_normal * torch.finfo(T).eps  # of results below the type's normal numbers
+    err = (out.double() - want).unflatten(-1, (-1, group)).norm(dim=-1)
+    norm = want.unflatten(-1, (-1, group)).norm(dim=-1)
+    assert (err <= most * norm + tiny * group**0.5).all(), ((err / norm).max(), most)

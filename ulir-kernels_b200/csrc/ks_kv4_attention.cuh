@@ -70,6 +70,7 @@
 #pragma once
 
 #include <atomic>
+#include <type_traits>
 
 #include "ks_kv4.cuh"
 
@@ -698,15 +699,20 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
       }
       float lift = 0.0f;
       __half2 scale_limit = __floats2half2_rn(0.0f, 0.0f);  // value scales up to this one fit
+      // The least value scale so far (a lane's own).  Below 2^-11 of the limit its weights would lose bits: from there on
+      // each tile's weights have a power of two of their own (apart).
+      __half2 least = __floats2half2_rn(INFINITY, INFINITY);
+      auto too_small = [&] { return !__hbge2(__hmul2(least, __floats2half2_rn(2048.0f, 2048.0f)), scale_limit); };
 
-      // A turn's sums (f16, bf16), added to those of the turns before it, which are in units of 2^folded_base (volatile: in
-      // local memory, the registers are taken); unfold brings them to units of 2^base, which has only risen.
-      [[maybe_unused]] volatile float folded[kFold ? NT : 1][kFold ? D / 16 : 1][4], folded_base[kFold ? NT : 1][2];
+      // Sums of the tiles before, in units of 2^folded_base (volatile: in local memory, the registers are taken), and their
+      // factor in units of 2^base, which has only risen.
+      [[maybe_unused]] volatile float folded[WEIGHTS ? 1 : NT][WEIGHTS ? 1 : D / 16][4], folded_base[WEIGHTS ? 1 : NT][2];
       [[maybe_unused]] auto unfold = [&](int nt, int e) { return fast_exp2(folded_base[nt][e] - base[nt][e]); };
-      auto fold = [&](int i) {
-        if constexpr (kFold) {
-          if (i == count) return;
-          const bool first = i == kFoldTiles;
+      bool has_folded = false;
+      auto fold = [&] {
+        if constexpr (!WEIGHTS) {
+          const bool first = !has_folded;
+          has_folded = true;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -724,9 +730,10 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
         }
       };
 
-      for (int i = 0, stage_out = 0; i < count; fold(i))  // turns, and tiles of a turn
-      for (const int turn = kFold ? min(i + kFoldTiles, count) : count; i < turn;
-           ++i, stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1) {
+      int i = 0, stage_out = 0;  // the tile and its place in the ring
+      // Goes over the tile (and is true), or finds that it has to be gone over with weights apart.
+      auto go_over = [&](auto weights_apart) {
+        [[maybe_unused]] constexpr bool kApart = decltype(weights_apart)::value;
         const int at = begin + (warp + i * kAttnWarps) * kTileTokens;
         char *buf = ring + stage_out * S::kStage;
         asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
@@ -780,12 +787,13 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
               for (int b = 1; b < kTileBlocks; ++b) m[nt][e] = fmaxf(m[nt][e], fmaxf(p[b][nt][e], p[b][nt][e + 2]));
               rise |= m[nt][e] > limit[nt][e];
             }
-          if (!whole) {  // what stands behind the last token is not a scale
+          if (!whole) {  // what stands behind the last token is not a scale: the tile's first token's in its place
+            const __half *first = reinterpret_cast<const __half *>(buf + S::kBlock / 2 + 8 * D);
             for (int x = lane; x < kTileTokens; x += 32)
               if (at + x >= end)
                 for (int gr = 0; gr < NG; ++gr)
                   reinterpret_cast<__half *>(buf + (x >> 4) * S::kBlock + S::kBlock / 2 + 8 * D)[(x & 15) * NG + gr] =
-                      __ushort_as_half(0);
+                      first[gr];
             __syncwarp();
           }
           __half2 h[kTileBlocks][2][(NG + 1) / 2], big = __floats2half2_rn(0.0f, 0.0f);
@@ -803,9 +811,12 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
                 for (int x = 0; x < NG / 2; ++x) h[b][e][x] = *reinterpret_cast<const __half2 *>(&w[x]);
               }
 #pragma unroll
-              for (int x = 0; x < (NG + 1) / 2; ++x) big = __hmax2(big, h[b][e][x]);
+              for (int x = 0; x < (NG + 1) / 2; ++x) {
+                big = __hmax2(big, h[b][e][x]);
+                if (!kApart) least = __hmin2(least, h[b][e][x]);
+              }
             }
-          if (__any_sync(0xffffffffu, rise || !__hble2(big, scale_limit))) {
+          if (__any_sync(0xffffffffu, rise || !__hble2(big, scale_limit) || (!kApart && too_small()))) {
             float all = fmaxf(__low2float(big), __high2float(big));
 #pragma unroll
             for (int x = 4; x < 32; x *= 2) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
@@ -833,10 +844,16 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
                 sum[nt][e] *= f;
 #pragma unroll
                 for (int d = 0; d < D / 16; ++d) {
-                  o[nt][d][e] *= f;
-                  o[nt][d][e + 2] *= f;
+                  if constexpr (kApart) {
+                    folded[nt][d][e] = folded[nt][d][e] * f;
+                    folded[nt][d][e + 2] = folded[nt][d][e + 2] * f;
+                  } else {
+                    o[nt][d][e] *= f;
+                    o[nt][d][e + 2] *= f;
+                  }
                 }
               }
+            if (!kApart && __any_sync(0xffffffffu, too_small())) return false;
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -857,79 +874,149 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
               lds<D / 16>(buf + b * S::kBlock + S::kBlock / 2 +
                               (kv4_token(2 * t + (e & 1)) + 8 * (e >> 1)) * (D / 2) + g * (D / 16),
                           v[b][e]);
+          // the slice m of the 16 elements of a block's tokens, as an A operand
+          auto value_slice = [&](int b, int m, uint32_t (&a)[4]) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t w = prmt(v[b][2 * e][m / 4], v[b][2 * e + 1][m / 4], (m % 4) | ((4 + m % 4) << 8));
+              const uint32_t lo = and_xor(w, 0x000F000Fu, 0x64086408u), hi = and_xor(w, 0x00F000F0u, 0x64806480u);
+              const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&lo), __floats2half2_rn(1032.0f, 1032.0f));
+              const __half2 y = __hfma2(*reinterpret_cast<const __half2 *>(&hi), __floats2half2_rn(0.0625f, 0.0625f),
+                                        __floats2half2_rn(-72.0f, -72.0f));
+              a[2 * e] = *reinterpret_cast<const uint32_t *>(&x);
+              a[2 * e + 1] = *reinterpret_cast<const uint32_t *>(&y);
+            }
+          };
+          // the value scale of group gr, of token g (e = 0) or g + 8 of a block
+          auto value_scale = [&](int b, int e, int gr) {
+            constexpr int kTwo = NG > 1 ? 2 : 1;
+            const __half2 pair = h[b][e][gr / kTwo];
+            return gr % kTwo ? __high2float(pair) : __low2float(pair);
+          };
           uint32_t ph[kTileBlocks][NT][2], pl[kTileBlocks][NT][2];
+          // two tokens' weights as (one or two) f16 parts, rows and tokens exchanged
+          auto place_weights = [&](int b, int nt, int e, float x0, float x1) {
+            const uint32_t h = pack_f16(x0, x1);
+            ph[b][nt][e] = transpose8x8(h);
+            if (PS == 2) {
+              const float2 r = unpack_f16(h);
+              pl[b][nt][e] = transpose8x8(pack_f16(x0 - r.x, x1 - r.y));
+            }
+          };
+          constexpr int M = D / 16 / NG;  // slices of a group
+          if constexpr (!kApart) {
 #pragma unroll
-          for (int m = 0; m < D / 16; ++m) {
-            constexpr int M = D / 16 / NG;  // slices of a group
-            if (m % M == 0) {
+            for (int m = 0; m < D / 16; ++m) {
+              if (m % M == 0) {
 #pragma unroll
-              for (int b = 0; b < kTileBlocks; ++b)
+                for (int b = 0; b < kTileBlocks; ++b)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                  constexpr int kTwo = NG > 1 ? 2 : 1;
-                  const __half2 pair = h[b][e][m / M / kTwo];
-                  const float f = m / M % kTwo ? __high2float(pair) : __low2float(pair);
+                  for (int e = 0; e < 2; ++e) {
+                    const float f = value_scale(b, e, m / M);
 #pragma unroll
-                  for (int nt = 0; nt < NT; ++nt) {
-                    const float x0 = p[b][nt][2 * e] * f, x1 = p[b][nt][2 * e + 1] * f;
-                    const uint32_t h = pack_f16(x0, x1);
-                    ph[b][nt][e] = transpose8x8(h);
-                    if (PS == 2) {
-                      const float2 r = unpack_f16(h);
-                      pl[b][nt][e] = transpose8x8(pack_f16(x0 - r.x, x1 - r.y));
-                    }
+                    for (int nt = 0; nt < NT; ++nt)
+                      place_weights(b, nt, e, p[b][nt][2 * e] * f, p[b][nt][2 * e + 1] * f);
                   }
+              }
+              float acc[NT][4];
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nt][e] = kWide ? 0.0f : o[nt][m][e];
+#pragma unroll
+              for (int b = 0; b < kTileBlocks; ++b) {
+                uint32_t a[4];
+                value_slice(b, m, a);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                  mma_f16(acc[nt], a[0], a[1], a[2], a[3], ph[b][nt][0], ph[b][nt][1]);
+                  if (PS == 2) mma_f16(acc[nt], a[0], a[1], a[2], a[3], pl[b][nt][0], pl[b][nt][1]);
                 }
+              }
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[nt][m][e] = kWide ? o[nt][m][e] + acc[nt][e] : acc[nt][e];
             }
-            float acc[NT][4];
+          } else {
+            // the tile's largest weight of a row and group in [2^13, 2^14), one slice and row tile after the other
+            float down[2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[nt][e] = kWide ? 0.0f : o[nt][m][e];
+              for (int m = 0; m < D / 16; ++m) {
+                if (m % M == 0) {
+                  float up[2];
 #pragma unroll
-            for (int b = 0; b < kTileBlocks; ++b) {
-              uint32_t a[4];
+                  for (int r = 0; r < 2; ++r) {
+                    float x = 0.0f;
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const uint32_t w = prmt(v[b][2 * e][m / 4], v[b][2 * e + 1][m / 4], (m % 4) | ((4 + m % 4) << 8));
-                const uint32_t lo = and_xor(w, 0x000F000Fu, 0x64086408u), hi = and_xor(w, 0x00F000F0u, 0x64806480u);
-                const __half2 x = __hsub2(*reinterpret_cast<const __half2 *>(&lo), __floats2half2_rn(1032.0f, 1032.0f));
-                const __half2 y = __hfma2(*reinterpret_cast<const __half2 *>(&hi), __floats2half2_rn(0.0625f, 0.0625f),
-                                          __floats2half2_rn(-72.0f, -72.0f));
-                a[2 * e] = *reinterpret_cast<const uint32_t *>(&x);
-                a[2 * e + 1] = *reinterpret_cast<const uint32_t *>(&y);
+                    for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+                      for (int e = 0; e < 2; ++e) x = fmaxf(x, p[b][nt][2 * e + r] * value_scale(b, e, m / M));
+#pragma unroll
+                    for (int y = 4; y < 32; y *= 2) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, y));
+                    const int power = x > 0.0f && isfinite(x) ? min(max(13 - ilogbf(x), -126), 126) : 0;
+                    up[r] = ldexpf(1.0f, power);
+                    down[r] = ldexpf(1.0f, -power);
+                  }
+#pragma unroll
+                  for (int b = 0; b < kTileBlocks; ++b)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                      const float f = value_scale(b, e, m / M);
+                      place_weights(b, nt, e, p[b][nt][2 * e] * f * up[0], p[b][nt][2 * e + 1] * f * up[1]);
+                    }
+                }
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int b = 0; b < kTileBlocks; ++b) {
+                  uint32_t a[4];
+                  value_slice(b, m, a);
+                  mma_f16(acc, a[0], a[1], a[2], a[3], ph[b][nt][0], ph[b][nt][1]);
+                  if (PS == 2) mma_f16(acc, a[0], a[1], a[2], a[3], pl[b][nt][0], pl[b][nt][1]);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; ++e) folded[nt][m][e] = fmaf(acc[e], down[e & 1], folded[nt][m][e]);
               }
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) {
-                mma_f16(acc[nt], a[0], a[1], a[2], a[3], ph[b][nt][0], ph[b][nt][1]);
-                if (PS == 2) mma_f16(acc[nt], a[0], a[1], a[2], a[3], pl[b][nt][0], pl[b][nt][1]);
-              }
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) o[nt][m][e] = kWide ? o[nt][m][e] + acc[nt][e] : acc[nt][e];
           }
         }
+        return true;
+      };
+      auto done = [&] {  // with the tile
         __syncwarp();  // every lane has read the stage
         fetch();
+        ++i;
+        stage_out = stage_out + 1 == kStages ? 0 : stage_out + 1;
+      };
+      bool together = true;
+      while (together && i < count) {
+        for (const int turn = kFold ? min(i + kFoldTiles, count) : count; i < turn; done())
+          if (!(together = go_over(std::false_type()))) break;
+        if (together && i < count) fold();
+      }
+      if constexpr (!WEIGHTS) {
+        if (!together) {
+          fold();
+          for (; i < count; done()) go_over(std::true_type());
+        }
       }
       if constexpr (!WEIGHTS) {
         // The next kernel may be set up: not before, or its CTAs would take the places that the first CTAs to end leave,
         // some SMs more of them than others.
         if (unit >= end_unit) kv4_next();
-        if constexpr (kFold) {
-          if (count > kFoldTiles)
+        if (has_folded) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float f = unfold(nt, e);
+            for (int e = 0; e < 2; ++e) {
+              const float f = unfold(nt, e);
 #pragma unroll
-                for (int m = 0; m < D / 16; ++m)
+              for (int m = 0; m < D / 16; ++m)
 #pragma unroll
-                  for (int h = e; h < 4; h += 2) o[nt][m][h] = fmaf(folded[nt][m][h], f, o[nt][m][h]);
-              }
+                for (int h = e; h < 4; h += 2)
+                  o[nt][m][h] = together ? fmaf(folded[nt][m][h], f, o[nt][m][h]) : folded[nt][m][h];
+            }
         }
         // join the warps: the ring is drained, each writes its part over it
 #pragma unroll
