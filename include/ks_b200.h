@@ -658,9 +658,11 @@ int ks_b200_kv4_read_bounded_async(const ks_b200_kv4_cache *cache,
  * new tokens, the j-th sees positions 0 .. seq_lens[s] - n + j, and query head
  * h reads key/value head h / (q_heads / kv_heads):
  *   out = sum_t exp(scale * q . k_t - lse) v_t,  lse = log sum_t exp(scale * q . k_t).
- * A row that sees nothing gets zeros and lse -inf.  Sums are f32; for f32
- * tensors the products keep 22 bits of queries and probabilities, so results
- * agree with f32 arithmetic; queries are finite and below 2^110.  lse: f32
+ * A row that sees nothing gets zeros and lse -inf.  Sums are f32.  For f32
+ * tensors the products keep queries to 2^-23 of their row's largest element and
+ * 22 bits of probabilities times value scales, so results agree with f32
+ * arithmetic; for f16 and bf16 tensors queries to 2^-35 of it and 22 and 11 bits
+ * of the latter.  Queries are finite and below 2^110.  lse: f32
  * [n_tokens][q_heads], or NULL.  accumulate != 0 adds to cache->weights of
  * every cached token the attention weight it received, summed over the
  * sequence's new tokens and the query heads of its key/value head, in a fixed

@@ -67,6 +67,14 @@
 // in f32 (kept for a whole item of 524288 tokens, they lost 7e-4, more than half
 // a step of f16; adding up after every tile, as for f32, takes 6 % more time at
 // 64 sequences of up to 8192, this 1 %).
+// A weight (probability times value scale) has its parts' last bit at 2^-24,
+// where the largest value scale stands at 2^10: 22 bits for scales down to 2^-11
+// of that.  Once a warp meets a smaller one, in any token or group, it goes on in
+// a second form of the loop, where the largest weight of each tile, row and group
+// is brought to 2^13 and each tile's product is added in f32: a result far below
+// values that have next to no weight in it keeps its bits (without, it lost all of
+// them from 2^-36 on).  Looking for such a scale takes 1 to 3 % (64 sequences of
+// up to 8192, bf16: 68.6 -> 69.4 us; 16 of up to 4096, f32: 21.7 -> 22.2).
 #pragma once
 
 #include <atomic>
