@@ -1219,3 +1219,24 @@ def test_values_of_unlike_sizes_in_long_items(ks, cuda, dtype, d, q_heads):
     err = (out.double() - want).unflatten(-1, (-1, group)).norm(dim=-1)
     norm = want.unflatten(-1, (-1, group)).norm(dim=-1)
     assert (err <= most * norm + tiny * group**0.5).all(), ((err / norm).max(), most)
+
+
+def test_append_from_most_rows(ks, cuda):
+    """As many rows as a call takes (one in memory, its stride 0), three of them a sequence's."""
+    import torch
+
+    d, page, rows = 64, 16, 2**31 - 1
+    pool = torch.zeros(2, ks.kv4_page_bytes(page, 1, d, 64), dtype=torch.uint8, device=cuda)
+    cache = ks.Kv4Cache(pool, 2, page, 1, d, 64)
+    table = torch.arange(2, dtype=torch.int32, device=cuda)[None]
+    lens = torch.tensor([20], dtype=torch.int32, device=cuda)
+    status = torch.zeros(2, dtype=torch.int32, device=cuda)
+    x = torch.randn(1, 1, d, device=cuda).expand(rows, 1, d)
+    offsets = torch.tensor([rows - 3, rows], dtype=torch.int32, device=cuda)
+    ks.kv4_append_async(cache, table, lens, x, x, token_offsets=offsets, status=status)
+    back = torch.zeros(2, 3, 1, d, device=cuda)
+    ks.kv4_read_async(cache, table, lens, back[0], back[1], token_offsets=offsets - (rows - 3), status=status)
+    torch.cuda.synchronize()
+    assert status.tolist() == [0, 0]
+    want = O.kv4_value(*O.kv4_quantize(x[0].double().cpu().numpy(), 64))
+    assert (back.double().cpu().numpy() == want).all()

@@ -209,7 +209,7 @@ __device__ __forceinline__ void append_rows(const Kv4View &c, const Kv4Place *pl
   for (RowWalk at(threadIdx.x >> 2, c.kv_heads); __any_sync(0xffffffffu, at.token < tokens); at.next()) {
     const int token = at.token, head = at.head;
     const Kv4Place p = token < tokens ? places[token] : Kv4Place{-1, 0};
-    const T *src = x + (int64_t)(first_row + token) * token_stride + head * head_stride;
+    const T *src = x + ((int64_t)first_row + token) * token_stride + head * head_stride;
     float v[E];
     if (p.page < 0) {
 #pragma unroll
@@ -345,7 +345,7 @@ __device__ __forceinline__ void read_rows(const Kv4View &c, const Kv4Place *plac
       load_scales<NG>(half + 8 * D + (p.slot & 15) * 2 * NG, sc);
 #pragma unroll
       for (int g = 0; g < D / 32; ++g) s[n][g] = sc[g * NG / (D / 32)];
-      dst[n] = x + (int64_t)(first_row + token) * token_stride + head * head_stride;
+      dst[n] = x + ((int64_t)first_row + token) * token_stride + head * head_stride;
     }
 #pragma unroll
     for (int n = 0; n < N; ++n) {
@@ -409,8 +409,9 @@ cudaError_t launch_rows(const Kv4View &c, const Kv4Batch &b, const Kv4Rows &r, u
   int tokens = (b.n_tokens - 1) / (kSlots * waves) + 1;
   tokens = (tokens + turn - 1) / turn * turn;
   tokens = tokens > kRowTokens ? kRowTokens : tokens;
-  while (tokens > 1 && (b.n_tokens + tokens - 1) / tokens < 148) tokens /= 2;
-  const dim3 grid((unsigned)((b.n_tokens + tokens - 1) / tokens), 2);
+  auto ctas = [&](int each) { return (unsigned)((b.n_tokens - 1) / each) + 1; };
+  while (tokens > 1 && ctas(tokens) < 148) tokens /= 2;
+  const dim3 grid(ctas(tokens), 2);
   auto *kernel = r.dtype == kF32   ? kv4_rows_kernel<float, D, NG, READ>
                  : r.dtype == kF16 ? kv4_rows_kernel<__half, D, NG, READ>
                                    : kv4_rows_kernel<__nv_bfloat16, D, NG, READ>;
