@@ -586,6 +586,7 @@ int ks_b200_import_ggml_q4_0_async(const void *blocks, size_t block_row_stride,
  * tokens than the sequence has or a key or value that is not finite (stored
  * as 0 if NaN, else as the largest code): no call reads or writes outside
  * its buffers then, the sequences concerned are unspecified.
+ * A sequence has at most 2^31 - 16385 tokens, whatever max_len says.
  * head_dim must be 64 or 128, group_size 32, 64 or 128 and at most head_dim,
  * page_size 16, 32, 64, 128 or 256, else KS_ERR_UNSUPPORTED.
  */

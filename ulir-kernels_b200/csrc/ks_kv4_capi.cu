@@ -214,6 +214,7 @@ extern "C" int ks_b200_kv4_read_bounded_async(const ks_b200_kv4_cache *cache, co
 extern "C" size_t ks_b200_kv4_attention_workspace(const ks_b200_kv4_cache *cache, size_t q_heads, size_t n_seqs,
                                                   size_t n_tokens, size_t max_new, size_t max_len) {
   (void)n_tokens;
+  if (max_len > kMaxLen) max_len = kMaxLen;  // as the call has it
   Kv4View v{};
   if (view_of(cache, &v) != KS_OK || !attention_sizes_ok(v, q_heads, n_seqs, max_new, max_len)) return 0;
   return attention_bytes(v, q_heads / v.kv_heads, n_seqs, max_new, max_len);
@@ -284,8 +285,8 @@ static size_t evict_bytes(const Kv4View &v, size_t n_seqs, size_t max_len, size_
 extern "C" size_t ks_b200_kv4_evict_workspace(const ks_b200_kv4_cache *cache, size_t n_seqs, size_t max_len,
                                               size_t budget) {
   Kv4View v{};
-  if (view_of(cache, &v) != KS_OK || n_seqs == 0 || n_seqs > 65535 || max_len == 0 || max_len > kMost || budget == 0 ||
-      budget > kMost)
+  if (max_len > kMaxLen) max_len = kMaxLen;  // as the call has it
+  if (view_of(cache, &v) != KS_OK || n_seqs == 0 || n_seqs > 65535 || max_len == 0 || budget == 0 || budget > kMost)
     return 0;
   return evict_bytes(v, n_seqs, max_len, budget);
 }
