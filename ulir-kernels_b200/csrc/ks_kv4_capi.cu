@@ -285,7 +285,7 @@ static size_t evict_bytes(const Kv4View &v, size_t n_seqs, size_t max_len, size_
 extern "C" size_t ks_b200_kv4_evict_workspace(const ks_b200_kv4_cache *cache, size_t n_seqs, size_t max_len,
                                               size_t budget) {
   Kv4View v{};
-  if (max_len > kMaxLen) max_len = kMaxLen;  // as the call has it
+  if (max_len > kMost) max_len = kMost;  // the call goes by kMaxLen, which is less
   if (view_of(cache, &v) != KS_OK || n_seqs == 0 || n_seqs > 65535 || max_len == 0 || budget == 0 || budget > kMost)
     return 0;
   return evict_bytes(v, n_seqs, max_len, budget);
