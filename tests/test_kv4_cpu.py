@@ -265,3 +265,15 @@ def test_workspaces_of_tables_beyond_31_bits(ks, call):
         need = ks.kv4_evict_workspace(c, 2, 2**31 - 16385, 32)
         assert ks.kv4_evict_workspace(c, 2, max_len, 32) >= need > 0
         assert call("evict", page_table_stride=stride, max_len=max_len, workspace_bytes=need - 1) == ks.KS_ERR_WORKSPACE
+
+
+def test_python_workspaces_are_contiguous(ks):
+    """One byte expanded to many is no workspace."""
+    torch = pytest.importorskip("torch")
+    c = ks.Kv4Cache(1 << 12, 40, 16, 2, 64, 32, weights=1 << 12)
+    table, lens, x = torch.zeros(2, 10, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(2, 2, 64)
+    for ws in (torch.zeros(1, dtype=torch.uint8).expand(1 << 20), torch.zeros(1 << 20, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match="contiguous"):
+            ks.kv4_attention_async(c, table, lens, x, x.clone(), 1.0, ws)
+        with pytest.raises(ValueError, match="contiguous"):
+            ks.kv4_evict_async(c, table, lens, table + 1, lens, 100, 40, 8, ws)

@@ -453,6 +453,12 @@ def _sequences(page_table, seq_lens, token_offsets=None):
     return stride, n_seqs, columns
 
 
+def _workspace(t):
+    if not t.is_contiguous():
+        raise ValueError("a workspace must be contiguous")
+    return t.data_ptr()
+
+
 def _bound(max_len, holds):
     """max_len, or what a row of the page table holds and it may not exceed."""
     if max_len is None:
@@ -536,7 +542,7 @@ def kv4_attention_async(cache, page_table, seq_lens, q, out, scale, workspace, t
     rc = lib().ks_b200_kv4_attention_async(
         cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), n_seqs, n_tokens,
         max_new, max_len, q.data_ptr(), qt, qh, q_heads, scale, out.data_ptr(), ot, oh, _DTYPES[q.dtype], _at(lse),
-        1 if accumulate else 0, workspace.data_ptr(), workspace.numel(), _at(status), stream_handle(stream))
+        1 if accumulate else 0, _workspace(workspace), workspace.numel(), _at(status), stream_handle(stream))
     if rc:
         check(rc)
 
@@ -562,7 +568,7 @@ def kv4_evict_async(cache, page_table, seq_lens, to_table, to_lens, max_len, bud
         raise ValueError("kept must be a contiguous int32 [n_seqs, kv_heads, budget]")
     rc = lib().ks_b200_kv4_evict_async(
         cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), n_seqs, max_len,
-        to_table.data_ptr(), to_stride, to_lens.data_ptr(), budget, recent, _at(kept), workspace.data_ptr(),
+        to_table.data_ptr(), to_stride, to_lens.data_ptr(), budget, recent, _at(kept), _workspace(workspace),
         workspace.numel(), _at(status), stream_handle(stream))
     if rc:
         check(rc)
