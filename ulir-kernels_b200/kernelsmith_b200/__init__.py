@@ -485,7 +485,7 @@ class Kv4Cache(ctypes.Structure):
                                           not _FLOAT32[weights.dtype] or not weights.is_contiguous()):
             raise ValueError("weights must be contiguous f32 [n_pages, kv_heads, page_size]")
         self._tensors = (pool, weights)
-        self._row = (kv_heads, head_dim)
+        self._row, self._page = (kv_heads, head_dim), page_size
         self._address = ctypes.addressof(self)
 
 
@@ -501,7 +501,7 @@ def _kv4_rows(call, cache, page_table, seq_lens, k, v, token_offsets, status, st
         raise ValueError("k and v must be [n_tokens, kv_heads, head_dim] of one type, the last dimension contiguous")
     stride, n_seqs, columns = _sequences(page_table, seq_lens, token_offsets)
     rc = call(cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), n_seqs,
-              shape[0], columns * cache.page_size, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DTYPES[k.dtype],
+              shape[0], columns * cache._page, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _DTYPES[k.dtype],
               _at(status), stream_handle(stream))
     if rc:
         check(rc)
@@ -538,7 +538,7 @@ def kv4_attention_async(cache, page_table, seq_lens, q, out, scale, workspace, t
         if token_offsets is not None:
             raise ValueError("token_offsets needs max_new, the most new tokens of a sequence")
         max_new = 1
-    max_len = _bound(max_len, columns * cache.page_size)
+    max_len = _bound(max_len, columns * cache._page)
     rc = lib().ks_b200_kv4_attention_async(
         cache._address, page_table.data_ptr(), stride, seq_lens.data_ptr(), _at(token_offsets), n_seqs, n_tokens,
         max_new, max_len, q.data_ptr(), qt, qh, q_heads, scale, out.data_ptr(), ot, oh, _DTYPES[q.dtype], _at(lse),
@@ -560,8 +560,8 @@ def kv4_evict_async(cache, page_table, seq_lens, to_table, to_lens, max_len, bud
     to_stride, to_seqs, to_columns = _sequences(to_table, to_lens)
     if to_seqs != n_seqs:
         raise ValueError("seq_lens and to_lens must be of one length")
-    max_len = _bound(max_len, columns * cache.page_size)
-    if to_columns * cache.page_size < min(budget, max_len):
+    max_len = _bound(max_len, columns * cache._page)
+    if to_columns * cache._page < min(budget, max_len):
         raise KernelSmithError(KS_ERR_INVALID_ARG, "a row of to_table holds fewer tokens than may be kept")
     if kept is not None and (kept.shape != (n_seqs, cache._row[0], budget) or not _INT32[kept.dtype] or
                              not kept.is_contiguous()):
