@@ -582,10 +582,12 @@ int ks_b200_import_ggml_q4_0_async(const void *blocks, size_t block_row_stride,
  *
  * Device pointers, queued on `stream`, no allocation, capturable.  status
  * word 0 becomes 1 if the device finds a length beyond the table (or
- * max_len), a page outside the pool, offsets outside n_tokens, more new
- * tokens than the sequence has or a key or value that is not finite (stored
- * as 0 if NaN, else as the largest code): no call reads or writes outside
- * its buffers then, the sequences concerned are unspecified.
+ * max_len), a page outside the pool where a token stands, offsets that fall or
+ * leave n_tokens, more new tokens than max_new (attention) or than the sequence
+ * has (append, read; to the attention those before position 0 see nothing), or
+ * a key or value that is not finite (stored as 0 if NaN, else as the largest
+ * code): no call reads or writes outside its buffers then, the sequences
+ * concerned are unspecified.  A call with n_tokens 0 does nothing.
  * A sequence has at most 2^31 - 16385 tokens, whatever max_len says.
  * head_dim must be 64 or 128, group_size 32, 64 or 128 and at most head_dim,
  * page_size 16, 32, 64, 128 or 256, else KS_ERR_UNSUPPORTED.

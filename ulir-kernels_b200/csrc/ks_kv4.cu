@@ -371,10 +371,11 @@ __device__ __forceinline__ void read_rows(const Kv4View &c, const Kv4Place *plac
 // One pass over what is read and written, with nothing shared between tokens:
 // four threads to a token's row, so that a warp's 16-byte pieces fill whole
 // sectors on both sides, keys and values in CTAs of their own.  19880 tokens,
-// 8 heads of 128, bf16, groups of 64: append 30 us (3.4 TB/s; the quantisation's
-// instructions bound it: quotients by a reciprocal, with one branch on
-// alignment to a row, took 8 us off), read 21 us (4.9 TB/s); 58000 tokens, f16:
-// read 57 us, 5.3 TB/s.
+// 8 heads of 128, bf16, groups of 64: append 30 us (3.4 TB/s; issued in 0.64 of the
+// cycles, the largest wait is for a row's loads, of which a thread has one row's
+// under way; quotients by a reciprocal, with one branch on alignment to a row, took
+// 8 us off), read 21 us (4.9 TB/s, two rows under way); 58000 tokens, f16: read
+// 57 us, 5.3 TB/s.
 // 64 tokens take 4 us, the latency of the lookup and of one row.
 template <typename T, int D, int NG, bool READ>
 __global__ void __launch_bounds__(kRowThreads, READ ? 4 : 3) kv4_rows_kernel(Kv4View c, Kv4Batch b, Kv4Rows r,

@@ -7,9 +7,9 @@
 //   key codes   16 rows of head_dim / 2 bytes
 //   key scales  16 rows of head_dim / group f16
 //   value codes, value scales likewise
-// in one piece, so that any run of tokens within a page arrives in shared
-// memory by a single bulk copy, and a block's keys alone by one too.  Codes
-// are the library's signed int4 (even element in the low half of its byte).
+// in one piece, so that any run of blocks within a page, and a block's keys
+// alone, are consecutive bytes, which arrive in shared memory by asynchronous
+// 16-byte copies.  Codes are the library's signed int4 (even element in the low half of its byte).
 // Within a row the bytes stand in the order in which the lanes of a warp feed
 // them to the tensor cores:
 //   keys    pair d, d+1 (d even) is byte (d%32/8) * (head_dim/8) + (d/32)*4 + d%8/2

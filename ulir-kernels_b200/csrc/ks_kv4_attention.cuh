@@ -11,8 +11,8 @@
 // (sequence, head, row tile, tokens) and every CTA of a grid that the GPU holds
 // at once takes an equal stretch of it, so that sequences of unequal lengths and
 // few long ones alike fill the GPU evenly.  An item's beginning counts as three units more,
-// about what it costs: 64 sequences of up to 8192 tokens, 8 heads, take 67 us
-// (70 before joins were made shorter, and then 98 without).  (Where few items
+// about what it costs: 64 sequences of up to 8192 tokens, 8 heads, take 69 us
+// (before joins were made shorter 70, and then 98 without).  (Where few items
 // give each CTA about one, it gets a part of one
 // item.)  Of an item (a row tile and all its tokens) that
 // a stretch ends within, each CTA leaves its part (maximum, sum, unnormalised
@@ -41,15 +41,22 @@
 // two, are only raised when a tile exceeds them (the maximum by 2^4), which a
 // vote finds: most tiles need no reduction over lanes and no rescaling.
 //
-// What bounds it.  Making the operands: about 260 instructions of a warp for 16
-// tokens of a head (f16, bf16; 128 elements) and 390 (f32), issued in 0.55 of
-// the cycles, half of them on the integer pipe, while the tensor cores are busy a
-// fifth of the time (which is why these are the warp-wide products, whose A
-// operand is made in registers: a tensor-memory operand would have to be stored
-// there first, and the products are not what takes the time).  444 equal
-// items of 4096 tokens, 128 elements, bf16: 54 us, 4.5 TB/s of codes and
-// scales with groups of 128, 61 us, 4.3 TB/s with groups of 32; f32 68 and 80 us,
-// 3.5 and 3.3 TB/s.  The copies without the products take 0.8 of the time.
+// What bounds it.  No unit is full; a warp's scores, vote, exponentials and value
+// products follow one another, and the three warps that a scheduler has (168
+// registers to a thread) do not fill each other's waits.  64 sequences of up to
+// 8192 tokens, 8 heads, bf16, groups of 64: 37.4 M warp instructions (275 for 16
+// tokens of a head, most of them widen codes), 32 us if every scheduler issued one
+// a cycle; they are issued in 0.54 of the cycles, the integer pipe is busy in 0.47,
+// the tensor cores in 0.25, DRAM in 0.48; 0.92 of a warp is ready in the mean, and
+// of a warp's waits the largest is for results of fixed latency.  For an eighth of
+// the time an SM has not begun or has no more work (16 sequences of up to 4096,
+// f32: for more than a quarter, 0.46 issued).  With few rows the products are not
+// what takes the time, which is why these are the warp-wide ones, whose A operand
+// is made in registers: a tensor-memory operand would have to be stored there
+// first.  444 equal items of 4096 tokens, 128 elements, bf16: 46 us, 5.2 TB/s of
+// codes and scales with groups of 128, 57 us, 4.6 TB/s with groups of 32; f16 52 and
+// 65, f32 60 and 75 us, 4.0 and 3.5 TB/s.  The copies without the products take 0.8
+// of the time.
 // A call's beginning (the lengths, the queries) and end (the four warps' sums,
 // the join of an item's parts) take 8 us together, which is what short calls
 // take.
@@ -121,7 +128,9 @@ struct Kv4AttnArgs {
 
 // CTAs of a pass that an SM holds, bounded by registers: 168 a thread, 255 with
 // NT 2.  (Four CTAs of 128 registers, tiles of two blocks, f16 and bf16: the same
-// time per item over 148 sequences of 4096 tokens, 4 heads.)
+// time per item over 148 sequences of 4096 tokens, 4 heads.)  With 128 elements some
+// kernels have more than fits and spill: f32 156 bytes a thread (groups of 64, NT 1),
+// 148 (groups of 32, NT 2), 28 (groups of 32, NT 1), others and f16 up to 8.
 constexpr int kv4_ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
 
 // Partial results of CTA c: rows_tile x head_dim f32, then rows_tile maxima
