@@ -277,3 +277,9 @@ def test_python_workspaces_are_contiguous(ks):
             ks.kv4_attention_async(c, table, lens, x, x.clone(), 1.0, ws)
         with pytest.raises(ValueError, match="contiguous"):
             ks.kv4_evict_async(c, table, lens, table + 1, lens, 100, 40, 8, ws)
+
+
+@pytest.mark.parametrize("name", ["attention", "evict"])
+def test_the_largest_max_len_is_refused(ks, call, name):
+    for bad in (129, 2**31, 2**63, 2**64 - 1):
+        assert call(name, max_len=bad) == ks.KS_ERR_INVALID_ARG, bad

@@ -61,11 +61,9 @@ int view_of(const ks_b200_kv4_cache *c, Kv4View *v) {
   return KS_OK;
 }
 
-// max_len kTableHolds: what a row of the table holds.
-constexpr size_t kTableHolds = ~(size_t)0;
-
+// max_len null: what a row of the table holds.
 int batch_of(const Kv4View &v, const int32_t *page_table, size_t stride, const int32_t *seq_lens,
-             const int32_t *offsets, size_t n_seqs, size_t n_tokens, size_t max_len, Kv4Batch *b) {
+             const int32_t *offsets, size_t n_seqs, size_t n_tokens, const size_t *max_len, Kv4Batch *b) {
   if (!page_table || !seq_lens) return fail(KS_ERR_INVALID_ARG, "NULL pointer");
   if (n_seqs == 0 || stride == 0) return fail(KS_ERR_INVALID_ARG, "n_seqs and the table's stride must be > 0");
   if (!offsets && n_tokens != n_seqs)
@@ -75,16 +73,15 @@ int batch_of(const Kv4View &v, const int32_t *page_table, size_t stride, const i
   if (n_seqs > 65535 || n_tokens > kMost || stride > kMost)
     return fail(KS_ERR_UNSUPPORTED, "at most 65535 sequences, 2^31 - 1 tokens and table entries");
   const size_t holds = stride << v.page_shift;
-  if (max_len == kTableHolds) max_len = holds;
-  if (max_len > holds) return fail(KS_ERR_INVALID_ARG, "max_len is more than a row of the page table holds");
-  if (max_len > kMaxLen) max_len = kMaxLen;
+  const size_t most = max_len ? *max_len : holds;
+  if (most > holds) return fail(KS_ERR_INVALID_ARG, "max_len is more than a row of the page table holds");
   b->table = page_table;
   b->table_stride = (int64_t)stride;
   b->lens = seq_lens;
   b->offsets = offsets;
   b->n_seqs = (int)n_seqs;
   b->n_tokens = (int)n_tokens;
-  b->max_len = (int)max_len;
+  b->max_len = (int)(most < kMaxLen ? most : kMaxLen);
   return KS_OK;
 }
 
@@ -142,8 +139,8 @@ extern "C" size_t ks_b200_kv4_page_bytes(size_t page_size, size_t kv_heads, size
 namespace {
 
 int rows_call(bool append, const ks_b200_kv4_cache *cache, const int32_t *page_table, size_t page_table_stride,
-              const int32_t *seq_lens, const int32_t *token_offsets, size_t n_seqs, size_t n_tokens, size_t max_len,
-              void *k, size_t k_token_stride, size_t k_head_stride, void *v, size_t v_token_stride,
+              const int32_t *seq_lens, const int32_t *token_offsets, size_t n_seqs, size_t n_tokens,
+              const size_t *max_len, void *k, size_t k_token_stride, size_t k_head_stride, void *v, size_t v_token_stride,
               size_t v_head_stride, int dtype, uint32_t *status, void *stream) {
   Kv4View view{};
   Kv4Batch b;
@@ -153,7 +150,7 @@ int rows_call(bool append, const ks_b200_kv4_cache *cache, const int32_t *page_t
       KS_OK)
     return rc;
   if (n_tokens == 0) return KS_OK;
-  if (max_len == 0) return fail(KS_ERR_INVALID_ARG, "max_len must be > 0");
+  if (max_len && *max_len == 0) return fail(KS_ERR_INVALID_ARG, "max_len must be > 0");
   if ((rc = rows_ok(k, n_tokens, k_token_stride, cache->kv_heads, k_head_stride, cache->head_dim, dtype, !append)) !=
           KS_OK ||
       (rc = rows_ok(v, n_tokens, v_token_stride, cache->kv_heads, v_head_stride, cache->head_dim, dtype, !append)) !=
@@ -174,7 +171,7 @@ extern "C" int ks_b200_kv4_append_async(const ks_b200_kv4_cache *cache, const in
                                         size_t k_token_stride, size_t k_head_stride, const void *v,
                                         size_t v_token_stride, size_t v_head_stride, int dtype, uint32_t *status,
                                         void *stream) {
-  return rows_call(true, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, kTableHolds,
+  return rows_call(true, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, nullptr,
                    const_cast<void *>(k), k_token_stride, k_head_stride, const_cast<void *>(v), v_token_stride,
                    v_head_stride, dtype, status, stream);
 }
@@ -185,8 +182,7 @@ extern "C" int ks_b200_kv4_append_bounded_async(const ks_b200_kv4_cache *cache, 
                                                 size_t max_len, const void *k, size_t k_token_stride,
                                                 size_t k_head_stride, const void *v, size_t v_token_stride,
                                                 size_t v_head_stride, int dtype, uint32_t *status, void *stream) {
-  if (max_len == kTableHolds) return fail(KS_ERR_INVALID_ARG, "max_len is more than a row of the page table holds");
-  return rows_call(true, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, max_len,
+  return rows_call(true, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, &max_len,
                    const_cast<void *>(k), k_token_stride, k_head_stride, const_cast<void *>(v), v_token_stride,
                    v_head_stride, dtype, status, stream);
 }
@@ -196,7 +192,7 @@ extern "C" int ks_b200_kv4_read_async(const ks_b200_kv4_cache *cache, const int3
                                       const int32_t *token_offsets, size_t n_seqs, size_t n_tokens, void *k,
                                       size_t k_token_stride, size_t k_head_stride, void *v, size_t v_token_stride,
                                       size_t v_head_stride, int dtype, uint32_t *status, void *stream) {
-  return rows_call(false, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, kTableHolds,
+  return rows_call(false, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, nullptr,
                    k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype, status, stream);
 }
 
@@ -206,8 +202,7 @@ extern "C" int ks_b200_kv4_read_bounded_async(const ks_b200_kv4_cache *cache, co
                                               size_t max_len, void *k, size_t k_token_stride, size_t k_head_stride,
                                               void *v, size_t v_token_stride, size_t v_head_stride, int dtype,
                                               uint32_t *status, void *stream) {
-  if (max_len == kTableHolds) return fail(KS_ERR_INVALID_ARG, "max_len is more than a row of the page table holds");
-  return rows_call(false, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, max_len, k,
+  return rows_call(false, cache, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, &max_len, k,
                    k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype, status, stream);
 }
 
@@ -233,7 +228,7 @@ extern "C" int ks_b200_kv4_attention_async(const ks_b200_kv4_cache *cache, const
   if ((rc = view_of(cache, &k.c)) != KS_OK) return rc;
   if (max_new == 0 || max_len == 0 || max_new > max_len)
     return fail(KS_ERR_INVALID_ARG, "max_new and max_len must be > 0, max_new <= max_len");
-  if ((rc = batch_of(k.c, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, max_len, &k.b)) !=
+  if ((rc = batch_of(k.c, page_table, page_table_stride, seq_lens, token_offsets, n_seqs, n_tokens, &max_len, &k.b)) !=
       KS_OK)
     return rc;
   if (q_heads == 0 || q_heads % k.c.kv_heads)
@@ -301,7 +296,7 @@ extern "C" int ks_b200_kv4_evict_async(const ks_b200_kv4_cache *cache, const int
   int rc;
   if ((rc = view_of(cache, &v)) != KS_OK) return rc;
   if (max_len == 0) return fail(KS_ERR_INVALID_ARG, "max_len must be > 0");
-  if ((rc = batch_of(v, page_table, page_table_stride, seq_lens, nullptr, n_seqs, n_seqs, max_len, &b)) != KS_OK)
+  if ((rc = batch_of(v, page_table, page_table_stride, seq_lens, nullptr, n_seqs, n_seqs, &max_len, &b)) != KS_OK)
     return rc;
   if (!cache->weights) return fail(KS_ERR_INVALID_ARG, "eviction needs cache->weights");
   if (!to_table || !to_lens) return fail(KS_ERR_INVALID_ARG, "NULL pointer");
