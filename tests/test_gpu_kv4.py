@@ -1240,3 +1240,101 @@ def test_append_from_most_rows(ks, cuda):
     assert status.tolist() == [0, 0]
     want = O.kv4_value(*O.kv4_quantize(x[0].double().cpu().numpy(), 64))
     assert (back.double().cpu().numpy() == want).all()
+
+
+@pytest.mark.parametrize("heads", [65, 130])
+def test_more_heads_than_a_turn_of_a_cta(ks, cuda, heads):
+    """Append and read, attention with weights and eviction with more heads than a CTA has rows under way."""
+    import torch
+
+    d, group, page = 64, 64, 16
+    c = Seqs(ks, cuda, [40, 7, 19], [5, 7, 1], heads, d, group, page, weights=True, garbage=False)
+    x = torch.randn(2, c.tokens, heads, d, device=cuda)
+    ks.kv4_append_async(c.cache, c.table, c.seq_lens, x[0], x[1], token_offsets=c.offsets, status=c.status)
+    back = torch.zeros_like(x)
+    ks.kv4_read_async(c.cache, c.table, c.seq_lens, back[0], back[1], token_offsets=c.offsets, status=c.status)
+    c.ok()
+    want = O.kv4_value(*O.kv4_quantize(x.double().cpu().numpy(), group))
+    assert (back.double().cpu().numpy() == want).all()
+    for s in range(3):
+        for j in range(c.news[s]):
+            pos = c.lens[s] - c.news[s] + j
+            c.k[c.pages[s][pos // page], :, pos % page] = want[0, c.first[s] + j]
+            c.v[c.pages[s][pos // page], :, pos % page] = want[1, c.first[s] + j]
+    c.scale_max = max(c.scale_max, np.abs(want[0]).max() / 7)
+    before = c.w.double().cpu().numpy()
+    q = _query(c, heads, "f32")
+    out, lse = _attend(c, q, 0.125, accumulate=True)
+    c.ok()
+    _check(c, q, 0.125, out, lse, "f32", weights=c.w, before=before)
+    _, _, _, _, _, to_lens, kept, keep = _evict(c, 12, 3)
+    c.ok()
+    w = c.w.cpu().numpy()
+    assert to_lens.tolist() == keep
+    for s in range(3):
+        for h in range(heads):
+            assert kept[s, h, : keep[s]].tolist() == _kept_of(c.weights_of(s, w)[h], c.lens[s], 12, 3).tolist()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,group,q_heads,heads,lens,news", [
+    (64, 32, 128, 1, [50, 300], [1, 1]),  # one key/value head for all
+    (128, 64, 142, 2, [77, 9], [1, 2]),
+    (64, 64, 2, 1, [300, 40], [300, 1]),  # a prompt from its first token, beside a decode row
+    (128, 128, 1, 1, [500], [213]),
+])
+def test_many_rows_to_a_head(ks, cuda, dtype, d, group, q_heads, heads, lens, news):
+    c = Seqs(ks, cuda, lens, news, heads, d, group, 32, seed=q_heads, weights=True)
+    before = c.w.double().cpu().numpy()
+    big = _query(c, q_heads + 1, dtype).reshape(c.tokens, -1)  # rows that start at any element
+    q = big[:, 1:1 + q_heads * d].unflatten(1, (q_heads, d))
+    out, lse = _attend(c, q, d**-0.5, accumulate=True)
+    c.ok()
+    _check(c, q, d**-0.5, out, lse, dtype, weights=c.w, before=before)
+
+
+def test_thousands_of_sequences(ks, cuda):
+    lens = [int(x) for x in np.random.default_rng(0).integers(0, 4, 5000)]
+    c = Seqs(ks, cuda, lens, [min(x, 1) for x in lens], 1, 64, 64, 16, weights=True, spare=3)
+    before = c.w.double().cpu().numpy()
+    q = _query(c, 2, "f32")
+    out, lse = _attend(c, q, 0.125, accumulate=True)
+    c.ok()
+    _check(c, q, 0.125, out, lse, "f32", weights=c.w, before=before)
+
+
+def test_a_captured_step_follows_its_offsets(ks, cuda):
+    """Drafted tokens in a graph: how many each sequence has, and where its rows are, changes between replays."""
+    import torch
+
+    heads, q_heads, d, group, page, rows = 2, 6, 64, 32, 16, 12
+    c = Seqs(ks, cuda, [96, 80, 48], [4, 4, 4], heads, d, group, page, garbage=False)  # pages for what comes
+    x = torch.randn(2, rows, heads, d, device=cuda)
+    q = torch.randn(rows, q_heads, d, device=cuda)
+    out, lse = torch.zeros_like(q), torch.zeros(rows, q_heads, device=cuda)
+    ws = torch.zeros(ks.kv4_attention_workspace(c.cache, q_heads, 3, rows, 8, 96), dtype=torch.uint8, device=cuda)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=stream):
+        ks.kv4_append_async(c.cache, c.table, c.seq_lens, x[0], x[1], token_offsets=c.offsets, status=c.status,
+                            stream=stream)
+        ks.kv4_attention_async(c.cache, c.table, c.seq_lens, q, out, 0.125, ws, token_offsets=c.offsets, max_new=8,
+                               max_len=96, lse=lse, status=c.status, stream=stream)
+    values = O.kv4_value(*O.kv4_quantize(x.double().cpu().numpy(), group))
+    for news, first, lens in (([4, 4, 4], 0, [90, 64, 33]), ([1, 8, 0], 2, [91, 70, 33]), ([0, 1, 1], 10, [91, 71, 34])):
+        c.lens, c.news, c.first = lens, news, first + np.concatenate([[0], np.cumsum(news)]).astype(int)
+        c.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        c.offsets.copy_(torch.tensor(c.first, dtype=torch.int32))
+        out.fill_(7)
+        g.replay()
+        c.ok()
+        for s in range(3):
+            for j in range(news[s]):
+                pos = lens[s] - news[s] + j
+                c.k[c.pages[s][pos // page], :, pos % page] = values[0, c.first[s] + j]
+                c.v[c.pages[s][pos // page], :, pos % page] = values[1, c.first[s] + j]
+        c.scale_max = max(c.scale_max, np.abs(values[0]).max() / 7)
+        _check(c, q, 0.125, out, lse, "f32")
+        assert (out[:first] == 7).all() and (out[c.first[-1]:] == 7).all()
+    del g
