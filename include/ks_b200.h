@@ -664,7 +664,7 @@ int ks_b200_kv4_read_bounded_async(const ks_b200_kv4_cache *cache,
  * A row that sees nothing gets zeros and lse -inf.  Sums are f32.  For f32
  * tensors the products keep queries to 2^-23 of their row's largest element and
  * 22 bits of probabilities times value scales, so results agree with f32
- * arithmetic; for f16 and bf16 tensors queries to 2^-35 of it and 22 and 11 bits
+ * arithmetic; for f16 and bf16 tensors queries to 2^-35 of it and 20 and 11 bits
  * of the latter.  Queries are finite and below 2^110.  lse: f32
  * [n_tokens][q_heads], or NULL.  accumulate != 0 adds to cache->weights of
  * every cached token the attention weight it received, summed over the

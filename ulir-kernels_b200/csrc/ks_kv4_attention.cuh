@@ -76,12 +76,14 @@
 // 64 sequences of up to 8192, this 1 %).
 // A weight (probability times value scale) has its parts' last bit at 2^-24,
 // where the largest value scale stands at 2^10: 22 bits for scales down to 2^-11
-// of that.  Once a warp meets a smaller one, in any token or group, it goes on in
-// a second form of the loop, where the largest weight of each tile, row and group
-// is brought to 2^13 and each tile's product is added in f32: a result far below
-// values that have next to no weight in it keeps its bits (without, it lost all of
-// them from 2^-36 on).  Looking for such a scale takes 1 to 3 % (64 sequences of
-// up to 8192, bf16: 68.6 -> 69.4 us; 16 of up to 4096, f32: 21.7 -> 22.2).
+// of that.  Once a warp meets a smaller one, in any token or group (f16 results:
+// 2^-14, bf16: 2^-15), it goes on in a second form of the loop, where the largest
+// weight of each tile, row and group is brought to 2^13 and each tile's product is
+// added in f32: a result far below values that have next to no weight in it keeps
+// its bits (without, it lost all of them from 2^-36 on).  The second form takes 1.2
+// times as long with groups of 128, twice as long with groups of 32.  Looking for
+// such a scale takes 1 to 3 % (64 sequences of up to 8192, bf16: 68.6 -> 69.4 us;
+// 16 of up to 4096, f32: 21.7 -> 22.2).
 #pragma once
 
 #include <atomic>
@@ -716,10 +718,11 @@ __global__ void __launch_bounds__(kAttnThreads, kv4_ctas_per_sm(NT)) kv4_attenti
       }
       float lift = 0.0f;
       __half2 scale_limit = __floats2half2_rn(0.0f, 0.0f);  // value scales up to this one fit
-      // The least value scale so far (a lane's own).  Below 2^-11 of the limit its weights would lose bits: from there on
-      // each tile's weights have a power of two of their own (apart).
+      // The least value scale so far (a lane's own).  So far below the limit that its weights would lose bits that a result
+      // of this type shows, each tile's weights have a power of two of their own (apart) from there on.
       __half2 least = __floats2half2_rn(INFINITY, INFINITY);
-      auto too_small = [&] { return !__hbge2(__hmul2(least, __floats2half2_rn(2048.0f, 2048.0f)), scale_limit); };
+      constexpr float kApartFrom = QS == 2 ? 0x1p11f : PS == 2 ? 0x1p14f : 0x1p15f;
+      auto too_small = [&] { return !__hbge2(__hmul2(least, __floats2half2_rn(kApartFrom, kApartFrom)), scale_limit); };
 
       // Sums of the tiles before, in units of 2^folded_base (volatile: in local memory, the registers are taken), and their
       // factor in units of 2^base, which has only risen.
